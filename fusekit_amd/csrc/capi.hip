@@ -976,6 +976,77 @@ fk_status fk_xcd_kslice_meta(const uint16_t* src, uint32_t n, uint32_t groups, u
     return xcd_kslice_meta(src, n, groups, dst, (hipStream_t)s);
 }
 
+// ---- several sequences over a paged cache; beam search ----
+fk_status fk_rope_frequencies(uint32_t dims, double theta, int scaling, double factor, double low, double high, uint32_t trained,
+                              double* d_freq, fk_stream s) {
+    Launch l;
+    FK_TRY(plan_rope_frequencies(dims, theta, scaling, factor, low, high, trained, d_freq, &l));
+    return run_launch(l, (hipStream_t)s);
+}
+
+fk_status fk_rope_paged_store(const uint16_t* q, uint32_t q_stride, const uint16_t* k, uint32_t k_stride, const uint16_t* v,
+                              uint32_t v_stride, uint16_t* q_out, uint32_t q_out_stride, uint32_t n_heads, const uint16_t* q_norm,
+                              const uint16_t* k_norm, float eps, uint32_t rope_dims, int interleaved, const double* d_freq,
+                              const fk_paged_batch* batch, const fk_page_pool* pool, fk_stream s) {
+    Launch l;
+    FK_TRY(plan_rope_paged_store(q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, n_heads, q_norm, k_norm, eps, rope_dims, interleaved,
+                                 d_freq, batch, pool, &l));
+    return run_launch(l, (hipStream_t)s);
+}
+
+fk_status fk_sdpa_paged_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t n_seqs, uint32_t rows, uint32_t max_len,
+                                        size_t* bytes) {
+    return sdpa_paged_workspace_bytes(n_heads, n_kv, head_dim, n_seqs, rows, max_len, bytes);
+}
+
+fk_status fk_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, uint32_t out_stride, uint32_t n_heads, float scale, float softcap,
+                        uint32_t window, const fk_paged_batch* batch, const fk_page_pool* pool, void* workspace, size_t workspace_bytes,
+                        fk_stream s) {
+    Launch l;
+    FK_TRY(plan_sdpa_paged(q, q_stride, out, out_stride, n_heads, scale, softcap, window, batch, pool, workspace, workspace_bytes, &l));
+    return run_launch(l, (hipStream_t)s);
+}
+
+fk_status fk_paged_check(uint32_t* fault, fk_stream s) {
+    if (!fault || (uintptr_t)fault & 3u) return set_error(FK_ERR_INVALID, "fk_paged_check: null or misaligned fault word");
+    FK_HIP(hipStreamSynchronize((hipStream_t)s));
+    uint32_t bits = 0;
+    FK_HIP(hipMemcpy(&bits, fault, 4, hipMemcpyDeviceToHost));
+    if (!bits) return FK_OK;
+    const uint32_t zero = 0;
+    FK_HIP(hipMemcpy(fault, &zero, 4, hipMemcpyHostToDevice));
+    std::string m = "paged cache:";
+    if (bits & FK_PAGED_BAD_ROWS) m += " row_start falls or exceeds the launch's rows;";
+    if (bits & FK_PAGED_BAD_LENGTH) m += " a length above max_len or below the sequence's new rows;";
+    if (bits & FK_PAGED_BAD_PAGE) m += " a page id that the pool does not have;";
+    return set_error(FK_ERR_INVALID, m);
+}
+
+fk_status fk_pages_copy(void* base, uint32_t n_planes, size_t plane_stride, uint32_t n_pages, size_t page_bytes, const uint32_t* pairs,
+                        uint32_t n_pairs, fk_stream s) {
+    return run_pages_copy(base, n_planes, plane_stride, n_pages, page_bytes, pairs, n_pairs, (hipStream_t)s);
+}
+
+fk_status fk_beam_select_workspace_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k, size_t* bytes) {
+    return beam_select_workspace_bytes(groups, beams, vocab, k, bytes);
+}
+
+fk_status fk_beam_select(const uint16_t* logits, size_t row_stride, const float* scores, const uint32_t* finished, uint32_t pad_token,
+                         uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k, float* out_scores, uint32_t* out_beams,
+                         uint32_t* out_tokens, void* workspace, size_t workspace_bytes, fk_stream s) {
+    Launch l;
+    FK_TRY(plan_beam_select(logits, row_stride, scores, finished, pad_token, groups, beams, vocab, k, out_scores, out_beams, out_tokens, workspace,
+                            workspace_bytes, &l));
+    return run_launch(l, (hipStream_t)s);
+}
+
+fk_status fk_beam_reorder(const void* src, void* dst, size_t row_bytes, const uint32_t* parents, uint32_t groups, uint32_t beams, uint32_t n_out,
+                          fk_stream s) {
+    Launch l;
+    FK_TRY(plan_beam_reorder(src, dst, row_bytes, parents, groups, beams, n_out, &l));
+    return run_launch(l, (hipStream_t)s);
+}
+
 fk_status fk_xcd_check(void* workspace, fk_stream s) {
     if (!workspace) return set_error(FK_ERR_INVALID, "fk_xcd_check: null workspace");
     FK_HIP(hipStreamSynchronize((hipStream_t)s));

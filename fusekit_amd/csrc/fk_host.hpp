@@ -395,6 +395,26 @@ fk_status plan_rmsnorm_rows(const uint16_t* x, const uint16_t* w, float eps, uin
 constexpr size_t kArgmaxWorkspaceBytes = 8 + 8 * 160;
 fk_status plan_argmax(const uint16_t* logits, uint32_t n, uint32_t* next_token, uint32_t* history,
                       uint32_t* hist_counter, uint32_t hist_capacity, void* workspace, Launch* out);
+// ---- several sequences over a paged cache; beam search (each refuses bad arguments before it looks for a device) ----
+fk_status plan_rope_frequencies(uint32_t dims, double theta, int scaling, double factor, double low, double high, uint32_t trained,
+                                double* freq, Launch* out);
+fk_status plan_rope_paged_store(const uint16_t* q, uint32_t q_stride, const uint16_t* k, uint32_t k_stride, const uint16_t* v,
+                                uint32_t v_stride, uint16_t* q_out, uint32_t q_out_stride, uint32_t n_heads, const uint16_t* q_norm,
+                                const uint16_t* k_norm, float eps, uint32_t rope_dims, int interleaved, const double* freq,
+                                const fk_paged_batch* batch, const fk_page_pool* pool, Launch* out);
+fk_status sdpa_paged_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t n_seqs, uint32_t rows, uint32_t max_len,
+                                     size_t* bytes);
+fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, uint32_t out_stride, uint32_t n_heads, float scale,
+                          float softcap, uint32_t window, const fk_paged_batch* batch, const fk_page_pool* pool, void* workspace,
+                          size_t workspace_bytes, Launch* launch);
+fk_status run_pages_copy(void* base, uint32_t n_planes, size_t plane_stride, uint32_t n_pages, size_t page_bytes, const uint32_t* pairs,
+                         uint32_t n_pairs, hipStream_t s);
+fk_status beam_select_workspace_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k, size_t* bytes);
+fk_status plan_beam_select(const uint16_t* logits, size_t row_stride, const float* scores, const uint32_t* finished, uint32_t pad_token,
+                           uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k, float* out_scores, uint32_t* out_beams,
+                           uint32_t* out_tokens, void* workspace, size_t workspace_bytes, Launch* out);
+fk_status plan_beam_reorder(const void* src, void* dst, size_t row_bytes, const uint32_t* parents, uint32_t groups, uint32_t beams,
+                            uint32_t n_out, Launch* out);
 fk_status plan_step_init(uint32_t* step_counter, uint32_t* offset, uint32_t* kv_len, Launch* out,
                          float* rope_tab = nullptr, uint32_t rope_dims = 0, float base_log2 = 0.f);
 fk_status plan_fill_u32(void* p, uint32_t value, size_t count, Launch* out);

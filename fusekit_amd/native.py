@@ -639,6 +639,95 @@ def xcd_check(workspace, stream=None) -> None:
     check(lib.fk_xcd_check(_addr(workspace), _addr(stream)))
 
 
+# ---------------------------------------------------------------- several sequences over a paged cache; beam search
+
+class PagePool(C.Structure):
+    """fk_page_pool: one layer's pages, k and v bf16 [n_pages, n_kv, page_rows, head_dim]."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("n_pages", C.c_uint32), ("page_rows", C.c_uint32), ("n_kv", C.c_uint32),
+                ("head_dim", C.c_uint32)]
+
+    def __init__(self, k, v, n_pages, page_rows, n_kv, head_dim):
+        super().__init__(_addr(k), _addr(v), n_pages, page_rows, n_kv, head_dim)
+
+
+class PagedBatch(C.Structure):
+    """fk_paged_batch: row_start [n_seqs + 1], kv_len [n_seqs] and page_table [n_seqs, table_stride], uint32 in device memory; what
+    a launch is sized for (rows of the buffers, new rows and positions of a sequence at most) as numbers."""
+    _fields_ = [("row_start", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p), ("table_stride", C.c_uint32),
+                ("n_seqs", C.c_uint32), ("rows", C.c_uint32), ("max_rows", C.c_uint32), ("max_len", C.c_uint32), ("fault", C.c_void_p)]
+
+    def __init__(self, row_start, kv_len, page_table, table_stride, n_seqs, rows, max_rows, max_len, fault=None):
+        super().__init__(_addr(row_start), _addr(kv_len), _addr(page_table), table_stride, n_seqs, rows, max_rows, max_len, _addr(fault))
+
+
+ROPE_SCALINGS = {"plain": 0, "linear": 1, "parts": 2, "ramp": 3}
+
+
+def rope_frequencies(dims, theta, freq, scaling="plain", factor=1.0, low=0.0, high=0.0, trained=0, stream=None):
+    """Revolutions a position of every rotary pair and the factor of cos and sin, dims / 2 + 1 doubles (fk_rope_frequencies)."""
+    check(lib.fk_rope_frequencies(dims, theta, ROPE_SCALINGS[scaling], factor, low, high, trained, _addr(freq), _addr(stream)))
+
+
+def rope_paged_store(q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, n_heads, q_norm, k_norm, eps, rope_dims, interleaved,
+                     freq, batch: PagedBatch, pool: PagePool, stream=None):
+    """Rotary positions of q and k, and k and v into the sequences' pages (fk_rope_paged_store)."""
+    check(lib.fk_rope_paged_store(_addr(q), q_stride, _addr(k), k_stride, _addr(v), v_stride, _addr(q_out), q_out_stride, n_heads,
+                                  _addr(q_norm), _addr(k_norm), eps, rope_dims, interleaved, _addr(freq), batch, pool, _addr(stream)))
+
+
+def sdpa_paged_workspace_bytes(n_heads, n_kv, head_dim, n_seqs, rows, max_len) -> int:
+    out = C.c_size_t()
+    check(lib.fk_sdpa_paged_workspace_bytes(n_heads, n_kv, head_dim, n_seqs, rows, max_len, C.byref(out)))
+    return out.value
+
+
+def sdpa_paged(q, q_stride, out, out_stride, n_heads, scale, softcap, window, batch: PagedBatch, pool: PagePool, workspace,
+               workspace_bytes, stream=None):
+    """Attention of a batch's new rows, chunks and single tokens, over its pages (fk_sdpa_paged)."""
+    check(lib.fk_sdpa_paged(_addr(q), q_stride, _addr(out), out_stride, n_heads, scale, softcap, window, batch, pool, _addr(workspace),
+                            workspace_bytes, _addr(stream)))
+
+
+def paged_check(fault, stream=None) -> None:
+    """Waits for the stream; InvalidArgument where a launch met a bad row, length or page (fk_paged_check)."""
+    check(lib.fk_paged_check(_addr(fault), _addr(stream)))
+
+
+def pages_copy(base, n_planes, plane_stride, n_pages, page_bytes, pairs, stream=None) -> None:
+    """Page pairs[i][0] to page pairs[i][1] in every plane of a pool (fk_pages_copy); pairs: host numbers [n, 2]."""
+    p = pairs if pairs.__class__ is np.ndarray and pairs.dtype == np.uint32 and pairs.flags.c_contiguous else _page_pairs(pairs)
+    if p.ndim != 2 or p.shape[1] != 2:
+        raise InvalidArgument(FK_ERR_INVALID, "pages_copy: pairs must be [n, 2]")
+    check(lib.fk_pages_copy(_addr(base), n_planes, plane_stride, n_pages, page_bytes, p.ctypes.data, p.shape[0], _addr(stream)))
+
+
+def _page_pairs(pairs) -> np.ndarray:
+    p = np.asarray(pairs)
+    if p.size == 0:
+        return np.zeros((0, 2), np.uint32)
+    if p.dtype.kind not in "iu" or p.min() < 0 or p.max() > 0xFFFFFFFF:
+        raise InvalidArgument(FK_ERR_INVALID, "pages_copy: pairs must be page ids")
+    return np.ascontiguousarray(p, dtype=np.uint32)
+
+
+def beam_select_workspace_bytes(groups, beams, vocab, k) -> int:
+    out = C.c_size_t()
+    check(lib.fk_beam_select_workspace_bytes(groups, beams, vocab, k, C.byref(out)))
+    return out.value
+
+
+def beam_select(logits, row_stride, scores, finished, pad_token, groups, beams, vocab, k, out_scores, out_beams, out_tokens, workspace,
+                workspace_bytes, stream=None):
+    """The k best continuations of each group's beams (fk_beam_select)."""
+    check(lib.fk_beam_select(_addr(logits), row_stride, _addr(scores), _addr(finished), pad_token, groups, beams, vocab, k,
+                             _addr(out_scores), _addr(out_beams), _addr(out_tokens), _addr(workspace), workspace_bytes, _addr(stream)))
+
+
+def beam_reorder(src, dst, row_bytes, parents, groups, beams, n_out, stream=None):
+    """dst[g, i] = src[g, parents[g, i]], rows of row_bytes (fk_beam_reorder); dst may be src where n_out == beams."""
+    check(lib.fk_beam_reorder(_addr(src), _addr(dst), row_bytes, _addr(parents), groups, beams, n_out, _addr(stream)))
+
+
 def copy(dst, src, nbytes, stream=None):
     check(lib.fk_copy(_ptr(dst), _ptr(src), C.c_size_t(nbytes), _ptr(stream)))
 
@@ -715,7 +804,8 @@ class Event:
 
 # Argument types of the operators, declared once: ctypes converts plain numbers and addresses in C, and a call does not build an
 # object for each (rmsnorm + q / k / v, thirteen arguments: 6.4 us a call with the objects, 5.4 without; a launch
-# alone takes 4.0).  p an address, W an fk_weight, Q a quantised cache, u / i / f a 32-bit number.
+# alone takes 4.0).  p an address, W an fk_weight, Q a quantised cache, B / P a paged batch / pool, u / i / f a 32-bit number, d a
+# 64-bit one, z a size.
 _SIGNATURES = {
     "fk_qgemv": "Wpppp", "fk_linear_residual": "Wppppp", "fk_rmsnorm_qkv": "ppfWWWppppppp",
     "fk_gateup_swiglu_rows": "pupfWWipp", "fk_rmsnorm_qkv_rows": "puupfWWWpupupup", "fk_gateup_swiglu": "ppfWWipp",
@@ -734,9 +824,13 @@ _SIGNATURES = {
     "fk_set_gemm_library_rows": "u", "fk_embed_lookup_decode": "Wpufpp", "fk_argmax_logits_decode": "pupppupp",
     "fk_step_init": "pppp", "fk_step_init_rope": "ppppufp", "fk_rope_store_sdpa_decode": "pppppppppuuuuuuffufpppp",
     "fk_xcd_kslice_meta": "puupp", "fk_xcd_check": "pp", "fk_route_order": "puupp", "fk_set_gemv_policy": "uu",
+    "fk_rope_frequencies": "udidddupp", "fk_rope_paged_store": "pupupupuuppfuipBPp", "fk_sdpa_paged_workspace_bytes": "uuuuuup",
+    "fk_sdpa_paged": "pupuuffuBPpzp", "fk_paged_check": "pp", "fk_pages_copy": "puzuzpup", "fk_beam_select_workspace_bytes": "uuuup",
+    "fk_beam_select": "pzppuuuuuppppzp", "fk_beam_reorder": "ppzpuuup",
     "fk_set_qgemm_wide": "i", "fk_set_gemv_flat_only": "i", "fk_stream_sync": "p",
 }
 
-_TYPES = {"p": C.c_void_p, "W": C.POINTER(Weight), "Q": C.POINTER(_KvQuantCache), "u": C.c_uint32, "i": C.c_int, "f": C.c_float}
+_TYPES = {"p": C.c_void_p, "W": C.POINTER(Weight), "Q": C.POINTER(_KvQuantCache), "u": C.c_uint32, "i": C.c_int, "f": C.c_float,
+          "B": C.POINTER(PagedBatch), "P": C.POINTER(PagePool), "d": C.c_double, "z": C.c_size_t}
 for _name, _signature in _SIGNATURES.items():
     getattr(lib, _name).argtypes = [_TYPES[_t] for _t in _signature]

@@ -568,6 +568,102 @@ typedef struct fk_prompt_model {
 fk_status fk_prompt_run(const fk_prompt_model *model, const uint32_t *tokens, uint32_t count, uint32_t start,
                         uint32_t rows_per_pass, uint32_t *next_token, fk_stream s);
 
+/* ---- several sequences over a paged cache ---------------------------------------------------
+ * A serving loop or a beam search keeps the keys and values of all its sequences in one pool of pages and a table of page
+ * ids for each sequence (an MI355X addition: the reference's caches belong to one sequence).  The arrays of a batch are
+ * device memory, so that a captured graph is replayed while the lengths grow; what a launch is sized for comes from the
+ * host (rows, max_rows, max_len).  Device values beyond that are cut to it and never take an address out of the pool, the
+ * table or the rows; they set bits of *fault (FK_PAGED_*), which fk_paged_check reports. */
+typedef struct fk_page_pool {           /* one layer's pages */
+    uint16_t *k, *v;                    /* bf16 [n_pages, n_kv, page_rows, head_dim] each, 16-byte aligned */
+    uint32_t n_pages, page_rows;        /* page_rows: a power of two, 16 .. 1024 */
+    uint32_t n_kv, head_dim;            /* head_dim 64 or 128 */
+} fk_page_pool;
+typedef struct fk_paged_batch {
+    const uint32_t *row_start;          /* device [n_seqs + 1]: sequence i has the new rows row_start[i] .. row_start[i + 1] - 1 (none, one or many) */
+    const uint32_t *kv_len;             /* device [n_seqs]: positions of a sequence, its new rows included; the last row sits at kv_len - 1 */
+    const uint32_t *page_table;         /* device [n_seqs, table_stride]: position p lies in row p % page_rows of page page_table[i][p / page_rows] */
+    uint32_t table_stride;
+    uint32_t n_seqs;
+    uint32_t rows;                      /* rows that the row buffers hold; rows from row_start[n_seqs] on are left as they are */
+    uint32_t max_rows, max_len;         /* no sequence has more new rows, or more positions (at most table_stride * page_rows) */
+    uint32_t *fault;                    /* device word, zeroed once, or NULL */
+} fk_paged_batch;
+enum {
+    FK_PAGED_BAD_ROWS = 1,              /* row_start falls, or a sequence has more rows than max_rows or the buffers hold */
+    FK_PAGED_BAD_LENGTH = 2,            /* kv_len above max_len, or below the sequence's new rows */
+    FK_PAGED_BAD_PAGE = 4               /* a page id that the pool does not have */
+};
+/* Synchronises the stream; FK_ERR_INVALID with a message where *fault is set, which is then zeroed.  What the launches
+ * since the last check wrote for the sequence at fault is undefined (inside its own rows and pages). */
+fk_status fk_paged_check(uint32_t *fault, fk_stream s);
+
+/* Rotary frequencies of one model as fk_rope_paged_store takes them, in 64 bits: d_freq[i], i < dims / 2, is how many
+ * revolutions pair i turns from one position to the next, theta^(-2 i / dims) / 2 pi after scaling, and d_freq[dims / 2]
+ * multiplies every cosine and sine (1 without scaling).  A program may fill the array by itself.
+ *   FK_ROPE_PLAIN    as it is
+ *   FK_ROPE_LINEAR   divided by factor
+ *   FK_ROPE_PARTS    by how often a pair turns within the trained context: high times and more as it is, low times and
+ *                    fewer divided by factor, in between linearly from one to the other
+ *   FK_ROPE_RAMP     by a linear ramp over the pair index, from the pair that turns high times within the trained
+ *                    context (as it is; index rounded down) to the one that turns low times (divided; rounded up); the
+ *                    multiplier is 0.1 ln(factor) + 1
+ * trained: positions of the trained context (PARTS, RAMP). */
+enum { FK_ROPE_PLAIN = 0, FK_ROPE_LINEAR = 1, FK_ROPE_PARTS = 2, FK_ROPE_RAMP = 3 };
+fk_status fk_rope_frequencies(uint32_t dims, double theta, int scaling, double factor, double low, double high,
+                              uint32_t trained, double *d_freq, fk_stream s);
+/* R   for a batch over pages: rotates the first rope_dims of every q and k head of every new row at its position and
+ *     appends k and v to the sequence's pages; the counterpart of fk_qkv_rope_store_rows.  q, k, v rows lie *_stride
+ *     elements apart (column blocks of one packed row, for instance), q_out rows q_out_stride (q_out may be q).
+ *     interleaved: pairs (2 i, 2 i + 1), else (i, i + rope_dims / 2).  q_norm / k_norm [head_dim] (each may be NULL) first
+ *     apply the per-head RMSNorm; everything up to the stored bf16 value is fp32 with one rounding, and the angle is formed
+ *     and reduced in 64 bits (at 100 000 positions an fp32 angle is off by some 4e-3).  rope_dims a multiple of 16 up to
+ *     head_dim, or 0 (d_freq then NULL); strides multiples of 8, pointers 16-byte aligned.  Two rows of a batch that
+ *     share a page must not share a position: fork the page first (fk_pages_copy). */
+fk_status fk_rope_paged_store(const uint16_t *q, uint32_t q_stride, const uint16_t *k, uint32_t k_stride, const uint16_t *v,
+                              uint32_t v_stride, uint16_t *q_out, uint32_t q_out_stride, uint32_t n_heads,
+                              const uint16_t *q_norm, const uint16_t *k_norm, float eps, uint32_t rope_dims,
+                              int interleaved, const double *d_freq, const fk_paged_batch *batch,
+                              const fk_page_pool *pool, fk_stream s);
+/* K4  for a batch over pages: row r of a sequence, at position p, attends to positions max(0, p - window + 1) .. p
+ *     (window 0: from 0), n_heads / n_kv query heads to a KV head.  Scores q.k * scale, with softcap > 0
+ *     softcap * tanh(score / softcap); fp32 scores, softmax and sums, one rounding of the output.  A row that sees
+ *     nothing (a length below the new rows) is set to zeros.  K and V behind a sequence's length, and pages that hold none
+ *     of its positions, may hold anything.  q, out: rows q_stride / out_stride elements apart, heads of a row adjacent;
+ *     strides multiples of 8, pointers 16-byte aligned.  One launch serves chunks of prompts and single tokens together.
+ *     workspace: at least fk_sdpa_paged_workspace_bytes() (more lets few long sequences be cut finer, up to 64 MB),
+ *     zeroed before the first launch, left ready by each; launches that share it must not overlap, nor may graphs. */
+fk_status fk_sdpa_paged_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t n_seqs, uint32_t rows,
+                                        uint32_t max_len, size_t *bytes);
+fk_status fk_sdpa_paged(const uint16_t *q, uint32_t q_stride, uint16_t *out, uint32_t out_stride, uint32_t n_heads,
+                        float scale, float softcap, uint32_t window, const fk_paged_batch *batch,
+                        const fk_page_pool *pool, void *workspace, size_t workspace_bytes, fk_stream s);
+/* Pages copied inside a pool: page pairs[2 i] to page pairs[2 i + 1] in each of n_planes planes that lie plane_stride
+ * bytes apart (the layers' K and V; n_pages pages of page_bytes, a multiple of 16).  pairs is HOST memory and is read
+ * before the call returns (a captured launch keeps the pairs it was captured with).  What a fork of a sequence leaves to
+ * copy, and what compacting a pool moves.  Refused: ids out of range, a page written twice, a page both read and
+ * written (the order of such moves would matter: call twice).  No pairs: nothing is done. */
+fk_status fk_pages_copy(void *base, uint32_t n_planes, size_t plane_stride, uint32_t n_pages, size_t page_bytes,
+                        const uint32_t *pairs, uint32_t n_pairs, fk_stream s);
+/* Beam search: of each group's beams * vocab continuations the k best, in order: score[b] + log softmax(logits[b])[t],
+ * ties to the lower b * vocab + t.  logits bf16 rows row_stride apart; scores fp32 [groups * beams]; finished (or NULL):
+ * u32 [groups * beams], a beam whose word is not 0 goes on only with pad_token and keeps its score.  The sum of a row's
+ * exponentials and all sums behind it are formed in more than 32 bits, inside a beam the order is that of the logits.  A NaN
+ * logit counts as -inf, a score that is not a number likewise.  Where fewer than k continuations are above -inf, the
+ * lowest b * vocab + t that are left follow with -inf.  out_* [groups, k]; beams and k up to 64, groups * beams up to
+ * 65535.  workspace: fk_beam_select_workspace_bytes(), zeroed once; launches that share it must not overlap. */
+fk_status fk_beam_select_workspace_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k, size_t *bytes);
+fk_status fk_beam_select(const uint16_t *logits, size_t row_stride, const float *scores, const uint32_t *finished,
+                         uint32_t pad_token, uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k,
+                         float *out_scores, uint32_t *out_beams, uint32_t *out_tokens, void *workspace,
+                         size_t workspace_bytes, fk_stream s);
+/* Rows of per-beam state follow the beams that were chosen: dst[g * n_out + i] = src[g * beams + parents[g * n_out + i]], rows of
+ * row_bytes (any number).  dst may be src where n_out == beams (rows are then exchanged in place); otherwise the two
+ * must not overlap.  parents: device u32 [groups, n_out]; an index beyond the group's beams takes the last one.  beams,
+ * n_out up to 64. */
+fk_status fk_beam_reorder(const void *src, void *dst, size_t row_bytes, const uint32_t *parents, uint32_t groups, uint32_t beams,
+                          uint32_t n_out, fk_stream s);
+
 /* E   x = T(embed[token] * out_scale), dense bf16 or MLX-affine table.  Replaces
  *     src/codegen/kernels/embed_lookup_decode.rs:17-108. */
 fk_status fk_embed_lookup_decode(const fk_weight *E, const uint32_t *d_token, uint32_t token, float out_scale,
