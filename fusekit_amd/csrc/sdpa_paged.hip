@@ -6,12 +6,15 @@
 #include <math.h>
 
 #include "fk_host.hpp"
+#include "mma32_device.hpp"
 #include "paged_device.hpp"
 
 namespace fk {
 
-// Probabilities carry this factor, which cancels: a sum of 2^24 of them times the type's largest values stays in fp32's range.
-constexpr float kSmall = 0x1p-32f;
+// Probabilities carry the factor 2^-32, which cancels: a sum of 2^16 times 2^8 of them times the type's largest values stays in
+// fp32's range (2^8: how far a step's maximum may lie above the softmax reference).
+constexpr float kSmallLog2 = 32.0f, kSmall = 0x1p-32f, kPagedLag = 8.0f;
+constexpr float kLog2E = 1.44269504088896341f;
 
 struct SdpaPagedArgs {
     PagedArgs b;
@@ -22,24 +25,23 @@ struct SdpaPagedArgs {
     uint32_t q_stride, out_stride, n_heads, group;
     uint32_t window;
     float scale, softcap;
+    float* partials;       // [slots][columns of a tile][D], then (m, l) [slots][columns of a tile]
+    uint32_t* counters;    // [slots], zero before the first launch, left zero
+    uint32_t slots;
+    uint32_t target, min_steps;   // items that a launch is cut into where its tiles are fewer; the least steps of an item
 };
 
-// A wave a (row, head).  64 positions at a time: a lane forms one score, then the lanes share out the dims.
+// ---- one row of one head by a wave: positions in the order they lie, what the row does not see is not touched ----
+// The statement of the operator as it stands; the tiles below come here for a column whose sums are not finite, since a zero
+// probability times an infinity that other rows of the tile see is no number.
 template <int D>
-__global__ __launch_bounds__(64) void sdpa_paged_row_kernel(const SdpaPagedArgs a) {
-    const uint32_t lane = threadIdx.x, row = blockIdx.x, head = blockIdx.y, kvh = head / a.group;
-    const uint32_t seq = paged_seq_of(a.b, row, lane);
-    if (seq >= a.b.n_seqs) return;
-    const PagedSeq s = paged_seq(a.b, seq);
-    uint32_t bad = s.bad;
-    if (bad && lane == 0) paged_fault(a.b, bad);
-    const uint32_t place = row - s.row0;
-    if (row < s.row0 || place >= s.rows) return;
-    const uint32_t page_rows = 1u << a.b.page_shift;
+__device__ __forceinline__ void paged_row(const SdpaPagedArgs& a, uint32_t seq, const PagedSeq& s, uint32_t place, uint32_t head, uint32_t lane) {
+    const uint32_t kvh = head / a.group, row = s.row0 + place, page_rows = 1u << a.b.page_shift;
     const uint32_t end = s.len + place + 1u > s.rows ? s.len + place + 1u - s.rows : 0u;   // positions up to the row's own
     const uint32_t first = a.window && end > a.window ? end - a.window : 0u;
     const uint16_t* qr = a.q + (size_t)row * a.q_stride + (size_t)head * D;
     constexpr int DL = D / 64;
+    uint32_t bad = 0;
     float m = -INFINITY, l = 0.f, o[DL];
 #pragma unroll
     for (int i = 0; i < DL; ++i) o[i] = 0.f;
@@ -49,6 +51,7 @@ __global__ __launch_bounds__(64) void sdpa_paged_row_kernel(const SdpaPagedArgs 
         const size_t base = (((size_t)page * a.b.n_kv + kvh) * page_rows + (pos & (page_rows - 1u))) * D;
         const uint4* kr = reinterpret_cast<const uint4*>(a.k + base);
         float x = 0.f;
+#pragma unroll 1
         for (int i = 0; i < D / 8; ++i) {
             const uint4 kk = kr[i], qq = reinterpret_cast<const uint4*>(qr)[i];
             const uint32_t kw[4] = {kk.x, kk.y, kk.z, kk.w}, qw[4] = {qq.x, qq.y, qq.z, qq.w};
@@ -64,6 +67,7 @@ __global__ __launch_bounds__(64) void sdpa_paged_row_kernel(const SdpaPagedArgs 
 #pragma unroll
         for (int i = 0; i < DL; ++i) o[i] *= alpha;
         const uint32_t n = end - at < 64u ? end - at : 64u;
+#pragma unroll 1
         for (uint32_t j = 0; j < n; ++j) {
             const float pj = __shfl(p, (int)j, 64);
             const size_t vb = __shfl((unsigned long long)base, (int)j, 64);
@@ -74,10 +78,417 @@ __global__ __launch_bounds__(64) void sdpa_paged_row_kernel(const SdpaPagedArgs 
 #pragma unroll
     for (int i = 0; i < DL; ++i)
         a.out[(size_t)row * a.out_stride + (size_t)head * D + lane + 64u * i] = (uint16_t)f32_to_bf16_bits(end > first ? o[i] / l : 0.f);
-    if (__builtin_amdgcn_ballot_w64(bad != 0)) {
-        if (bad) paged_fault(a.b, bad);
+}
+
+// ---- which piece of the work a block does ----
+// The columns of a sequence and KV head are its new rows times the query heads of a group, place * group + head; COLS of them are a tile.
+// A tile walks its positions in steps of 64; where all tiles of the launch are fewer than `target` the steps are cut over several items.
+// Every wave finds its block's item by itself from the batch's arrays, 64 sequences with one request: lengths stay on the device.
+struct PagedItem {
+    uint32_t seq, kvh, tile, split, n_splits;
+    PagedSeq s;
+    bool any;
+};
+template <uint32_t COLS>
+__device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t index, uint32_t lane) {
+    const uint32_t n_kv = a.b.n_kv;
+    auto tiles_of = [&](const PagedSeq& s) { return (uint32_t)(((uint64_t)s.rows * a.group + COLS - 1u) / COLS); };
+    auto steps_of = [&](const PagedSeq& s) {   // of a tile of the sequence, at most
+        uint32_t seen = s.len;
+        if (a.window) {
+            const uint64_t w = (uint64_t)a.window + (s.rows < COLS / a.group + 1u ? s.rows : COLS / a.group + 1u) + 63u;
+            seen = w < seen ? (uint32_t)w : seen;
+        }
+        return (seen + 63u) / 64u;
+    };
+    auto read = [&](uint32_t at) {
+        const uint32_t i = at + lane;
+        PagedSeq s = paged_seq(a.b, i < a.b.n_seqs ? i : a.b.n_seqs - 1u);
+        if (i >= a.b.n_seqs) s.rows = 0;
+        if (s.bad && i < a.b.n_seqs && index == 0) paged_fault(a.b, s.bad);
+        return s;
+    };
+    float work = 0.f, pairs = 0.f;
+    PagedSeq mine = read(0);
+    for (uint32_t at = 0;;) {
+        const float t = (float)tiles_of(mine) * (float)n_kv;
+        work += t * (float)steps_of(mine);
+        pairs += t;
+        if ((at += 64u) >= a.b.n_seqs) break;
+        mine = read(at);
+    }
+    work = wave_sum(work);
+    pairs = wave_sum(pairs);
+    const bool cut = pairs + (float)a.target <= (float)a.slots;
+    // (of at least work / target steps: all items together are at most target + pairs)
+    const float share = work / (float)a.target;
+    uint32_t unit = share < 0x1p30f ? (uint32_t)ceilf(share) : 1u << 30;
+    unit = unit < a.min_steps ? a.min_steps : unit;
+    PagedItem it;
+    it.any = false;
+    uint32_t left = index;
+    for (uint32_t at = 0; at < a.b.n_seqs; at += 64u) {
+        if (a.b.n_seqs > 64u) mine = read(at);
+        const uint32_t tiles = tiles_of(mine);
+        uint32_t splits = cut ? (steps_of(mine) + unit - 1u) / unit : 1u;
+        splits = splits < 1u ? 1u : splits;
+        const uint32_t items = tiles * splits * n_kv;
+        uint32_t upto = items;   // with those of the lanes before
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t v = __shfl_up(upto, o, 64);
+            upto += lane >= (uint32_t)o ? v : 0u;
+        }
+        const unsigned long long past = __builtin_amdgcn_ballot_w64(upto > left);
+        if (!past) {
+            left -= (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+            continue;
+        }
+        const int who = (int)__builtin_ctzll(past);
+        auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, who); };
+        left -= of(upto) - of(items);
+        it.seq = at + (uint32_t)who;
+        it.s = PagedSeq{of(mine.row0), of(mine.rows), of(mine.len), of(mine.bad)};
+        it.n_splits = of(splits);
+        it.kvh = left % n_kv;
+        left /= n_kv;
+        it.split = left % it.n_splits;
+        it.tile = of(tiles) - 1u - left / it.n_splits;   // the longest first
+        it.any = true;
+        break;
+    }
+    return it;
+}
+
+// ---- tiles of 128 columns ----
+// A block is four waves of 32 columns on the same 64 positions a step.  The products and the softmax are those of the causal attention of one
+// sequence over a contiguous cache (sdpa_prefill.hip: S^T = K Q^T, a lane owns one query; O^T += V^T P^T with the score registers as they lie; V^T
+// through ds_read_b64_tr_b16; probabilities formed between the matrix instructions).  A wave requests 16 rows of K and of V a step, which lie
+// in one page: one page id, loaded two steps ahead into a scalar register.
+constexpr uint32_t kTileCols = 128, kTileStep = 64;
+constexpr uint32_t tile_lds_bytes(uint32_t d) {
+    const uint32_t stage = 2u * 2u * kTileStep * d * 2u, outb = kTileCols * (d + 4u) * 4u;
+    return (stage > outb ? stage : outb) + 16u;   // and a word for the block
+}
+constexpr int kPastCaches = 16;   // (sc1: what another block wrote, or is to read)
+
+template <int D, bool CAP>
+__global__ __launch_bounds__(256, 2) void sdpa_paged_tile_kernel(const SdpaPagedArgs a) {
+    constexpr int KB = D / 16, DT = D / 32, VP = D / 8;
+    constexpr uint32_t ROW = D * 2u, TILE = kTileStep * ROW, STAGE = 2u * TILE;      // bytes: a row, K (or V) of a step, both
+    constexpr uint32_t RPI = 1024u / ROW;                                            // rows of one wave's request
+    constexpr int REQ = 16 / (int)RPI;                                               // requests of a wave, matrix and step
+    extern __shared__ uint4 lds_raw[];
+    unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_raw);
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kb = lane >> 5, nl = lane & 31u;
+    const PagedItem it = paged_item<kTileCols>(a, blockIdx.x, lane);
+    if (!it.any) return;
+    const uint32_t G = a.group, columns = it.s.rows * G;   // (below 2^31: the host has checked)
+    auto limit_of = [&](uint32_t place) { return it.s.len + place + 1u > it.s.rows ? it.s.len + place + 1u - it.s.rows : 0u; };   // positions a row may see end here
+    auto low_of = [&](uint32_t limit) { return a.window && limit > a.window ? limit - a.window : 0u; };                           // and begin here
+    const uint32_t e_tile = it.tile * kTileCols, e_last = columns - e_tile < kTileCols ? columns - 1u : e_tile + kTileCols - 1u;
+    const uint32_t kv_end = __builtin_amdgcn_readfirstlane(limit_of(e_last / G));
+    const uint32_t step0 = __builtin_amdgcn_readfirstlane(low_of(limit_of(e_tile / G)) / kTileStep);
+    const uint32_t all_steps = (kv_end + kTileStep - 1u) / kTileStep - (kv_end ? step0 : 0u);
+    const uint32_t per = (all_steps + it.n_splits - 1u) / it.n_splits;
+    const uint32_t n_active = per ? (all_steps + per - 1u) / per : 1u;   // items of this tile that have steps (one at least)
+    if (it.split >= n_active) return;
+    const uint32_t begin = __builtin_amdgcn_readfirstlane(step0 + it.split * per);
+    const uint32_t stop = __builtin_amdgcn_readfirstlane(it.split + 1u == n_active ? step0 + all_steps : begin + per);
+
+    // this lane's column; a wave's columns past the last repeat it, and a wave without columns does the last one's loads and nothing else
+    const uint32_t e0 = e_tile + wave * 32u;
+    const uint32_t live = e0 <= e_last ? (e_last - e0 < 31u ? e_last - e0 + 1u : 32u) : 0u;
+    const uint32_t e = live ? e0 + (nl < live ? nl : live - 1u) : e_last;
+    const uint32_t place = e / G, head = it.kvh * G + (e - place * G);
+    const uint32_t q_limit = limit_of(place), q_low = low_of(q_limit);
+    const uint32_t first_limit = live ? __builtin_amdgcn_readfirstlane(limit_of(e0 / G)) : 0u, first_low = __builtin_amdgcn_readfirstlane(low_of(first_limit));
+    const uint32_t last_limit = live ? __builtin_amdgcn_readfirstlane(limit_of((e0 + live - 1u) / G)) : 0u, last_low = __builtin_amdgcn_readfirstlane(low_of(last_limit));
+    pf_u32x4_t qreg[KB];
+    {
+        const pf_u32x4_t* qp = reinterpret_cast<const pf_u32x4_t*>(a.q + (size_t)(it.s.row0 + place) * a.q_stride + (size_t)head * D + kb * 8u);
+#pragma unroll
+        for (int j = 0; j < KB; ++j) qreg[j] = qp[2 * j];
+    }
+
+    // the 16-byte piece of a row that lies at place `at`: K reads 16 rows of one piece at a time, V 8 rows of 64 bytes
+    auto k_swizzle = [](uint32_t row) { return D == 128 ? row & 15u : (row >> 1) & 7u; };
+    auto v_swizzle = [](uint32_t row) { return D == 128 ? (row & 3u) << 2 : ((row >> 1) & 1u) << 2; };
+    const uint32_t irow = lane / (uint32_t)VP, at_piece = lane % (uint32_t)VP;
+    const uint32_t shift = a.b.page_shift, in_page = (1u << shift) - 1u;
+    typedef const uint32_t __attribute__((address_space(4)))* scalar_ptr;
+    const uintptr_t table = (uintptr_t)(a.b.table + (size_t)__builtin_amdgcn_readfirstlane(it.seq) * a.b.table_stride);
+    uint32_t bad = 0;
+    auto span_of = [&](uint32_t step) { return step * kTileStep + wave * 16u; };   // the first of this wave's 16 rows of a step
+    auto page_of = [&](uint32_t step) {                                             // (past the range: the last position's)
+        const uint32_t span = span_of(step), at = span < kv_end ? span : kv_end - 1u;
+        return *(scalar_ptr)(table + (size_t)(at >> shift) * 4u);
+    };
+    auto issue = [&](uint32_t step, uint32_t page, uint32_t stage) {
+        if (page >= a.b.n_pages) {
+            page = 0;
+            bad = FK_PAGED_BAD_PAGE;
+        }
+        const uint32_t span = span_of(step), at = span < kv_end ? span : kv_end - 1u, left = kv_end - 1u - at;
+        const size_t off = (((size_t)page * a.b.n_kv + it.kvh) * (in_page + 1u) + (at & in_page)) * ROW;
+        const unsigned char *ks = reinterpret_cast<const unsigned char*>(a.k) + off, *vs = reinterpret_cast<const unsigned char*>(a.v) + off;
+#pragma unroll
+        for (int i = 0; i < REQ; ++i) {
+            const uint32_t r = (uint32_t)i * RPI + irow, row = wave * 16u + r, from = r < left ? r : left;   // (past the range: masked scores, zero probabilities)
+            const uint32_t to = stage * STAGE + (wave * (uint32_t)REQ + (uint32_t)i) * 1024u;
+            dma16(to, from * ROW + ((at_piece ^ k_swizzle(row)) * 16u), ks);
+            dma16(to + TILE, from * ROW + ((at_piece ^ v_swizzle(row)) * 16u), vs);
+        }
+    };
+
+    float m_run = -INFINITY, l_run = 0.f;
+    pf_f32x16_t oacc[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) oacc[i][r] = 0.f;
+
+    // fragments: K row nl (+ 32), piece 2 j + kb; V rows 4 kb + (0..3) (+ 8) of 16, columns 32 i + nl
+    const uint32_t vrow = 4u * kb + ((lane & 15u) >> 2), vcol = ((lane >> 4) & 1u) * 2u + ((lane & 3u) >> 1), vlow = (lane & 1u) * 8u;
+    auto barrier = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const float scale2 = CAP ? 1.0f : a.scale * kLog2E;                              // scores to exponents of two
+    const float cap2 = a.softcap * kLog2E, turn2 = CAP ? 2.0f * a.scale * kLog2E / a.softcap : 0.f;
+
+    uint32_t page_next = 0;
+    if (begin < stop) {
+        const uint32_t page = page_of(begin);
+        if (begin + 1u < stop) page_next = page_of(begin + 1u);
+        issue(begin, page, 0);
+    }
+    uint32_t stage = 0;
+#pragma unroll 1
+    for (uint32_t step = begin; step < stop; ++step, stage ^= 1u) {
+        wait_loads<0>();
+        barrier();   // this step's rows are everybody's; the other stage has been read
+        if (step + 1u < stop) {
+            issue(step + 1u, page_next, stage ^ 1u);
+            if (step + 2u < stop) page_next = page_of(step + 2u);
+        }
+        const uint32_t kv0 = step * kTileStep;
+        if (kv0 >= last_limit || kv0 + kTileStep <= first_low) continue;   // nothing that a row of this wave sees
+        const unsigned char *ks = lds + stage * STAGE, *vs = ks + TILE;
+        // all of a product's fragments are asked for before its first matrix instruction
+        pf_u32x4_t kf[KB][2];
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint32_t row = (uint32_t)t * 32u + nl;
+                kf[j][t] = *reinterpret_cast<const pf_u32x4_t*>(ks + row * ROW + (((uint32_t)(2 * j) + kb) ^ k_swizzle(row)) * 16u);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+        pf_f32x16_t s[2];
+        static_for<KB>([&](auto j) __attribute__((always_inline)) {
+            mfma32_scores<j() == 0>(s[0], kf[j()][0], qreg[j()]);
+            mfma32_scores<j() == 0>(s[1], kf[j()][1], qreg[j()]);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+        pf_s16x4_t vf[4][DT][2];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t row = (uint32_t)(c * 16 + h * 8) + vrow;
+                    const unsigned char* at = vs + row * ROW + (((uint32_t)(4 * i) + vcol) ^ v_swizzle(row)) * 16u + vlow;
+                    typedef __attribute__((address_space(3))) pf_s16x4_t* lds_ptr;
+                    vf[c][i][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(pf_s16x4_t*)at);
+                }
+        __builtin_amdgcn_sched_barrier(0);
+        settle_matrix_ops();
+        asm volatile("" : "+v"(s[0]), "+v"(s[1]));
+        if constexpr (CAP) {   // softcap * tanh(x / softcap) * log2 e, tanh(y) = 1 - 2 / (1 + 2^(2 y log2 e)): off by some 2^-22 of the cap
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    s[t][r] = fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[t][r] * turn2)), cap2);
+        }
+        if (kv0 + kTileStep > first_limit || kv0 < last_low) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const uint32_t kv = kv0 + (uint32_t)(t * 32 + r % 4 + 8 * (r / 4)) + 4u * kb;
+                    if (kv >= q_limit || kv < q_low) s[t][r] = -INFINITY;
+                }
+        }
+        // the softmax reference moves only when a step's maximum outgrows it by 2^8
+        float mt = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) mt = fmaxf(mt, s[i / 16][i % 16]);
+        mt = other_half_max(mt) * scale2;
+        const bool grow = mt > m_run + kPagedLag;
+        const float m_new = grow ? mt : m_run, m_ref = m_new == -INFINITY ? 0.f : m_new, m_sub = m_ref + kSmallLog2;
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_ref) : 1.0f;
+        m_run = m_new;
+        l_run *= alpha;
+        if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
+            settle_matrix_ops();
+#pragma unroll
+            for (int i = 0; i < DT; ++i) {
+                asm volatile("" : "+v"(oacc[i]));
+#pragma unroll
+                for (int r = 0; r < 16; ++r) oacc[i][r] *= alpha;
+            }
+        }
+        // the second product of 16 positions, and between its matrix instructions the probabilities of the next 16
+        pf_u32x4_t pb[4];
+        auto probabilities = [&](auto c, auto w) __attribute__((always_inline)) {
+            constexpr int at = c() * 8 + w() * 2;
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[at / 16][at % 16], scale2, -m_sub));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[at / 16][at % 16 + 1], scale2, -m_sub));
+            l_run += p0 + p1;
+            pb[c()][w()] = pack_bf16(p0, p1);
+        };
+        static_for<4>([&](auto w) __attribute__((always_inline)) { probabilities(std::integral_constant<int, 0>{}, w); });
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_nop 1");
+        static_for<4>([&](auto c) __attribute__((always_inline)) {
+            static_for<DT>([&](auto i) __attribute__((always_inline)) {
+                const pf_u32x2_t lo = __builtin_bit_cast(pf_u32x2_t, vf[c()][i()][0]), hi = __builtin_bit_cast(pf_u32x2_t, vf[c()][i()][1]);
+                mfma32_acc(oacc[i()], pf_u32x4_t{lo[0], lo[1], hi[0], hi[1]}, pb[c()]);
+                if constexpr (c() < 3)
+                    static_for<4 / DT>([&](auto w) __attribute__((always_inline)) {
+                        probabilities(std::integral_constant<int, c() + 1>{}, std::integral_constant<int, i() * (4 / DT) + w()>{});
+                    });
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            asm volatile("s_nop 1");
+        });
+    }
+    settle_matrix_ops();
+#pragma unroll
+    for (int i = 0; i < DT; ++i) asm volatile("" : "+v"(oacc[i]));
+    barrier();
+    if (bad && lane == 0) paged_fault(a.b, bad);
+
+    // ---- what the tile hands on: through this wave's own LDS rows, so that the stores are whole 16-byte pieces ----
+    l_run = both_halves_sum(l_run);
+    constexpr uint32_t OS = D + 4;
+    float* const ob = reinterpret_cast<float*>(lds_raw) + wave * 32u * OS;
+    const bool whole = n_active == 1u;
+    const float f = whole ? (l_run > 0.f || l_run != l_run ? 1.0f / l_run : 0.f) : 1.0f;   // (a row that sees nothing: zeros)
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<float4*>(ob + nl * OS + (uint32_t)(i * 32 + 8 * g) + 4u * kb) =
+                make_float4(oacc[i][4 * g + 0] * f, oacc[i][4 * g + 1] * f, oacc[i][4 * g + 2] * f, oacc[i][4 * g + 3] * f);
+    wave_lds_order();
+    // rows of this wave's columns whose sums are not finite, done again one by one (bit c: column e0 + c)
+    auto store_row = [&](uint32_t col, uint32_t pc, const float4& lo, const float4& hi) {
+        const uint32_t ec = e0 + col, pl = ec / G, hd = it.kvh * G + (ec - pl * G);
+        *reinterpret_cast<uint4*>(a.out + (size_t)(it.s.row0 + pl) * a.out_stride + (size_t)hd * D + pc * 8u) =
+            make_uint4(pack_bf16(lo.x, lo.y), pack_bf16(lo.z, lo.w), pack_bf16(hi.x, hi.y), pack_bf16(hi.z, hi.w));
+    };
+    auto finite = [](const float4& v) {
+        const float t = __builtin_fabsf(v.x) + __builtin_fabsf(v.y) + __builtin_fabsf(v.z) + __builtin_fabsf(v.w);
+        return t < INFINITY;
+    };
+    unsigned long long again = 0;
+    if (whole) {
+        for (uint32_t base = 0; base < live * (uint32_t)VP; base += 64u) {
+            const uint32_t idx = base + lane, col = idx / (uint32_t)VP, pc = idx % (uint32_t)VP;
+            const bool in = col < live;
+            const float4 lo = *reinterpret_cast<const float4*>(ob + (in ? col : 0u) * OS + pc * 8u);
+            const float4 hi = *reinterpret_cast<const float4*>(ob + (in ? col : 0u) * OS + pc * 8u + 4u);
+            if (in) store_row(col, pc, lo, hi);
+            unsigned long long odd = __builtin_amdgcn_ballot_w64(in && !(finite(lo) && finite(hi)));
+            for (; odd; odd &= odd - 1u) again |= 1ull << ((base + (uint32_t)__builtin_ctzll(odd)) / (uint32_t)VP);
+        }
+    } else {
+        const uint32_t slot = blockIdx.x;
+        float* const part = a.partials + (size_t)slot * (kTileCols * (D + 2u));
+        const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(part, 0, (int)(kTileCols * (D + 2u) * 4u), 0x27000);
+        for (uint32_t idx = lane; idx < live * (uint32_t)(D / 4); idx += 64u) {
+            const uint32_t col = idx / (uint32_t)(D / 4), pc = idx % (uint32_t)(D / 4);
+            const pf_u32x4_t v = *reinterpret_cast<const pf_u32x4_t*>(ob + col * OS + pc * 4u);
+            __builtin_amdgcn_raw_buffer_store_b128(v, mem, (int)(((wave * 32u + col) * D + pc * 4u) * 4u), 0, kPastCaches);
+        }
+        if (kb == 0 && nl < live) {
+            const pf_u32x2_t ml = {__float_as_uint(m_run), __float_as_uint(l_run)};
+            __builtin_amdgcn_raw_buffer_store_b64(ml, mem, (int)((kTileCols * D + (wave * 32u + nl) * 2u) * 4u), 0, kPastCaches);
+        }
+        // the item that arrives last merges the tile's, in their order
+        volatile uint32_t* const last = reinterpret_cast<volatile uint32_t*>(lds + tile_lds_bytes(D) - 16u);   // (LDS starts with the stages: their addresses are absolute)
+        const uint32_t n_kv = a.b.n_kv, base = slot - it.split * n_kv;   // the slot of the tile's first item
+        wait_memory_ops_done();
+        __syncthreads();
+        if (tid == 0) *last = atomicAdd(&a.counters[base], 1u) == n_active - 1u ? 1u : 0u;
+        __syncthreads();
+        if (!*last) return;
+        if (tid == 0) __hip_atomic_store(&a.counters[base], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc(a.partials, 0, (int)(a.slots * (uint32_t)(kTileCols * (D + 2u) * 4u)), 0x27000);
+        constexpr uint32_t SLOT = kTileCols * (D + 2u) * 4u;
+        for (uint32_t b0 = 0; b0 < live * (uint32_t)VP; b0 += 64u) {
+            const uint32_t idx = b0 + lane, col = idx / (uint32_t)VP, pc = idx % (uint32_t)VP;
+            const bool in = col < live;
+            const uint32_t c = wave * 32u + (in ? col : 0u);
+            float M = -INFINITY, l = 0.f;
+            float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+            for (uint32_t i = 0; i < n_active; ++i) {
+                const uint32_t at = (base + i * n_kv) * SLOT;
+                const pf_u32x2_t ml = __builtin_bit_cast(pf_u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(all, (int)(at + (kTileCols * D + c * 2u) * 4u), 0, kPastCaches));
+                const pf_u32x4_t u0 = __builtin_bit_cast(pf_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(all, (int)(at + (c * D + pc * 8u) * 4u), 0, kPastCaches));
+                const pf_u32x4_t u1 = __builtin_bit_cast(pf_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(all, (int)(at + (c * D + pc * 8u + 4u) * 4u), 0, kPastCaches));
+                const float mi = __uint_as_float(ml[0]), Mn = fmaxf(M, mi), ref = Mn == -INFINITY ? 0.f : Mn;
+                const float w0 = __builtin_amdgcn_exp2f(M - ref), w1 = __builtin_amdgcn_exp2f(mi - ref);
+                M = Mn;
+                l = l * w0 + __uint_as_float(ml[1]) * w1;
+                lo = make_float4(fmaf(__uint_as_float(u0[0]), w1, lo.x * w0), fmaf(__uint_as_float(u0[1]), w1, lo.y * w0),
+                                 fmaf(__uint_as_float(u0[2]), w1, lo.z * w0), fmaf(__uint_as_float(u0[3]), w1, lo.w * w0));
+                hi = make_float4(fmaf(__uint_as_float(u1[0]), w1, hi.x * w0), fmaf(__uint_as_float(u1[1]), w1, hi.y * w0),
+                                 fmaf(__uint_as_float(u1[2]), w1, hi.z * w0), fmaf(__uint_as_float(u1[3]), w1, hi.w * w0));
+            }
+            const float r = l > 0.f || l != l ? 1.0f / l : 0.f;
+            lo = make_float4(lo.x * r, lo.y * r, lo.z * r, lo.w * r);
+            hi = make_float4(hi.x * r, hi.y * r, hi.z * r, hi.w * r);
+            if (in) store_row(col, pc, lo, hi);
+            unsigned long long odd = __builtin_amdgcn_ballot_w64(in && !(finite(lo) && finite(hi)));
+            for (; odd; odd &= odd - 1u) again |= 1ull << ((b0 + (uint32_t)__builtin_ctzll(odd)) / (uint32_t)VP);
+        }
+    }
+    for (; again; again &= again - 1u) {
+        const uint32_t ec = e0 + (uint32_t)__builtin_ctzll(again), pl = ec / G;
+        paged_row<D>(a, it.seq, it.s, pl, it.kvh * G + (ec - pl * G), lane);
     }
 }
+
+namespace {
+
+// How a launch is cut: fewer tiles than `target` are cut along their positions, into items of `min_steps` steps at least.
+struct PagedPlan {
+    uint32_t target, min_steps, slots;
+    uint64_t tiles;    // of all sequences and KV heads, at most
+    size_t slot_bytes, bytes;
+};
+PagedPlan paged_plan(uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t n_seqs, uint32_t rows) {
+    PagedPlan p;
+    p.target = 448;
+    p.min_steps = 4;
+    p.tiles = ((uint64_t)rows * (n_heads / n_kv) / kTileCols + n_seqs) * n_kv;
+    p.slot_bytes = (size_t)kTileCols * (head_dim + 2) * 4;
+    // (twice the target: what is cut then ends up with at most twice as many items as there are tiles)
+    p.slots = p.tiles + p.target <= 2 * p.target ? (uint32_t)p.tiles + p.target : 0;
+    p.bytes = 4096 + p.slots * p.slot_bytes;
+    return p;
+}
+
+}  // namespace
 
 fk_status sdpa_paged_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t n_seqs, uint32_t rows, uint32_t max_len,
                                      size_t* bytes) {
@@ -85,7 +496,7 @@ fk_status sdpa_paged_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t h
     if (n_heads == 0 || n_kv == 0 || n_heads % n_kv || n_seqs == 0 || rows == 0 || max_len == 0)
         return set_error(FK_ERR_INVALID, "sdpa_paged workspace: empty shape, or n_heads not a multiple of n_kv");
     if (head_dim != 64 && head_dim != 128) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged workspace: head dimension 64 or 128");
-    *bytes = 4096;
+    *bytes = paged_plan(n_heads, n_kv, head_dim, n_seqs, rows).bytes;
     return FK_OK;
 }
 
@@ -103,17 +514,28 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15u) return set_error(FK_ERR_INVALID, "sdpa_paged: pointers must be 16-byte aligned");
     if (!(scale > 0.f) || !std::isfinite(scale)) return set_error(FK_ERR_INVALID, "sdpa_paged: scale must be positive");
     if (!(softcap >= 0.f) || !std::isfinite(softcap)) return set_error(FK_ERR_INVALID, "sdpa_paged: softcap must not be negative");
+    if ((uint64_t)batch->max_rows * (n_heads / n_kv) > 0x7fffffffull) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: too many rows of a sequence");
     size_t need = 0;
     FK_TRY(sdpa_paged_workspace_bytes(n_heads, n_kv, D, batch->n_seqs, batch->rows, batch->max_len, &need));
     if (workspace_bytes < need) return set_error(FK_ERR_INVALID, "sdpa_paged: workspace too small");
+    const PagedPlan p = paged_plan(n_heads, n_kv, D, batch->n_seqs, batch->rows);
+    if (p.tiles + p.target > 0x7fffffffull) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: too many rows");
     const DeviceFacts* dev;
     FK_TRY(device_facts(&dev));
     a.q = q; a.k = pool->k; a.v = pool->v; a.out = out;
     a.q_stride = q_stride; a.out_stride = out_stride; a.n_heads = n_heads; a.group = n_heads / n_kv;
     a.window = window; a.scale = scale; a.softcap = softcap;
-    l->func = D == 64 ? reinterpret_cast<const void*>(&sdpa_paged_row_kernel<64>) : reinterpret_cast<const void*>(&sdpa_paged_row_kernel<128>);
-    l->grid = dim3(batch->rows, n_heads, 1);
-    l->block = dim3(64, 1, 1);
+    a.counters = static_cast<uint32_t*>(workspace);
+    a.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + 4096);
+    a.slots = p.slots; a.target = p.target; a.min_steps = p.min_steps;
+    const void* func[2][2] = {{reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<64, false>), reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<64, true>)},
+                              {reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<128, false>), reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<128, true>)}};
+    l->func = func[D == 128][softcap > 0.f];
+    l->grid = dim3((uint32_t)(p.slots ? p.slots : p.tiles), 1, 1);
+    l->block = dim3(256, 1, 1);
+    l->shmem = tile_lds_bytes(D);
+    if ((int)l->shmem > dev->max_dyn_lds) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: LDS tile does not fit");
+    FK_TRY(raise_dynamic_lds(l->func, l->shmem));
     l->set_args(a);
     return FK_OK;
 }

@@ -30,13 +30,9 @@
 
 #include "dma_device.hpp"
 #include "fk_host.hpp"
+#include "mma32_device.hpp"
 
 namespace fk {
-
-typedef __bf16 pf_bf16x8_t __attribute__((ext_vector_type(8)));
-typedef float pf_f32x16_t __attribute__((ext_vector_type(16)));
-typedef unsigned int pf_u32x2_t __attribute__((ext_vector_type(2)));
-typedef unsigned int pf_u32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kPrefillBlock = 256;
 constexpr uint32_t kPrefillWaves = 4;
@@ -66,15 +62,6 @@ __device__ __forceinline__ uint32_t prefill_kv_len(const SdpaPrefillArgs& a) {
     uint32_t n = a.kv_len_ptr ? *a.kv_len_ptr : a.kv_len;
     n = n < a.rows ? a.rows : n;
     return n > a.capacity ? a.capacity : n;
-}
-
-__device__ __forceinline__ float other_half_max(float v) {
-    const pf_u32x2_t r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float both_halves_sum(float v) {
-    const pf_u32x2_t r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // The rescale of the output accumulators, in place in the accumulation registers of the matrix unit.
@@ -528,19 +515,6 @@ constexpr uint32_t prefill_dma_lds_bytes(uint32_t d, uint32_t split) {
     const uint32_t stage = 2u * 2u * split * kPrefillStep * d * 2u, outb = kPrefillWaves * kPrefillRows * (d + 4u) * 4u;
     return stage > outb ? stage : outb;
 }
-typedef short pf_s16x4_t __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ void mfma32_acc(pf_f32x16_t& acc, const pf_u32x4_t& a, const pf_u32x4_t& b) {
-    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(acc) : "v"(a), "v"(b));
-}
-
-// scores stay in VGPRs, where the softmax takes them
-template <bool FIRST>
-__device__ __forceinline__ void mfma32_scores(pf_f32x16_t& s, const pf_u32x4_t& a, const pf_u32x4_t& b) {
-    if constexpr (FIRST) asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "v"(b));
-    else asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "v"(b));
-}
-
 template <int D, int SPLIT>
 __global__ __launch_bounds__(kPrefillBlock, 2) void sdpa_prefill_dma_kernel(const SdpaPrefillArgs a) {
     constexpr int KB = D / 16, DT = D / 32, VP = D / 8;

@@ -631,8 +631,8 @@ fk_status fk_rope_paged_store(const uint16_t *q, uint32_t q_stride, const uint16
  *     nothing (a length below the new rows) is set to zeros.  K and V behind a sequence's length, and pages that hold none
  *     of its positions, may hold anything.  q, out: rows q_stride / out_stride elements apart, heads of a row adjacent;
  *     strides multiples of 8, pointers 16-byte aligned.  One launch serves chunks of prompts and single tokens together.
- *     workspace: at least fk_sdpa_paged_workspace_bytes() (more lets few long sequences be cut finer, up to 64 MB),
- *     zeroed before the first launch, left ready by each; launches that share it must not overlap, nor may graphs. */
+ *     workspace: fk_sdpa_paged_workspace_bytes() bytes (below 64 MB), zeroed before the first launch and left ready by each;
+ *     launches that share it must not overlap, those of graphs included. */
 fk_status fk_sdpa_paged_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t n_seqs, uint32_t rows,
                                         uint32_t max_len, size_t *bytes);
 fk_status fk_sdpa_paged(const uint16_t *q, uint32_t q_stride, uint16_t *out, uint32_t out_stride, uint32_t n_heads,
