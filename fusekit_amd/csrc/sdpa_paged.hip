@@ -82,24 +82,24 @@ __device__ __forceinline__ void paged_row(const SdpaPagedArgs& a, uint32_t seq, 
 
 // ---- which piece of the work a block does ----
 // The columns of a sequence and KV head are its new rows times the query heads of a group, place * group + head; COLS of them are a tile.
-// A tile walks its positions in steps of 64; where all tiles of the launch are fewer than `target` the steps are cut over several items.
+// A tile walks its positions in steps of STEP; where all tiles of the launch are fewer than `target` the steps are cut over several items.
 // Every wave finds its block's item by itself from the batch's arrays, 64 sequences with one request: lengths stay on the device.
 struct PagedItem {
     uint32_t seq, kvh, tile, split, n_splits;
     PagedSeq s;
     bool any;
 };
-template <uint32_t COLS>
+template <uint32_t COLS, uint32_t STEP>
 __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t index, uint32_t lane) {
     const uint32_t n_kv = a.b.n_kv;
     auto tiles_of = [&](const PagedSeq& s) { return (uint32_t)(((uint64_t)s.rows * a.group + COLS - 1u) / COLS); };
     auto steps_of = [&](const PagedSeq& s) {   // of a tile of the sequence, at most
         uint32_t seen = s.len;
         if (a.window) {
-            const uint64_t w = (uint64_t)a.window + (s.rows < COLS / a.group + 1u ? s.rows : COLS / a.group + 1u) + 63u;
+            const uint64_t w = (uint64_t)a.window + (s.rows < COLS / a.group + 1u ? s.rows : COLS / a.group + 1u) + STEP - 1u;
             seen = w < seen ? (uint32_t)w : seen;
         }
-        return (seen + 63u) / 64u;
+        return (seen + STEP - 1u) / STEP;
     };
     auto read = [&](uint32_t at) {
         const uint32_t i = at + lane;
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256, 2) void sdpa_paged_tile_kernel(const SdpaPaged
     unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_raw);
 
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kb = lane >> 5, nl = lane & 31u;
-    const PagedItem it = paged_item<kTileCols>(a, blockIdx.x, lane);
+    const PagedItem it = paged_item<kTileCols, kTileStep>(a, blockIdx.x, lane);
     if (!it.any) return;
     const uint32_t G = a.group, columns = it.s.rows * G;   // (below 2^31: the host has checked)
     auto limit_of = [&](uint32_t place) { return it.s.len + place + 1u > it.s.rows ? it.s.len + place + 1u - it.s.rows : 0u; };   // positions a row may see end here
@@ -468,23 +468,339 @@ __global__ __launch_bounds__(256, 2) void sdpa_paged_tile_kernel(const SdpaPaged
     }
 }
 
+// ---- single tokens: at most 16 columns of a sequence and KV head ----
+// The products are those of the decode attention over a contiguous cache (sdpa_mma.hip: 16x16x32, K rows and V^T as the first operand, the queries as
+// columns), a probability as the sum of two bf16 values, hi + lo, which leaves 2^-17 of it: of up to 8 columns in the columns 8 on, of more in an
+// instruction of its own.  A wave owns its steps of 32 positions and their place in LDS: it waits for no other wave until the block's waves
+// meet, its keys are requested again as soon as they are in registers, its values behind the second product.  Two blocks a CU keep 128 KB in
+// flight.  Bound by the bytes.
+constexpr uint32_t kFewCols = 16, kFewStep = 32, kFewRound = 4 * kFewStep;
+constexpr uint32_t few_lds_bytes(uint32_t d) {
+    const uint32_t stages = 4u * kFewStep * d * 4u, meet = 4u * kFewCols * (d + 4u) * 4u + 2u * 4u * kFewCols * 4u;
+    return (stages > meet ? stages : meet) + 16u;   // and two words for the block
+}
+
+template <int D, bool CAP, bool WIDE>
+__global__ __launch_bounds__(256, 2) void sdpa_paged_few_kernel(const SdpaPagedArgs a) {
+    constexpr uint32_t ROW = D * 2u, P = D / 8u, KT = kFewStep * ROW, STAGE = 2u * KT, RPI = 1024u / ROW;   // pieces of a row; rows of a request
+    constexpr int REQ = (int)(KT / 1024u), KS = D / 32, DT = D / 16, PARTS = WIDE ? 2 : 1;
+    constexpr uint32_t QT = WIDE ? 16u : 8u;
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    extern __shared__ uint4 lds_raw[];
+    unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_raw);
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
+    const PagedItem it = paged_item<kFewCols, kFewRound>(a, blockIdx.x, lane);
+    if (!it.any) return;
+    const uint32_t G = a.group, columns = it.s.rows * G;
+    auto limit_of = [&](uint32_t place) { return it.s.len + place + 1u > it.s.rows ? it.s.len + place + 1u - it.s.rows : 0u; };
+    auto low_of = [&](uint32_t limit) { return a.window && limit > a.window ? limit - a.window : 0u; };
+    const uint32_t kv_end = __builtin_amdgcn_readfirstlane(limit_of(it.s.rows - 1u)), lim_lo = __builtin_amdgcn_readfirstlane(limit_of(0));
+    const uint32_t low_lo = __builtin_amdgcn_readfirstlane(low_of(lim_lo)), low_hi = __builtin_amdgcn_readfirstlane(low_of(kv_end));
+    const uint32_t round0 = low_lo / kFewRound, rounds = (kv_end + kFewRound - 1u) / kFewRound - (kv_end ? round0 : 0u);
+    const uint32_t per = (rounds + it.n_splits - 1u) / it.n_splits;
+    const uint32_t n_active = per ? (rounds + per - 1u) / per : 1u;
+    if (it.split >= n_active) return;
+    const uint32_t first = (round0 + it.split * per) * kFewRound + wave * kFewStep;
+    uint32_t end = (round0 + (it.split + 1u) * per) * kFewRound;
+    end = __builtin_amdgcn_readfirstlane(end < kv_end ? end : kv_end);
+    const uint32_t n_steps = __builtin_amdgcn_readfirstlane(end > first ? (end - first + kFewRound - 1u) / kFewRound : 0u);
+
+    const uint32_t mine = n % QT < columns ? n % QT : columns - 1u;   // (columns past the last repeat it and store nothing)
+    const uint32_t place = mine / G, q_limit = limit_of(place), q_low = low_of(q_limit);
+    pf_bf16x8_t qf[KS];
+    {
+        const uint16_t* qr = a.q + (size_t)(it.s.row0 + place) * a.q_stride + (size_t)(it.kvh * G + (mine - place * G)) * D + g * 8u;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const pf_bf16x8_t*>(qr + s * 32);
+    }
+
+    auto k_swizzle = [](uint32_t row) { return P == 16u ? row & 15u : (row >> 1) & 7u; };
+    auto v_swizzle = [](uint32_t row) { return P == 16u ? (row & 7u) << 1 : ((row >> 1) & 3u) << 1; };
+    const uint32_t irow = lane / P, at_piece = lane % P, my_stage = wave * STAGE;
+    const uint32_t shift = a.b.page_shift, in_page = (1u << shift) - 1u;
+    typedef const uint32_t __attribute__((address_space(4)))* scalar_ptr;
+    const uintptr_t table = (uintptr_t)(a.b.table + (size_t)__builtin_amdgcn_readfirstlane(it.seq) * a.b.table_stride);
+    uint32_t bad = 0;
+    // a step's 32 positions lie in one page or two: 16 rows of each half in one
+    auto page_of = [&](uint32_t pos) {
+        const uint32_t at = pos < kv_end ? pos : kv_end - 1u;
+        return *(scalar_ptr)(table + (size_t)(at >> shift) * 4u);
+    };
+    auto issue = [&](const uint16_t* pages, uint32_t to, uint32_t kv0, const uint32_t (&page)[2], auto swizzle) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t id = page[h];
+            if (id >= a.b.n_pages) {
+                id = 0;
+                bad = FK_PAGED_BAD_PAGE;
+            }
+            const uint32_t span = kv0 + 16u * h, at = span < kv_end ? span : kv_end - 1u, left = kv_end - 1u - at;
+            const unsigned char* base = reinterpret_cast<const unsigned char*>(pages) +
+                                        (((size_t)id * a.b.n_kv + it.kvh) * (in_page + 1u) + (at & in_page)) * ROW;
+#pragma unroll
+            for (int i = 0; i < REQ / 2; ++i) {
+                const uint32_t r = (uint32_t)i * RPI + irow, from = r < left ? r : left;   // (past the context: its last row, masked)
+                dma16(to + (uint32_t)(h * (REQ / 2) + i) * 1024u, from * ROW + ((at_piece ^ swizzle(16u * h + r)) * 16u), base);
+            }
+        }
+    };
+    auto issue_k = [&](uint32_t kv0, const uint32_t (&page)[2]) { issue(a.k, my_stage, kv0, page, k_swizzle); };
+    auto issue_v = [&](uint32_t kv0, const uint32_t (&page)[2]) { issue(a.v, my_stage + KT, kv0, page, v_swizzle); };
+
+    f32x4_t acc[PARTS][DT];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+        for (int i = 0; i < DT; ++i) acc[p][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m_run = -INFINITY, l_run = 0.f;
+    const float scale2 = CAP ? 1.0f : a.scale * kLog2E;
+    const float cap2 = a.softcap * kLog2E, turn2 = CAP ? 2.0f * a.scale * kLog2E / a.softcap : 0.f;
+
+    uint32_t page[2] = {0, 0};
+    if (n_steps) {
+        page[0] = page_of(first);
+        page[1] = page_of(first + 16u);
+        issue_k(first, page);
+        issue_v(first, page);
+        if (n_steps > 1u) {
+            page[0] = page_of(first + kFewRound);
+            page[1] = page_of(first + kFewRound + 16u);
+        }
+    }
+#pragma unroll 1
+    for (uint32_t j = 0; j < n_steps; ++j) {
+        const uint32_t kv0 = first + j * kFewRound;
+        unsigned char* const ks = lds + my_stage;
+        unsigned char* const vs = ks + KT;
+        const bool more = j + 1u < n_steps;
+        wait_loads<REQ>();   // the keys; the values may be on their way
+        pf_bf16x8_t kf[2][KS];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const uint32_t row = (uint32_t)t * 16u + n;
+                kf[t][s] = *reinterpret_cast<const pf_bf16x8_t*>(ks + row * ROW + ((((uint32_t)s * 4u + g) ^ k_swizzle(row)) * 16u));
+            }
+        // (two chains a score beyond 64 dims: in one, each instruction's rounding is that of the whole sum so far)
+        float x[8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            constexpr int HALF = KS >= 4 ? KS / 2 : KS;
+            f32x4_t s4 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < HALF; ++s) s4 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][s], qf[s], s4, 0, 0, 0);
+            if constexpr (HALF < KS) {
+                f32x4_t s5 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = HALF; s < KS; ++s) s5 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t][s], qf[s], s5, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s4[i] += s5[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[t * 4 + i] = s4[i];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) issue_k(kv0 + kFewRound, page);   // the keys are in registers: their place takes the next step's
+        if constexpr (CAP) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[i] * turn2)), cap2);
+        }
+        if (kv0 + kFewStep > lim_lo || kv0 < low_hi) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t kv = kv0 + (uint32_t)(i / 4) * 16u + 4u * g + (uint32_t)(i % 4);
+                if (kv >= q_limit || kv < q_low) x[i] = -INFINITY;
+            }
+        }
+        float mx = x[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+        mx *= scale2;
+        if (__builtin_amdgcn_ballot_w64(mx > m_run + kPagedLag) != 0) {   // rare after the first steps
+            mx = rows_max(mx);
+            const bool grow = mx > m_run + kPagedLag;
+            const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - mx) : 1.0f;
+            m_run = grow ? mx : m_run;
+            l_run *= alpha;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                for (int i = 0; i < DT; ++i) acc[p][i] *= alpha;
+        }
+        const float m_sub = (m_run == -INFINITY ? 0.f : m_run) + kSmallLog2;
+        pf_u32x4_t pb[PARTS];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float p0 = __builtin_amdgcn_exp2f(fmaf(x[2 * i], scale2, -m_sub)), p1 = __builtin_amdgcn_exp2f(fmaf(x[2 * i + 1], scale2, -m_sub));
+            l_run += p0 + p1;
+            const uint32_t hi = pack_bf16(p0, p1), lo = pack_bf16(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
+            if constexpr (WIDE) {
+                pb[0][i] = hi;
+                pb[PARTS - 1][i] = lo;
+            } else {
+                pb[0][i] = n < 8u ? hi : lo;
+            }
+        }
+        if (more) wait_loads<REQ>();   // the values; the next keys may be on their way
+        else wait_loads<0>();
+        pf_bf16x8_t vf[DT];
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+            s16x4 v4[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t row = (uint32_t)h * 16u + 4u * g + (n >> 2), piece = (uint32_t)(2 * i) + ((n & 3u) >> 1);
+                unsigned char* at = vs + row * ROW + ((piece ^ v_swizzle(row)) * 16u) + (n & 1u) * 8u;
+                typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+                v4[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(s16x4*)at);
+            }
+            vf[i] = __builtin_bit_cast(pf_bf16x8_t, __builtin_shufflevector(v4[0], v4[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int i = 0; i < DT; ++i) acc[p][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[i], __builtin_bit_cast(pf_bf16x8_t, pb[p]), acc[p][i], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) {
+            issue_v(kv0 + kFewRound, page);
+            if (j + 2u < n_steps) {
+                page[0] = page_of(kv0 + 2u * kFewRound);
+                page[1] = page_of(kv0 + 2u * kFewRound + 16u);
+            }
+        }
+    }
+    if (bad && lane == 0) paged_fault(a.b, bad);
+
+    // ---- the waves meet ----
+    const float l_all = [&] {
+        const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+        const float v = __uint_as_float(h[0]) + __uint_as_float(h[1]);
+        const auto f = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return __uint_as_float(f[0]) + __uint_as_float(f[1]);
+    }();
+    __syncthreads();
+    constexpr uint32_t OS = D + 4u;
+    float* const red = reinterpret_cast<float*>(lds);                   // [wave][column][OS]
+    float* const wm = red + 4u * kFewCols * OS;                         // [wave][column] references, sums
+    float* const wl = wm + 4u * kFewCols;
+    volatile uint32_t* const word = reinterpret_cast<volatile uint32_t*>(lds + few_lds_bytes(D) - 16u);
+    if (tid == 0) word[1] = 0;
+    if (g == 0) {
+        wm[wave * kFewCols + n] = m_run;
+        wl[wave * kFewCols + n] = l_all;
+    }
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+        f32x4_t o;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            o[r] = WIDE ? acc[0][i][r] + acc[PARTS - 1][i][r]
+                        : acc[0][i][r] + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(acc[0][i][r]), 0x108, 0xF, 0xF, true));   // the columns 8 on
+        if (n < QT) *reinterpret_cast<float4*>(red + (wave * kFewCols + n) * OS + (uint32_t)i * 16u + 4u * g) = make_float4(o[0], o[1], o[2], o[3]);
+    }
+    __syncthreads();
+    const bool whole = n_active == 1u;
+    constexpr uint32_t SLOT = kFewCols * (D + 2u) * 4u;
+    const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials, 0, (int)(a.slots * SLOT), 0x27000);
+    auto store = [&](uint32_t c, uint32_t d, const float4& o, float l) {
+        const float f = l > 0.f || l != l ? 1.0f / l : 0.f;   // (a row that sees nothing: zeros)
+        const float t = (__builtin_fabsf(o.x) + __builtin_fabsf(o.y)) + (__builtin_fabsf(o.z) + __builtin_fabsf(o.w));
+        const uint32_t pl = c / G;
+        *reinterpret_cast<uint2*>(a.out + (size_t)(it.s.row0 + pl) * a.out_stride + (size_t)(it.kvh * G + (c - pl * G)) * D + d) =
+            make_uint2(pack_bf16(o.x * f, o.y * f), pack_bf16(o.z * f, o.w * f));
+        if (!(t * f < INFINITY)) atomicOr(const_cast<uint32_t*>(&word[1]), 1u << c);
+    };
+    for (uint32_t i = tid; i < columns * (D / 4u); i += 256u) {
+        const uint32_t c = i / (D / 4u), d = (i % (D / 4u)) * 4u;
+        float M = wm[c];
+#pragma unroll
+        for (uint32_t w = 1; w < 4; ++w) M = fmaxf(M, wm[w * kFewCols + c]);
+        const float ref = M == -INFINITY ? 0.f : M;
+        float l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (uint32_t w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(wm[w * kFewCols + c] - ref);
+            const float4 p = *reinterpret_cast<const float4*>(red + (w * kFewCols + c) * OS + d);
+            l = fmaf(wl[w * kFewCols + c], f, l);
+            o = make_float4(fmaf(p.x, f, o.x), fmaf(p.y, f, o.y), fmaf(p.z, f, o.z), fmaf(p.w, f, o.w));
+        }
+        if (whole) {
+            store(c, d, o, l);
+        } else {
+            const uint32_t at = blockIdx.x * SLOT;
+            const pf_u32x4_t v = {__float_as_uint(o.x), __float_as_uint(o.y), __float_as_uint(o.z), __float_as_uint(o.w)};
+            __builtin_amdgcn_raw_buffer_store_b128(v, mem, (int)(at + (c * D + d) * 4u), 0, kPastCaches);
+            if (d == 0) {
+                const pf_u32x2_t ml = {__float_as_uint(M), __float_as_uint(l)};
+                __builtin_amdgcn_raw_buffer_store_b64(ml, mem, (int)(at + (kFewCols * D + c * 2u) * 4u), 0, kPastCaches);
+            }
+        }
+    }
+    if (!whole) {   // the item that arrives last merges the sequence's, in their order
+        const uint32_t n_kv = a.b.n_kv, base = blockIdx.x - it.split * n_kv;
+        wait_memory_ops_done();
+        __syncthreads();
+        if (tid == 0) word[0] = atomicAdd(&a.counters[base], 1u) == n_active - 1u ? 1u : 0u;
+        __syncthreads();
+        if (!word[0]) return;
+        if (tid == 0) __hip_atomic_store(&a.counters[base], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (uint32_t i = tid; i < columns * (D / 4u); i += 256u) {
+            const uint32_t c = i / (D / 4u), d = (i % (D / 4u)) * 4u;
+            float M = -INFINITY, l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            constexpr uint32_t AHEAD = 8;   // partials requested together
+            for (uint32_t b0 = 0; b0 < n_active; b0 += AHEAD) {
+                pf_u32x2_t ml[AHEAD];
+                pf_u32x4_t u[AHEAD];
+#pragma unroll
+                for (uint32_t k = 0; k < AHEAD; ++k) {
+                    const uint32_t at = (base + (b0 + k < n_active ? b0 + k : n_active - 1u) * n_kv) * SLOT;
+                    ml[k] = __builtin_bit_cast(pf_u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(mem, (int)(at + (kFewCols * D + c * 2u) * 4u), 0, kPastCaches));
+                    u[k] = __builtin_bit_cast(pf_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(mem, (int)(at + (c * D + d) * 4u), 0, kPastCaches));
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < AHEAD; ++k) {
+                    if (b0 + k >= n_active) break;
+                    const float mk = __uint_as_float(ml[k][0]), Mn = fmaxf(M, mk), ref = Mn == -INFINITY ? 0.f : Mn;
+                    const float w0 = __builtin_amdgcn_exp2f(M - ref), w1 = __builtin_amdgcn_exp2f(mk - ref);
+                    M = Mn;
+                    l = l * w0 + __uint_as_float(ml[k][1]) * w1;
+                    o = make_float4(fmaf(__uint_as_float(u[k][0]), w1, o.x * w0), fmaf(__uint_as_float(u[k][1]), w1, o.y * w0),
+                                    fmaf(__uint_as_float(u[k][2]), w1, o.z * w0), fmaf(__uint_as_float(u[k][3]), w1, o.w * w0));
+                }
+            }
+            store(c, d, o, l);
+        }
+    }
+    __syncthreads();
+    for (uint32_t again = word[1], c = 0; again; again >>= 1, ++c)
+        if ((again & 1u) && c % 4u == wave) paged_row<D>(a, it.seq, it.s, c / G, it.kvh * G + c % G, lane);
+}
+
 namespace {
 
 // How a launch is cut: fewer tiles than `target` are cut along their positions, into items of `min_steps` steps at least.
 struct PagedPlan {
+    bool few;          // single tokens: 16 columns a sequence and KV head at most
     uint32_t target, min_steps, slots;
     uint64_t tiles;    // of all sequences and KV heads, at most
     size_t slot_bytes, bytes;
 };
-PagedPlan paged_plan(uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t n_seqs, uint32_t rows) {
+constexpr size_t kPagedCounterBytes = 16384;   // a word for a slot
+PagedPlan paged_plan(bool few, uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t n_seqs, uint32_t rows) {
     PagedPlan p;
-    p.target = 448;
-    p.min_steps = 4;
-    p.tiles = ((uint64_t)rows * (n_heads / n_kv) / kTileCols + n_seqs) * n_kv;
-    p.slot_bytes = (size_t)kTileCols * (head_dim + 2) * 4;
-    // (twice the target: what is cut then ends up with at most twice as many items as there are tiles)
-    p.slots = p.tiles + p.target <= 2 * p.target ? (uint32_t)p.tiles + p.target : 0;
-    p.bytes = 4096 + p.slots * p.slot_bytes;
+    const uint32_t cols = few ? kFewCols : kTileCols;
+    p.few = few;
+    p.target = few ? 1024 : 448;
+    p.min_steps = few ? 2 : 4;
+    p.tiles = few ? (uint64_t)n_seqs * n_kv : ((uint64_t)rows * (n_heads / n_kv) / cols + n_seqs) * n_kv;
+    p.slot_bytes = (size_t)cols * (head_dim + 2) * 4;
+    // (an item more for every tile: what is cut into items of equal work has one that is not full)
+    p.slots = p.tiles <= p.target ? (uint32_t)p.tiles + p.target : 0;
+    p.bytes = kPagedCounterBytes + p.slots * p.slot_bytes;
     return p;
 }
 
@@ -496,7 +812,8 @@ fk_status sdpa_paged_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t h
     if (n_heads == 0 || n_kv == 0 || n_heads % n_kv || n_seqs == 0 || rows == 0 || max_len == 0)
         return set_error(FK_ERR_INVALID, "sdpa_paged workspace: empty shape, or n_heads not a multiple of n_kv");
     if (head_dim != 64 && head_dim != 128) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged workspace: head dimension 64 or 128");
-    *bytes = paged_plan(n_heads, n_kv, head_dim, n_seqs, rows).bytes;
+    const size_t few = paged_plan(true, n_heads, n_kv, head_dim, n_seqs, rows).bytes, tiles = paged_plan(false, n_heads, n_kv, head_dim, n_seqs, rows).bytes;
+    *bytes = few > tiles ? few : tiles;
     return FK_OK;
 }
 
@@ -518,7 +835,7 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     size_t need = 0;
     FK_TRY(sdpa_paged_workspace_bytes(n_heads, n_kv, D, batch->n_seqs, batch->rows, batch->max_len, &need));
     if (workspace_bytes < need) return set_error(FK_ERR_INVALID, "sdpa_paged: workspace too small");
-    const PagedPlan p = paged_plan(n_heads, n_kv, D, batch->n_seqs, batch->rows);
+    const PagedPlan p = paged_plan(batch->max_rows * (n_heads / n_kv) <= kFewCols, n_heads, n_kv, D, batch->n_seqs, batch->rows);
     if (p.tiles + p.target > 0x7fffffffull) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: too many rows");
     const DeviceFacts* dev;
     FK_TRY(device_facts(&dev));
@@ -526,14 +843,19 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     a.q_stride = q_stride; a.out_stride = out_stride; a.n_heads = n_heads; a.group = n_heads / n_kv;
     a.window = window; a.scale = scale; a.softcap = softcap;
     a.counters = static_cast<uint32_t*>(workspace);
-    a.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + 4096);
+    a.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kPagedCounterBytes);
     a.slots = p.slots; a.target = p.target; a.min_steps = p.min_steps;
-    const void* func[2][2] = {{reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<64, false>), reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<64, true>)},
+    const void* tile[2][2] = {{reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<64, false>), reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<64, true>)},
                               {reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<128, false>), reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<128, true>)}};
-    l->func = func[D == 128][softcap > 0.f];
+    const void* few[2][2][2] = {
+        {{reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, false, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, false, true>)},
+         {reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, true, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, true, true>)}},
+        {{reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, true>)},
+         {reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, true>)}}};
+    l->func = p.few ? few[D == 128][softcap > 0.f][batch->max_rows * (n_heads / n_kv) > 8u] : tile[D == 128][softcap > 0.f];
     l->grid = dim3((uint32_t)(p.slots ? p.slots : p.tiles), 1, 1);
     l->block = dim3(256, 1, 1);
-    l->shmem = tile_lds_bytes(D);
+    l->shmem = p.few ? few_lds_bytes(D) : tile_lds_bytes(D);
     if ((int)l->shmem > dev->max_dyn_lds) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: LDS tile does not fit");
     FK_TRY(raise_dynamic_lds(l->func, l->shmem));
     l->set_args(a);
