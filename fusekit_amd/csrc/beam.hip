@@ -11,94 +11,306 @@
 
 namespace fk {
 
-constexpr uint32_t kBeamMax = 64;
+constexpr uint32_t kBeamMax = 64, kBeamGroups = 4096;
+constexpr size_t kBeamCounterBytes = 4 * kBeamGroups;   // at the same place for every shape: a workspace serves one call after another
 
+// One launch.  A block takes a piece of a row: it leaves the piece's largest logit, its sum of exponentials and its k largest logits in order; the
+// block of a group that comes last forms lse and the k best of what all pieces left.  The pieces are cut by token, never by address: rows that
+// hold the same values have the same sums wherever they lie, so that ties between beams stay ties.
+//
+// The k largest of a piece without sorting it: the k-th largest of the 256 threads' largest values is a bound that at least k values reach and few
+// more (16 of 256: 17 on average); found by bisection over its 16 bits with ballots.  What reaches it is collected in LDS and ranked by counting.
+// Only a piece full of ties has more than fit there: its k largest are then taken one by one.
 struct BeamArgs {
     const uint16_t* logits;
     size_t row_stride;
     const float* scores;
     const uint32_t* finished;
-    uint32_t pad, groups, beams, vocab, k;
+    uint32_t pad, beams, vocab, k, pieces;
     float* out_scores;
     uint32_t* out_beams;
     uint32_t* out_tokens;
-    double* base;      // [groups * beams]: score - lse
-    uint64_t* best;    // [groups * beams][k]: (order of the logit << 32) | ~token, 0 where the row has no more
+    uint32_t* arrived;   // [groups], zero before the first launch, left zero
+    double* sums;        // [groups * beams][pieces]
+    float* tops;         // [groups * beams][pieces]
+    uint32_t* best;      // [groups * beams][pieces][k]: (order of the logit << 16) | (65535 - place in the piece), 0 where there are no more
 };
 
-// a NaN counts as -inf; -0 as 0
-__device__ __forceinline__ float beam_logit(uint32_t bits) {
-    const float v = bf16_bits_to_f32(bits);
-    return v != v ? -INFINITY : v + 0.0f;
+constexpr uint32_t kBeamList = 512;   // candidates that fit in LDS
+
+__device__ __forceinline__ double wave_sum_wide(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
 }
 
-__global__ __launch_bounds__(256) void beam_rows_kernel(const BeamArgs a) {
-    __shared__ float red[8];
-    __shared__ uint64_t win[4];
-    __shared__ double part[4];
-    const uint32_t row = blockIdx.x, tid = threadIdx.x;
-    const uint16_t* x = a.logits + (size_t)row * a.row_stride;
-    float m = -INFINITY;
-    for (uint32_t t = tid; t < a.vocab; t += 256u) m = fmaxf(m, beam_logit(x[t]));
-    m = block_max<256>(m, red);
-    double sum = 0.0;
-    for (uint32_t t = tid; t < a.vocab; t += 256u) sum += (double)expf(beam_logit(x[t]) - m);
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if ((tid & 63u) == 0) part[tid >> 6] = sum;
+// The largest bound that at least k of the block's 256 values reach, or 1 where fewer than k are not 0; `all`: LDS, 256 words.
+template <int BITS, int LOW>
+__device__ __forceinline__ uint32_t bound_of_best(uint32_t mine, uint32_t k, uint32_t* all) {
+    const uint32_t lane = threadIdx.x & 63u;
+    all[threadIdx.x] = mine;
     __syncthreads();
-    if (tid == 0) a.base[row] = (double)a.scores[row] - ((double)m + log((part[0] + part[1]) + (part[2] + part[3])));
-    uint64_t last = ~0ull;
-    for (uint32_t i = 0; i < a.k; ++i) {
-        uint64_t best = 0;
-        for (uint32_t t = tid; t < a.vocab; t += 256u) {
-            const uint64_t c = ((uint64_t)order_key(beam_logit(x[t])) << 32) | (uint32_t)~t;
-            if (c < last && c > best) best = c;
-        }
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t other = __shfl_xor(best, o, 64);
-            best = other > best ? other : best;
-        }
-        if ((tid & 63u) == 0) win[tid >> 6] = best;
-        __syncthreads();
-        for (int w = 0; w < 4; ++w) best = win[w] > best ? win[w] : best;
-        __syncthreads();
-        last = best;
-        if (tid == 0) a.best[(size_t)row * a.k + i] = best;
-        if (best == 0) last = 1;   // nothing is left: every further one is 0 too
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = all[lane + 64u * i];
+    uint32_t t = 0;
+#pragma unroll 1
+    for (int bit = LOW + BITS - 1; bit >= LOW; --bit) {
+        const uint32_t at = t | (1u << bit);
+        uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] >= at));
+        if (n >= k) t = at;
     }
+    return t ? t : 1u;
 }
 
-__device__ __forceinline__ float order_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+template <int VEC>   // 16-byte loads of a thread
+__global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
+    constexpr uint32_t PIECE = 2048u * VEC;
+    typedef uint32_t loose __attribute__((ext_vector_type(4), aligned(2)));   // (rows of an odd length start anywhere)
+    __shared__ uint32_t all[256];
+    __shared__ uint32_t list[kBeamList];
+    __shared__ double values[kBeamList], part[4], base[kBeamMax];
+    __shared__ uint32_t n_list, flag;
+    __shared__ float top[4];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    const uint32_t piece = blockIdx.x, row = blockIdx.y, g = row / a.beams, k = a.k;
+    const uint32_t from = piece * PIECE, left = a.vocab - from;
+    const bool over = a.finished && a.finished[row];   // (the same for the block)
+    if (!over) {
+        const uint16_t* x = a.logits + (size_t)row * a.row_stride + from;
+        loose w[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const uint32_t at = ((uint32_t)i * 256u + tid) * 8u;
+            if (at + 8u <= left) {
+                w[i] = *reinterpret_cast<const loose*>(x + at);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t lo = at + 2u * e < left ? x[at + 2u * e] : 0xff80u, hi = at + 2u * e + 1u < left ? x[at + 2u * e + 1u] : 0xff80u;
+                    w[i][e] = lo | hi << 16;
+                }
+            }
+        }
+        // (a NaN counts as -inf: the larger of the two)
+        auto value = [&](int i, int e) { return fmaxf(e & 1 ? bf16_hi(w[i][e >> 1]) : bf16_lo(w[i][e >> 1]), -INFINITY); };
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, value(i, e));
+        const float mw = wave_max(m), ref = mw == -INFINITY ? 0.f : mw;
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            float s8[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s8[e] = __builtin_amdgcn_exp2f((value(i, e) - ref) * 1.44269504088896341f);
+            sum += (double)((s8[0] + s8[1]) + (s8[2] + s8[3])) + (double)((s8[4] + s8[5]) + (s8[6] + s8[7]));
+        }
+        sum = wave_sum_wide(sum);
+        if (lane == 0) {
+            top[wave] = mw;
+            part[wave] = sum;
+        }
+        if (tid == 0) n_list = 0;
+        const uint32_t bound = bound_of_best<16, 16>(m == -INFINITY ? 0u : order_key(m + 0.0f), k, all);   // (-0 as 0)
+        const float least = __uint_as_float(bound >= 0x80000000u ? (bound & 0x7fff0000u) : (~bound & 0xffff0000u));   // (bound 1: a NaN's pattern)
+        const bool any = bound < 0x10000u;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = value(i, e);
+                if (v > -INFINITY && (any || v >= least)) {
+                    const uint32_t at = atomicAdd(&n_list, 1u);
+                    if (at < kBeamList) list[at] = (order_key(v + 0.0f) & 0xffff0000u) | (0xffffu - (((uint32_t)i * 256u + tid) * 8u + e));
+                }
+            }
+        __syncthreads();
+        const uint32_t n = n_list;
+        uint32_t* const out = a.best + ((size_t)row * a.pieces + piece) * k;
+        if (n <= kBeamList) {
+            for (uint32_t c = tid; c < n; c += 256u) {
+                const uint32_t mine = list[c];
+                uint32_t rank = 0;
+                for (uint32_t o = 0; o < n; ++o) rank += list[o] > mine ? 1u : 0u;
+                if (rank < k) __hip_atomic_store(&out[rank], mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            for (uint32_t c = n + tid; c < k; c += 256u) __hip_atomic_store(&out[c], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        } else {
+            uint32_t last = ~0u;
+            for (uint32_t c = 0; c < k; ++c) {
+                uint32_t best = 0;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float v = value(i, e);
+                        const uint32_t key = v > -INFINITY ? (order_key(v + 0.0f) & 0xffff0000u) | (0xffffu - (((uint32_t)i * 256u + tid) * 8u + e)) : 0u;
+                        best = key < last && key > best ? key : best;
+                    }
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) {
+                    const uint32_t other = __shfl_xor(best, o, 64);
+                    best = other > best ? other : best;
+                }
+                __syncthreads();
+                if (lane == 0) all[wave] = best;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) best = all[i] > best ? all[i] : best;
+                if (tid == 0) __hip_atomic_store(&out[c], best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                last = best;   // (0: nothing is left, and nothing is below it)
+            }
+        }
+        if (tid == 0) {
+            const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), rt = mt == -INFINITY ? 0.f : mt;
+            double s = 0.0;
+            for (int i = 0; i < 4; ++i) s += part[i] * (double)__builtin_amdgcn_exp2f((top[i] - rt) * 1.44269504088896341f);
+            const size_t at = (size_t)row * a.pieces + piece;
+            __hip_atomic_store(&a.tops[at], mt, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(reinterpret_cast<unsigned long long*>(&a.sums[at]), (unsigned long long)__double_as_longlong(s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
 
-// One wave a group.
-__global__ __launch_bounds__(64) void beam_merge_kernel(const BeamArgs a) {
-    __shared__ uint64_t chosen[kBeamMax];
-    const uint32_t g = blockIdx.x, lane = threadIdx.x;
-    const uint64_t vocab = a.vocab;
+    // ---- the group's last block ----
+    wait_memory_ops_done();
+    __syncthreads();
+    if (tid == 0) flag = atomicAdd(&a.arrived[g], 1u) == a.beams * a.pieces - 1u ? 1u : 0u;
+    __syncthreads();
+    if (!flag) return;
+    if (tid == 0) {
+        __hip_atomic_store(&a.arrived[g], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        n_list = 0;
+    }
+    for (uint32_t b = wave; b < a.beams; b += 4u) {
+        const uint32_t r = g * a.beams + b;
+        const float score = a.scores[r];
+        if (a.finished && a.finished[r]) {
+            if (lane == 0) base[b] = (double)score;
+            continue;
+        }
+        float m = -INFINITY;
+        for (uint32_t p = lane; p < a.pieces; p += 64u) m = fmaxf(m, __hip_atomic_load(&a.tops[(size_t)r * a.pieces + p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        m = wave_max(m);
+        double s = 0.0;
+        for (uint32_t p = lane; p < a.pieces; p += 64u) {
+            const size_t at = (size_t)r * a.pieces + p;
+            const float mp = __hip_atomic_load(&a.tops[at], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const double sp = __longlong_as_double((long long)__hip_atomic_load(reinterpret_cast<unsigned long long*>(&a.sums[at]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+            if (mp > -INFINITY) s += sp * exp((double)mp - (double)m);
+        }
+        s = wave_sum_wide(s);
+        if (lane == 0) base[b] = (double)score - ((double)m + log(s));
+    }
+    __syncthreads();
+    const uint32_t row_n = a.pieces * k, total = a.beams * row_n;
+    const uint32_t* const group_best = a.best + (size_t)g * total;
+    // candidate i of the group: its score and its place, or -inf
+    auto candidate = [&](uint32_t i, uint32_t key, uint64_t& flat) {
+        const uint32_t b = i / row_n, j = i - b * row_n;
+        if (a.finished && a.finished[g * a.beams + b]) {
+            flat = (uint64_t)b * a.vocab + a.pad;
+            return j == 0 ? base[b] : (double)-INFINITY;
+        }
+        flat = (uint64_t)b * a.vocab + (j / k) * PIECE + (0xffffu - (key & 0xffffu));
+        const uint32_t o = key & 0xffff0000u;
+        const double v = base[b] + (double)__uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o & 0xffff0000u);
+        return key && v > -INFINITY ? v : (double)-INFINITY;
+    };
+    constexpr uint32_t AHEAD = 8;
+    auto load = [&](uint32_t i) { return i < total ? __hip_atomic_load(&group_best[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0u; };
+    // (of a finished row nothing was written: its keys are not looked at, whatever they are)
+    uint32_t mine = 0;
+    uint32_t kept[AHEAD];
+    for (uint32_t at = 0; at < total; at += 256u * AHEAD) {
+        uint32_t key[AHEAD];
+#pragma unroll
+        for (uint32_t u = 0; u < AHEAD; ++u) key[u] = load(at + u * 256u + tid);
+#pragma unroll
+        for (uint32_t u = 0; u < AHEAD; ++u) {
+            const uint32_t i = at + u * 256u + tid;
+            if (i >= total) continue;
+            uint64_t flat;
+            const double v = candidate(i, key[u], flat);
+            if (v > -INFINITY) {
+                const uint32_t o = order_key((float)v);
+                mine = o > mine ? o : mine;
+            }
+        }
+        if (at == 0) {
+#pragma unroll
+            for (uint32_t u = 0; u < AHEAD; ++u) kept[u] = key[u];
+        }
+    }
+    const uint32_t bound = bound_of_best<32, 0>(mine, k, all);
+    auto collect = [&](uint32_t i, uint32_t key) {
+        if (i >= total) return;
+        uint64_t flat;
+        const double v = candidate(i, key, flat);
+        if (v > -INFINITY && order_key((float)v) >= bound) {
+            const uint32_t at = atomicAdd(&n_list, 1u);
+            if (at < kBeamList) {
+                list[at] = i;
+                values[at] = v;
+            }
+        }
+    };
+#pragma unroll
+    for (uint32_t u = 0; u < AHEAD; ++u) collect(u * 256u + tid, kept[u]);
+    for (uint32_t i = 256u * AHEAD + tid; i < total; i += 256u) collect(i, load(i));
+    __syncthreads();
+    uint32_t n = n_list;
+    auto put = [&](uint32_t at, double v, uint64_t flat) {
+        a.out_scores[(size_t)g * k + at] = (float)v;
+        a.out_beams[(size_t)g * k + at] = (uint32_t)(flat / a.vocab);
+        a.out_tokens[(size_t)g * k + at] = (uint32_t)(flat % a.vocab);
+    };
+    if (n <= kBeamList) {
+        // their places in LDS too, then each one's rank by counting
+        __shared__ uint64_t flats[kBeamList];
+        for (uint32_t c = tid; c < n; c += 256u) {
+            uint64_t flat;
+            candidate(list[c], load(list[c]), flat);
+            flats[c] = flat;
+        }
+        __syncthreads();
+        for (uint32_t c = tid; c < n; c += 256u) {
+            const double v = values[c];
+            const uint64_t flat = flats[c];
+            uint32_t rank = 0;
+            for (uint32_t o = 0; o < n; ++o) rank += values[o] > v || (values[o] == v && flats[o] < flat) ? 1u : 0u;
+            if (rank < k) put(rank, v, flat);
+        }
+        if (n >= k || tid != 0) return;
+        // fewer than k above -inf: the lowest places that are not among them
+        uint64_t at = 0;
+        for (uint32_t i = n; i < k; ++i, ++at) {
+            for (bool again = true; again;) {
+                again = false;
+                for (uint32_t c = 0; c < n; ++c)
+                    if (flats[c] == at) {
+                        ++at;
+                        again = true;
+                    }
+            }
+            put(i, -INFINITY, at);
+        }
+        return;
+    }
+    // ties beyond the list: one by one
     double last = INFINITY;
     uint64_t last_at = 0;
-    bool any = false;
-    uint32_t n = 0;
-    for (; n < a.k; ++n) {
+    for (uint32_t c = 0; c < k; ++c) {
         double best = -INFINITY;
         uint64_t at = ~0ull;
-        for (uint32_t c = lane; c < a.beams * a.k; c += 64u) {
-            const uint32_t b = c / a.k, row = g * a.beams + b;
-            double v;
-            uint32_t t;
-            if (a.finished && a.finished[row]) {
-                if (c % a.k) continue;
-                v = a.scores[row];
-                t = a.pad;
-            } else {
-                const uint64_t e = a.best[(size_t)row * a.k + c % a.k];
-                if (!e) continue;
-                v = a.base[row] + (double)order_value((uint32_t)(e >> 32));
-                t = ~(uint32_t)e;
-            }
-            if (!(v > -INFINITY)) continue;
-            const uint64_t flat = b * vocab + t;
-            if (any && !(v < last || (v == last && flat > last_at))) continue;   // chosen before
+        for (uint32_t i = tid; i < total; i += 256u) {
+            uint64_t flat;
+            const double v = candidate(i, load(i), flat);
+            if (!(v > -INFINITY) || (c && !(v < last || (v == last && flat > last_at)))) continue;
             if (v > best || (v == best && flat < at)) {
                 best = v;
                 at = flat;
@@ -112,42 +324,39 @@ __global__ __launch_bounds__(64) void beam_merge_kernel(const BeamArgs a) {
                 at = oa;
             }
         }
-        if (at == ~0ull) break;
+        __syncthreads();
+        if (lane == 0) {
+            values[wave] = best;
+            values[4 + wave] = __longlong_as_double((long long)at);
+        }
+        __syncthreads();
+        for (int i = 0; i < 4; ++i) {
+            const double ov = values[i];
+            const uint64_t oa = (uint64_t)__double_as_longlong(values[4 + i]);
+            if (ov > best || (ov == best && oa < at)) {
+                best = ov;
+                at = oa;
+            }
+        }
         last = best;
         last_at = at;
-        any = true;
-        if (lane == 0) {
-            chosen[n] = at;
-            a.out_scores[(size_t)g * a.k + n] = (float)best;
-            a.out_beams[(size_t)g * a.k + n] = (uint32_t)(at / vocab);
-            a.out_tokens[(size_t)g * a.k + n] = (uint32_t)(at % vocab);
-        }
-    }
-    if (lane != 0) return;
-    // nothing above -inf is left: the lowest places that were not chosen
-    uint64_t at = 0;
-    for (uint32_t found = n; n < a.k; ++n, ++at) {
-        for (bool again = true; again;) {
-            again = false;
-            for (uint32_t i = 0; i < found; ++i)
-                if (chosen[i] == at) {
-                    ++at;
-                    again = true;
-                }
-        }
-        a.out_scores[(size_t)g * a.k + n] = -INFINITY;
-        a.out_beams[(size_t)g * a.k + n] = (uint32_t)(at / vocab);
-        a.out_tokens[(size_t)g * a.k + n] = (uint32_t)(at % vocab);
+        if (tid == 0) put(c, best, at);   // (more than fit into the list: k of them exist)
     }
 }
+
+// Pieces of 8192 tokens where that makes two blocks a CU, else of 2048.
+static uint32_t beam_piece(uint32_t groups, uint32_t beams, uint32_t vocab) { return (uint64_t)groups * beams * ((vocab + 8191u) / 8192u) >= 512u ? 8192u : 2048u; }
 
 fk_status beam_select_workspace_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k, size_t* bytes) {
     if (!bytes) return set_error(FK_ERR_INVALID, "beam_select workspace: null pointer");
     if (groups == 0 || beams == 0 || vocab == 0 || k == 0) return set_error(FK_ERR_INVALID, "beam_select: empty shape");
     if (beams > kBeamMax || k > kBeamMax) return set_error(FK_ERR_UNSUPPORTED, "beam_select: beams and k up to 64");
+    if (groups > kBeamGroups) return set_error(FK_ERR_UNSUPPORTED, "beam_select: more than 4096 groups");
     if ((uint64_t)groups * beams > 65535) return set_error(FK_ERR_UNSUPPORTED, "beam_select: more than 65535 beams in all groups");
     if (k > (uint64_t)beams * vocab) return set_error(FK_ERR_INVALID, "beam_select: k exceeds the continuations of a group");
-    *bytes = (size_t)groups * beams * 8 * (1 + k);
+    const size_t rows = (size_t)groups * beams, pieces = ((size_t)vocab + 2047) / 2048;   // (the smaller pieces, whichever are taken)
+    if (pieces > 65535) return set_error(FK_ERR_UNSUPPORTED, "beam_select: vocabulary too large");
+    *bytes = kBeamCounterBytes + rows * pieces * (12 + 4 * (size_t)k);
     return FK_OK;
 }
 
@@ -165,19 +374,17 @@ fk_status plan_beam_select(const uint16_t* logits, size_t row_stride, const floa
     if (workspace_bytes < need) return set_error(FK_ERR_INVALID, "beam_select: workspace too small");
     const DeviceFacts* dev;
     FK_TRY(device_facts(&dev));
-    BeamArgs a{logits, row_stride, scores, finished, pad_token, groups, beams, vocab, k, out_scores, out_beams, out_tokens, nullptr, nullptr};
-    a.base = static_cast<double*>(workspace);
-    a.best = reinterpret_cast<uint64_t*>(a.base + (size_t)groups * beams);
-    l->func = reinterpret_cast<const void*>(&beam_rows_kernel);
-    l->grid = dim3(groups * beams, 1, 1);
+    const uint32_t piece = beam_piece(groups, beams, vocab), pieces = (vocab + piece - 1) / piece;
+    const size_t rows = (size_t)groups * beams;
+    BeamArgs a{logits, row_stride, scores, finished, pad_token, beams, vocab, k, pieces, out_scores, out_beams, out_tokens, nullptr, nullptr, nullptr, nullptr};
+    a.arrived = static_cast<uint32_t*>(workspace);
+    a.sums = reinterpret_cast<double*>(static_cast<unsigned char*>(workspace) + kBeamCounterBytes);
+    a.tops = reinterpret_cast<float*>(a.sums + rows * pieces);
+    a.best = reinterpret_cast<uint32_t*>(a.tops + rows * pieces);
+    l->func = piece == 8192 ? reinterpret_cast<const void*>(&beam_select_kernel<4>) : reinterpret_cast<const void*>(&beam_select_kernel<1>);
+    l->grid = dim3(pieces, (uint32_t)rows, 1);
     l->block = dim3(256, 1, 1);
     l->set_args(a);
-    Launch m;
-    m.func = reinterpret_cast<const void*>(&beam_merge_kernel);
-    m.grid = dim3(groups, 1, 1);
-    m.block = dim3(64, 1, 1);
-    m.set_args(a);
-    l->then.push_back(m);
     return FK_OK;
 }
 

@@ -121,10 +121,12 @@ def test_first_step(fk):
 
 
 def test_a_workspace_serves_one_call_after_another(fk):
-    ws = fk.zeros(fk.beam_select_workspace_bytes(4, 8, 20000, 16))
+    """Whatever its shape: also many groups behind one, whose counters lie where sums might have lain."""
+    ws = fk.zeros(fk.beam_select_workspace_bytes(40, 8, 20000, 16))
     for i in range(3):
         check(fk, *make(20 + i, 4, 8, 20000), 4, 8, 16, workspace=ws)
         check(fk, *make(30 + i, 1, 3, 500), 1, 3, 4, workspace=ws)
+        check(fk, *make(40 + i, 40, 2, 700), 40, 2, 4, workspace=ws)
 
 
 @pytest.mark.parametrize("row_bytes", [1, 3, 4, 16, 20, 1000, 4096, 65552])
