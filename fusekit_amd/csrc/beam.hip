@@ -6,21 +6,27 @@
 // contributes only its k largest logits; rows are then compared in 64 bits.
 #include <math.h>
 
+#include <algorithm>
+
 #include "argmax_tail.hpp"
 #include "fk_host.hpp"
 
 namespace fk {
 
 constexpr uint32_t kBeamMax = 64, kBeamGroups = 4096;
-constexpr size_t kBeamCounterBytes = 4 * kBeamGroups;   // at the same place for every shape: a workspace serves one call after another
+// A group's counter has a line of its own: atomics on one line follow one another, also on different words of it (2432 arrivals of 16 groups in
+// one line: 18 us).  They lie at the same place for every shape: a workspace serves one call after another.
+constexpr uint32_t kBeamCounterStep = 32;
+constexpr size_t kBeamCounterBytes = (size_t)4 * kBeamCounterStep * kBeamGroups;
 
 // One launch.  A block takes a piece of a row: it leaves the piece's largest logit, its sum of exponentials and its k largest logits in order; the
 // block of a group that comes last forms lse and the k best of what all pieces left.  The pieces are cut by token, never by address: rows that
 // hold the same values have the same sums wherever they lie, so that ties between beams stay ties.
 //
-// The k largest of a piece without sorting it: the k-th largest of the 256 threads' largest values is a bound that at least k values reach and few
-// more (16 of 256: 17 on average); found by bisection over its 16 bits with ballots.  What reaches it is collected in LDS and ranked by counting.
-// Only a piece full of ties has more than fit there: its k largest are then taken one by one.
+// The k largest of a piece without sorting it: the k-th largest of the maxima of 64 (beyond k = 24: 256) parts of it is a bound that at least k
+// values reach and few more; found by bisection over its 16 bits with ballots.  What reaches it is collected in LDS and ranked by counting.
+// Only a piece full of ties has more than fit there: its k largest are then taken one by one.  Logits are compared two at a time as 16-bit
+// integers: with a negative one's magnitude negated, bf16 values are in order (and -0 is 0).
 struct BeamArgs {
     const uint16_t* logits;
     size_t row_stride;
@@ -30,13 +36,15 @@ struct BeamArgs {
     float* out_scores;
     uint32_t* out_beams;
     uint32_t* out_tokens;
-    uint32_t* arrived;   // [groups], zero before the first launch, left zero
+    uint32_t* arrived;   // [groups][kBeamCounterStep], zero before the first launch, left zero
     double* sums;        // [groups * beams][pieces]
     float* tops;         // [groups * beams][pieces]
     uint32_t* best;      // [groups * beams][pieces][k]: (order of the logit << 16) | (65535 - place in the piece), 0 where there are no more
 };
 
-constexpr uint32_t kBeamList = 512;   // candidates that fit in LDS
+constexpr uint32_t kBeamList = 512, kBeamPart = kBeamList / 4;   // candidates that fit in LDS, of a wave
+constexpr float kBeamLog2E = 1.44269504088896341f;
+typedef short i16x2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ double wave_sum_wide(double v) {
 #pragma unroll
@@ -44,25 +52,36 @@ __device__ __forceinline__ double wave_sum_wide(double v) {
     return v;
 }
 
-// The largest bound that at least k of the block's 256 values reach, or 1 where fewer than k are not 0; `all`: LDS, 256 words.
+// Two logits as integers in their order; the float that an order stands for; the smallest order above -inf.
+__device__ __forceinline__ i16x2_t beam_order(uint32_t w) {
+    const i16x2_t x = __builtin_bit_cast(i16x2_t, w), s = x >> 15;
+    return (x ^ (s & 0x7fff)) - s;
+}
+__device__ __forceinline__ float beam_value(int order) { return __uint_as_float((uint32_t)(order < 0 ? 0x8000 | -order : order) << 16); }
+constexpr int kBeamLeast = -0x7f80 + 1;
+
+// A bound that at least k of what the block's threads hold reach, the k-th largest of their `mine` or of the maxima of four of them (k up to 24), or
+// 0 where fewer than k are not 0; its bits below LOW are not looked for.  `all`: LDS, 256 words.
 template <int BITS, int LOW>
 __device__ __forceinline__ uint32_t bound_of_best(uint32_t mine, uint32_t k, uint32_t* all) {
     const uint32_t lane = threadIdx.x & 63u;
     all[threadIdx.x] = mine;
     __syncthreads();
-    uint32_t v[4];
+    uint32_t v[4], t = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = all[lane + 64u * i];
-    uint32_t t = 0;
-#pragma unroll 1
-    for (int bit = LOW + BITS - 1; bit >= LOW; --bit) {
-        const uint32_t at = t | (1u << bit);
-        uint32_t n = 0;
+    auto count = [&](uint32_t x, uint32_t at) { return (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(x >= at)); };
+    if (k <= 24u) {
+        const uint32_t a = v[0] > v[1] ? v[0] : v[1], b = v[2] > v[3] ? v[2] : v[3], m = a > b ? a : b;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) n += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] >= at));
-        if (n >= k) t = at;
+        for (int bit = BITS - 1; bit >= LOW; --bit)
+            if (count(m, t | (1u << bit)) >= k) t |= 1u << bit;
+    } else {
+#pragma unroll 1
+        for (int bit = BITS - 1; bit >= LOW; --bit)
+            if (count(v[0], t | (1u << bit)) + count(v[1], t | (1u << bit)) + count(v[2], t | (1u << bit)) + count(v[3], t | (1u << bit)) >= k) t |= 1u << bit;
     }
-    return t ? t : 1u;
+    return t;
 }
 
 template <int VEC>   // 16-byte loads of a thread
@@ -70,9 +89,14 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
     constexpr uint32_t PIECE = 2048u * VEC;
     typedef uint32_t loose __attribute__((ext_vector_type(4), aligned(2)));   // (rows of an odd length start anywhere)
     __shared__ uint32_t all[256];
-    __shared__ uint32_t list[kBeamList];
+    __shared__ uint4 list4[kBeamList / 4];
+    uint32_t* const list = reinterpret_cast<uint32_t*>(list4);
     __shared__ double values[kBeamList], part[4], base[kBeamMax];
-    __shared__ uint32_t n_list, flag;
+    __shared__ uint64_t flats[kBeamList];
+    __shared__ uint32_t counts[4], flag, ended[kBeamMax];
+    __shared__ float near[kBeamMax];
+    constexpr uint32_t AHEAD = 6;
+    __shared__ uint32_t keys[AHEAD * 256u];
     __shared__ float top[4];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     const uint32_t piece = blockIdx.x, row = blockIdx.y, g = row / a.beams, k = a.k;
@@ -80,78 +104,134 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
     const bool over = a.finished && a.finished[row];   // (the same for the block)
     if (!over) {
         const uint16_t* x = a.logits + (size_t)row * a.row_stride + from;
-        loose w[VEC];
+        uint32_t w[VEC * 4];
+        if (left >= PIECE) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const uint32_t at = ((uint32_t)i * 256u + tid) * 8u;
-            if (at + 8u <= left) {
-                w[i] = *reinterpret_cast<const loose*>(x + at);
-            } else {
+            for (int i = 0; i < VEC; ++i) {
+                const loose v = *reinterpret_cast<const loose*>(x + ((uint32_t)i * 256u + tid) * 8u);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t lo = at + 2u * e < left ? x[at + 2u * e] : 0xff80u, hi = at + 2u * e + 1u < left ? x[at + 2u * e + 1u] : 0xff80u;
-                    w[i][e] = lo | hi << 16;
+                for (int e = 0; e < 4; ++e) w[i * 4 + e] = v[e];
+            }
+        } else {   // the row's last piece: -inf behind its end
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const uint32_t at = ((uint32_t)i * 256u + tid) * 8u;
+                loose v = {0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
+                if (at + 8u <= left) {
+                    v = *reinterpret_cast<const loose*>(x + at);
+                } else if (at < left) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t lo = at + 2u * e < left ? x[at + 2u * e] : 0xff80u, hi = at + 2u * e + 1u < left ? x[at + 2u * e + 1u] : 0xff80u;
+                        v[e] = lo | hi << 16;
+                    }
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[i * 4 + e] = v[e];
             }
         }
-        // (a NaN counts as -inf: the larger of the two)
-        auto value = [&](int i, int e) { return fmaxf(e & 1 ? bf16_hi(w[i][e >> 1]) : bf16_lo(w[i][e >> 1]), -INFINITY); };
-        float m = -INFINITY;
+        int most;
+        float mw;
+        double sum;
+#pragma unroll 1
+        for (int pass = 0;; ++pass) {
+            i16x2_t m2 = beam_order(w[0]);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
+            for (int i = 1; i < VEC * 4; ++i) m2 = __builtin_elementwise_max(m2, beam_order(w[i]));
+            most = m2[0] > m2[1] ? m2[0] : m2[1];
+            mw = wave_max(beam_value(most));
+            // exp(x - m) as 2^(x L - r), one rounding in the exponent, r the rounded m L: what r and L are off by is put right below
+            const float ref = mw == -INFINITY ? 0.f : mw, r = ref * kBeamLog2E;
+            sum = 0.0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m = fmaxf(m, value(i, e));
-        const float mw = wave_max(m), ref = mw == -INFINITY ? 0.f : mw;
-        double sum = 0.0;
+            for (int i = 0; i < VEC * 2; ++i) {
+                const float e0 = __builtin_amdgcn_exp2f(fmaf(bf16_lo(w[2 * i]), kBeamLog2E, -r)), e1 = __builtin_amdgcn_exp2f(fmaf(bf16_hi(w[2 * i]), kBeamLog2E, -r));
+                const float e2 = __builtin_amdgcn_exp2f(fmaf(bf16_lo(w[2 * i + 1]), kBeamLog2E, -r)), e3 = __builtin_amdgcn_exp2f(fmaf(bf16_hi(w[2 * i + 1]), kBeamLog2E, -r));
+                sum += (double)((e0 + e1) + (e2 + e3));
+            }
+            sum = wave_sum_wide(sum);
+            sum *= 1.0 - 0.69314718055994531 * ((double)ref * (double)kBeamLog2E - (double)r);
+            if (pass != 0 || sum == sum) break;
+            // a NaN among them: it counts as -inf (and an infinity's sum stays what it is)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            float s8[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s8[e] = __builtin_amdgcn_exp2f((value(i, e) - ref) * 1.44269504088896341f);
-            sum += (double)((s8[0] + s8[1]) + (s8[2] + s8[3])) + (double)((s8[4] + s8[5]) + (s8[6] + s8[7]));
+            for (int i = 0; i < VEC * 4; ++i) {
+                if ((w[i] & 0x7fffu) > 0x7f80u) w[i] = (w[i] & 0xffff0000u) | 0xff80u;
+                if ((w[i] & 0x7fff0000u) > 0x7f800000u) w[i] = (w[i] & 0xffffu) | 0xff800000u;
+            }
         }
-        sum = wave_sum_wide(sum);
         if (lane == 0) {
             top[wave] = mw;
             part[wave] = sum;
         }
-        if (tid == 0) n_list = 0;
-        const uint32_t bound = bound_of_best<16, 16>(m == -INFINITY ? 0u : order_key(m + 0.0f), k, all);   // (-0 as 0)
-        const float least = __uint_as_float(bound >= 0x80000000u ? (bound & 0x7fff0000u) : (~bound & 0xffff0000u));   // (bound 1: a NaN's pattern)
-        const bool any = bound < 0x10000u;
+        const uint32_t found = bound_of_best<16, 0>(most >= kBeamLeast ? (uint32_t)(most + 0x8000) : 0u, k, all);
+        int bound = (int)found - 0x8000;
+        bound = bound < kBeamLeast ? kBeamLeast : bound;
+        auto entry = [&](int order, int i, int h) { return (uint32_t)(order + 0x8000) << 16 | (0xffffu - (((uint32_t)(i / 4) * 256u + tid) * 8u + (uint32_t)((i % 4) * 2 + h))); };
+        auto again = [&] {   // (the orders are formed anew, not kept: two registers a word are what lets fewer blocks stand on a CU)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
+            for (int i = 0; i < VEC * 4; ++i) asm volatile("" : "+v"(w[i]));
+        };
+        again();
+        // a wave's part of the list, without a counter to wait for
+        uint32_t mine = 0;   // entries of this wave so far
+        {
+            const i16x2_t below = {(short)(bound - 1), (short)(bound - 1)};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float v = value(i, e);
-                if (v > -INFINITY && (any || v >= least)) {
-                    const uint32_t at = atomicAdd(&n_list, 1u);
-                    if (at < kBeamList) list[at] = (order_key(v + 0.0f) & 0xffff0000u) | (0xffffu - (((uint32_t)i * 256u + tid) * 8u + e));
+            for (int i = 0; i < VEC * 4; ++i) {
+                const i16x2_t o = beam_order(w[i]), reached = __builtin_elementwise_max(o, below);
+                if (__builtin_amdgcn_ballot_w64(__builtin_bit_cast(uint32_t, reached) != __builtin_bit_cast(uint32_t, below)) == 0) continue;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const unsigned long long in = __builtin_amdgcn_ballot_w64(o[h] >= bound);
+                    const uint32_t at = mine + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0u));
+                    if (o[h] >= bound && at < kBeamPart) list[wave * kBeamPart + at] = entry(o[h], i, h);
+                    mine += (uint32_t)__builtin_popcountll(in);
                 }
             }
+        }
+        if (lane == 0) counts[wave] = mine;
+        if (lane < 4u && mine + lane < kBeamPart) list[wave * kBeamPart + mine + lane] = 0u;   // (read four at a time below)
         __syncthreads();
-        const uint32_t n = n_list;
+        const uint32_t n = counts[0] + counts[1] + counts[2] + counts[3];
+        const bool fits = counts[0] <= kBeamPart && counts[1] <= kBeamPart && counts[2] <= kBeamPart && counts[3] <= kBeamPart;
         uint32_t* const out = a.best + ((size_t)row * a.pieces + piece) * k;
-        if (n <= kBeamList) {
-            for (uint32_t c = tid; c < n; c += 256u) {
-                const uint32_t mine = list[c];
+        if (fits && n <= 64u) {   // one wave, an entry a lane
+            if (wave == 0) {
+                const uint32_t c0 = counts[0], c1 = c0 + counts[1], c2 = c1 + counts[2];
+                const uint32_t at = lane < c0 ? lane : lane < c1 ? kBeamPart + lane - c0 : lane < c2 ? 2u * kBeamPart + lane - c1 : 3u * kBeamPart + lane - c2;
+                const uint32_t key = lane < n ? list[at] : 0u, all_n = __builtin_amdgcn_readfirstlane(n);
                 uint32_t rank = 0;
-                for (uint32_t o = 0; o < n; ++o) rank += list[o] > mine ? 1u : 0u;
-                if (rank < k) __hip_atomic_store(&out[rank], mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                for (uint32_t o = 0; o < all_n; ++o) rank += (uint32_t)__builtin_amdgcn_readlane((int)key, (int)o) > key ? 1u : 0u;
+                if (lane < n && rank < k) __hip_atomic_store(&out[rank], key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (lane >= n && lane < k) __hip_atomic_store(&out[lane], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        } else if (fits) {
+            for (uint32_t c = lane; c < mine; c += 64u) {
+                const uint32_t key = list[wave * kBeamPart + c];
+                uint32_t rank = 0;
+                for (uint32_t p = 0; p < 4u; ++p)
+                    for (uint32_t o = 0; o < counts[p]; o += 4u) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(&list[p * kBeamPart + o]);
+                        rank += (v.x > key ? 1u : 0u) + (v.y > key ? 1u : 0u) + (v.z > key ? 1u : 0u) + (v.w > key ? 1u : 0u);
+                    }
+                if (rank < k) __hip_atomic_store(&out[rank], key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             for (uint32_t c = n + tid; c < k; c += 256u) __hip_atomic_store(&out[c], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         } else {
             uint32_t last = ~0u;
+#pragma unroll 1
             for (uint32_t c = 0; c < k; ++c) {
                 uint32_t best = 0;
+                again();
 #pragma unroll
-                for (int i = 0; i < VEC; ++i)
+                for (int i = 0; i < VEC * 4; ++i) {
+                    const i16x2_t o = beam_order(w[i]);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float v = value(i, e);
-                        const uint32_t key = v > -INFINITY ? (order_key(v + 0.0f) & 0xffff0000u) | (0xffffu - (((uint32_t)i * 256u + tid) * 8u + e)) : 0u;
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t key = o[h] >= kBeamLeast ? entry(o[h], i, h) : 0u;
                         best = key < last && key > best ? key : best;
                     }
+                }
 #pragma unroll
                 for (int o = 32; o > 0; o >>= 1) {
                     const uint32_t other = __shfl_xor(best, o, 64);
@@ -169,7 +249,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
         if (tid == 0) {
             const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), rt = mt == -INFINITY ? 0.f : mt;
             double s = 0.0;
-            for (int i = 0; i < 4; ++i) s += part[i] * (double)__builtin_amdgcn_exp2f((top[i] - rt) * 1.44269504088896341f);
+            for (int i = 0; i < 4; ++i) s += part[i] * (double)__builtin_amdgcn_exp2f((top[i] - rt) * kBeamLog2E);
             const size_t at = (size_t)row * a.pieces + piece;
             __hip_atomic_store(&a.tops[at], mt, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __hip_atomic_store(reinterpret_cast<unsigned long long*>(&a.sums[at]), (unsigned long long)__double_as_longlong(s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -179,121 +259,161 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
     // ---- the group's last block ----
     wait_memory_ops_done();
     __syncthreads();
-    if (tid == 0) flag = atomicAdd(&a.arrived[g], 1u) == a.beams * a.pieces - 1u ? 1u : 0u;
+    if (tid == 0) flag = atomicAdd(&a.arrived[g * kBeamCounterStep], 1u) == a.beams * a.pieces - 1u ? 1u : 0u;
     __syncthreads();
     if (!flag) return;
-    if (tid == 0) {
-        __hip_atomic_store(&a.arrived[g], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        n_list = 0;
-    }
-    for (uint32_t b = wave; b < a.beams; b += 4u) {
-        const uint32_t r = g * a.beams + b;
-        const float score = a.scores[r];
-        if (a.finished && a.finished[r]) {
-            if (lane == 0) base[b] = (double)score;
-            continue;
-        }
-        float m = -INFINITY;
-        for (uint32_t p = lane; p < a.pieces; p += 64u) m = fmaxf(m, __hip_atomic_load(&a.tops[(size_t)r * a.pieces + p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-        m = wave_max(m);
-        double s = 0.0;
-        for (uint32_t p = lane; p < a.pieces; p += 64u) {
-            const size_t at = (size_t)r * a.pieces + p;
-            const float mp = __hip_atomic_load(&a.tops[at], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const double sp = __longlong_as_double((long long)__hip_atomic_load(reinterpret_cast<unsigned long long*>(&a.sums[at]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-            if (mp > -INFINITY) s += sp * exp((double)mp - (double)m);
-        }
-        s = wave_sum_wide(s);
-        if (lane == 0) base[b] = (double)score - ((double)m + log(s));
-    }
-    __syncthreads();
-    const uint32_t row_n = a.pieces * k, total = a.beams * row_n;
+    if (tid == 0) __hip_atomic_store(&a.arrived[g * kBeamCounterStep], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint32_t total = a.beams * a.pieces * k;
     const uint32_t* const group_best = a.best + (size_t)g * total;
-    // candidate i of the group: its score and its place, or -inf
-    auto candidate = [&](uint32_t i, uint32_t key, uint64_t& flat) {
-        const uint32_t b = i / row_n, j = i - b * row_n;
-        if (a.finished && a.finished[g * a.beams + b]) {
-            flat = (uint64_t)b * a.vocab + a.pad;
-            return j == 0 ? base[b] : (double)-INFINITY;
-        }
-        flat = (uint64_t)b * a.vocab + (j / k) * PIECE + (0xffffu - (key & 0xffffu));
-        const uint32_t o = key & 0xffff0000u;
-        const double v = base[b] + (double)__uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o & 0xffff0000u);
-        return key && v > -INFINITY ? v : (double)-INFINITY;
-    };
-    constexpr uint32_t AHEAD = 8;
     auto load = [&](uint32_t i) { return i < total ? __hip_atomic_load(&group_best[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0u; };
     // (of a finished row nothing was written: its keys are not looked at, whatever they are)
-    uint32_t mine = 0;
-    uint32_t kept[AHEAD];
-    for (uint32_t at = 0; at < total; at += 256u * AHEAD) {
+    // The first entries of all lists go into LDS with one request, as many of each as fit.
+    const uint32_t lists = a.beams * a.pieces, deep = lists * k <= AHEAD * 256u ? k : AHEAD * 256u / lists;
+    if (deep) {
+        const uint32_t whole = lists * deep;
         uint32_t key[AHEAD];
 #pragma unroll
-        for (uint32_t u = 0; u < AHEAD; ++u) key[u] = load(at + u * 256u + tid);
-#pragma unroll
         for (uint32_t u = 0; u < AHEAD; ++u) {
-            const uint32_t i = at + u * 256u + tid;
-            if (i >= total) continue;
-            uint64_t flat;
-            const double v = candidate(i, key[u], flat);
-            if (v > -INFINITY) {
-                const uint32_t o = order_key((float)v);
-                mine = o > mine ? o : mine;
-            }
+            const uint32_t i = u * 256u + tid, l = i / deep;
+            key[u] = i < whole ? load(l * k + (i - l * deep)) : 0u;
         }
-        if (at == 0) {
 #pragma unroll
-            for (uint32_t u = 0; u < AHEAD; ++u) kept[u] = key[u];
+        for (uint32_t u = 0; u < AHEAD; ++u) keys[u * 256u + tid] = key[u];
+    }
+    auto key_of = [&](uint32_t l, uint32_t j) { return j < deep ? keys[l * deep + j] : load(l * k + j); };
+    const uint32_t of_beam = g * a.beams + (tid < a.beams ? tid : 0u), is_over = a.finished ? a.finished[of_beam] : 0u;
+    const float score = a.scores[of_beam];
+    for (uint32_t b0 = wave; b0 < a.beams; b0 += 16u) {   // four beams of a wave with one request
+        float m4[4];
+        double s4[4];
+        auto sums_of = [&](uint32_t b, uint32_t p, float& mp, double& sp) {
+            const size_t at = (size_t)(g * a.beams + (b < a.beams ? b : b0)) * a.pieces + (p < a.pieces ? p : a.pieces - 1u);
+            mp = __hip_atomic_load(&a.tops[at], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            sp = __longlong_as_double((long long)__hip_atomic_load(reinterpret_cast<unsigned long long*>(&a.sums[at]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        };
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) sums_of(b0 + 4u * u, lane, m4[u], s4[u]);
+#pragma unroll 1
+        for (uint32_t u = 0; u < 4; ++u) {
+            const uint32_t b = b0 + 4u * u;
+            if (b >= a.beams) break;
+            float m = wave_max(m4[0]), ref = m == -INFINITY ? 0.f : m;   // the sum is relative to m, which is the wave's
+            double s = lane < a.pieces ? s4[0] * (double)__builtin_amdgcn_exp2f((m4[0] - ref) * kBeamLog2E) : 0.0;
+            for (uint32_t p0 = 64u; p0 < a.pieces; p0 += 64u) {
+                float mp;
+                double sp;
+                sums_of(b, p0 + lane, mp, sp);
+                const float mn = fmaxf(m, wave_max(mp));
+                ref = mn == -INFINITY ? 0.f : mn;
+                s = s * (double)__builtin_amdgcn_exp2f((m - ref) * kBeamLog2E) +
+                    (p0 + lane < a.pieces ? sp * (double)__builtin_amdgcn_exp2f((mp - ref) * kBeamLog2E) : 0.0);
+                m = mn;
+            }
+            s = wave_sum_wide(s);
+            if (lane == 0) {
+                values[b] = (double)m;
+                values[kBeamMax + b] = s;
+            }
+            m4[0] = m4[1], m4[1] = m4[2], m4[2] = m4[3];
+            s4[0] = s4[1], s4[1] = s4[2], s4[2] = s4[3];
         }
     }
-    const uint32_t bound = bound_of_best<32, 0>(mine, k, all);
-    auto collect = [&](uint32_t i, uint32_t key) {
-        if (i >= total) return;
-        uint64_t flat;
-        const double v = candidate(i, key, flat);
-        if (v > -INFINITY && order_key((float)v) >= bound) {
-            const uint32_t at = atomicAdd(&n_list, 1u);
-            if (at < kBeamList) {
-                list[at] = i;
-                values[at] = v;
-            }
-        }
-    };
-#pragma unroll
-    for (uint32_t u = 0; u < AHEAD; ++u) collect(u * 256u + tid, kept[u]);
-    for (uint32_t i = 256u * AHEAD + tid; i < total; i += 256u) collect(i, load(i));
     __syncthreads();
-    uint32_t n = n_list;
+    if (tid < a.beams) {
+        ended[tid] = is_over;
+        base[tid] = is_over ? (double)score : (double)score - (values[tid] + log(values[kBeamMax + tid]));
+        near[tid] = (float)base[tid];
+    }
+    __syncthreads();
+    // Entry j of list l (a piece's, in order): its fp32 score, off by less than `margin`, or -inf; and in 64 bits, with its place as beam << 32 |
+    // token, which is in the order of beam * vocab + token.  A finished row's one candidate is the first entry of its first piece.
+    auto rough = [&](uint32_t b, uint32_t p, uint32_t j, uint32_t key, float& margin) {
+        const float c = near[b], x = ended[b] ? 0.f : beam_value((int)(key >> 16) - 0x8000), v = c + x;
+        margin = fminf(fmaxf(__builtin_fabsf(c), __builtin_fabsf(x)) * 0x1p-22f, 1e30f);
+        return (ended[b] ? (p | j) == 0u : key != 0u) && v > -INFINITY ? v : -INFINITY;
+    };
+    auto exactly = [&](uint32_t b, uint32_t p, uint32_t j, uint32_t key, uint64_t& flat) {
+        if (ended[b]) {
+            flat = (uint64_t)b << 32 | a.pad;
+            return (p | j) == 0u ? base[b] : (double)-INFINITY;
+        }
+        flat = (uint64_t)b << 32 | (p * PIECE + (0xffffu - (key & 0xffffu)));
+        const double v = base[b] + (double)beam_value((int)(key >> 16) - 0x8000);
+        return key && v > -INFINITY ? v : (double)-INFINITY;
+    };
+    // The bound: of up to 256 lists from the first 256 / lists entries of each, of more from their first.  k fp32 scores less their margins reach it,
+    // so that k scores do.
+    uint32_t mine = 0;
+#pragma unroll 1
+    for (uint32_t l0 = tid; l0 < (lists < 256u ? 256u : lists); l0 += 256u) {
+        const uint32_t j = lists < 256u ? l0 / lists : 0u, l = lists < 256u ? l0 - j * lists : l0;
+        if (j >= k) break;
+        const uint32_t b = l / a.pieces;
+        float margin;
+        const float v = rough(b, l - b * a.pieces, j, key_of(l, j), margin);
+        const uint32_t o = v > -INFINITY ? order_key(v - margin) : 0u;
+        mine = o > mine ? o : mine;
+    }
+    const uint32_t bound = bound_of_best<32, 12>(mine, k, all);
+    // Who reaches it: a thread goes down a list as far as fp32 scores with their margins do, and looks at those in 64 bits.
+    uint32_t found_here = 0;   // of this wave
+    __syncthreads();           // (the sums that lay in `values` have been read)
+#pragma unroll 1
+    for (uint32_t l0 = 0; l0 < lists; l0 += 256u) {
+        const uint32_t l = l0 + tid < lists ? l0 + tid : 0u, b = l / a.pieces, p = l - b * a.pieces;
+        bool on = l0 + tid < lists;
+#pragma unroll 1
+        for (uint32_t j = 0; j < k; ++j) {
+            const uint32_t key = on ? key_of(l, j) : 0u;
+            float margin;
+            const float near_v = rough(b, p, j, key, margin);
+            on = on && near_v > -INFINITY && order_key(near_v + margin) >= bound;
+            if (__builtin_amdgcn_ballot_w64(on) == 0) break;
+            uint64_t flat;
+            const double v = exactly(b, p, j, key, flat);
+            const bool is = on && v > -INFINITY && order_key((float)v) >= bound;
+            const unsigned long long in = __builtin_amdgcn_ballot_w64(is);
+            const uint32_t at = found_here + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0u));
+            if (is && at < kBeamPart) {
+                values[wave * kBeamPart + at] = v;
+                flats[wave * kBeamPart + at] = flat;
+            }
+            found_here += (uint32_t)__builtin_popcountll(in);
+        }
+    }
+    if (lane == 0) counts[wave] = found_here;
+    __syncthreads();
+    const uint32_t n = counts[0] + counts[1] + counts[2] + counts[3];
+    const bool fits = counts[0] <= kBeamPart && counts[1] <= kBeamPart && counts[2] <= kBeamPart && counts[3] <= kBeamPart;
     auto put = [&](uint32_t at, double v, uint64_t flat) {
         a.out_scores[(size_t)g * k + at] = (float)v;
-        a.out_beams[(size_t)g * k + at] = (uint32_t)(flat / a.vocab);
-        a.out_tokens[(size_t)g * k + at] = (uint32_t)(flat % a.vocab);
+        a.out_beams[(size_t)g * k + at] = (uint32_t)(flat >> 32);
+        a.out_tokens[(size_t)g * k + at] = (uint32_t)flat;
     };
-    if (n <= kBeamList) {
-        // their places in LDS too, then each one's rank by counting
-        __shared__ uint64_t flats[kBeamList];
-        for (uint32_t c = tid; c < n; c += 256u) {
-            uint64_t flat;
-            candidate(list[c], load(list[c]), flat);
-            flats[c] = flat;
-        }
-        __syncthreads();
-        for (uint32_t c = tid; c < n; c += 256u) {
-            const double v = values[c];
-            const uint64_t flat = flats[c];
+    if (fits) {
+        for (uint32_t c = lane; c < found_here; c += 64u) {
+            const double v = values[wave * kBeamPart + c];
+            const uint64_t flat = flats[wave * kBeamPart + c];
             uint32_t rank = 0;
-            for (uint32_t o = 0; o < n; ++o) rank += values[o] > v || (values[o] == v && flats[o] < flat) ? 1u : 0u;
+            for (uint32_t p = 0; p < 4u; ++p)
+#pragma unroll 2
+                for (uint32_t o = p * kBeamPart; o < p * kBeamPart + counts[p]; ++o) {
+                    const double other = values[o];
+                    const uint64_t place = flats[o];
+                    rank += (uint32_t)(other > v) | ((uint32_t)(other == v) & (uint32_t)(place < flat));
+                }
             if (rank < k) put(rank, v, flat);
         }
         if (n >= k || tid != 0) return;
         // fewer than k above -inf: the lowest places that are not among them
         uint64_t at = 0;
-        for (uint32_t i = n; i < k; ++i, ++at) {
+        auto next = [&] { at = (uint32_t)at + 1u < a.vocab ? at + 1u : ((at >> 32) + 1u) << 32; };
+        for (uint32_t i = n; i < k; ++i, next()) {
             for (bool again = true; again;) {
                 again = false;
-                for (uint32_t c = 0; c < n; ++c)
-                    if (flats[c] == at) {
-                        ++at;
+                for (uint32_t c = 0; c < kBeamList; ++c)
+                    if (c % kBeamPart < counts[c / kBeamPart] && flats[c] == at) {
+                        next();
                         again = true;
                     }
             }
@@ -308,8 +428,9 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
         double best = -INFINITY;
         uint64_t at = ~0ull;
         for (uint32_t i = tid; i < total; i += 256u) {
+            const uint32_t l = i / k, b = l / a.pieces;
             uint64_t flat;
-            const double v = candidate(i, load(i), flat);
+            const double v = exactly(b, l - b * a.pieces, i - l * k, load(i), flat);
             if (!(v > -INFINITY) || (c && !(v < last || (v == last && flat > last_at)))) continue;
             if (v > best || (v == best && flat < at)) {
                 best = v;
@@ -327,15 +448,13 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
         __syncthreads();
         if (lane == 0) {
             values[wave] = best;
-            values[4 + wave] = __longlong_as_double((long long)at);
+            flats[wave] = at;
         }
         __syncthreads();
         for (int i = 0; i < 4; ++i) {
-            const double ov = values[i];
-            const uint64_t oa = (uint64_t)__double_as_longlong(values[4 + i]);
-            if (ov > best || (ov == best && oa < at)) {
-                best = ov;
-                at = oa;
+            if (values[i] > best || (values[i] == best && flats[i] < at)) {
+                best = values[i];
+                at = flats[i];
             }
         }
         last = best;
@@ -389,7 +508,9 @@ fk_status plan_beam_select(const uint16_t* logits, size_t row_stride, const floa
 }
 
 // ---- rows of state that follow the beams ----
-// A thread takes one column of a group: it reads that column of every row before it writes one, so that src may be dst.
+// A thread takes one column of a group and N of its output rows: it requests them all before it writes one.  In place N covers all rows (of 16-byte
+// columns up to 16: more would not stay in registers, and go by words); apart, eight rows a thread and a part of the grid for each eight.
+// Bound by the bytes; the two columns that a wave's rows share a line in cost nothing that shows.
 struct ReorderArgs {
     const void* src;
     void* dst;
@@ -401,21 +522,31 @@ template <typename T, uint32_t N>
 __global__ __launch_bounds__(256) void beam_reorder_kernel(const ReorderArgs a) {
     const size_t c = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (c >= a.columns) return;
-    const uint32_t g = blockIdx.y;
+    const uint32_t g = blockIdx.y, first = blockIdx.z * N;
     const T* src = static_cast<const T*>(a.src) + (size_t)g * a.beams * a.columns + c;
-    T* dst = static_cast<T*>(a.dst) + (size_t)g * a.n_out * a.columns + c;
+    T* dst = static_cast<T*>(a.dst) + ((size_t)g * a.n_out + first) * a.columns + c;
+    const uint32_t* parents = a.parents + (size_t)g * a.n_out + first;
+    const uint32_t rows = a.n_out - first;
     T v[N];
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i) {
-        if (i < a.n_out) {
-            const uint32_t p = a.parents[(size_t)g * a.n_out + i];
-            v[i] = src[(size_t)(p < a.beams ? p : a.beams - 1u) * a.columns];
-        }
+        const uint32_t p = parents[i < rows ? i : rows - 1u];
+        v[i] = src[(size_t)(p < a.beams ? p : a.beams - 1u) * a.columns];
     }
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i)
-        if (i < a.n_out) dst[(size_t)i * a.columns] = v[i];
+        if (i < rows) dst[(size_t)i * a.columns] = v[i];
 }
+
+namespace {
+// the smallest form whose threads hold N rows or more, or null
+template <typename T, uint32_t... N>
+const void* reorder_form(uint32_t rows, uint32_t* held) {
+    const void* f = nullptr;
+    ((f == nullptr && rows <= N ? (f = reinterpret_cast<const void*>(&beam_reorder_kernel<T, N>), *held = N) : 0u), ...);
+    return f;
+}
+}  // namespace
 
 fk_status plan_beam_reorder(const void* src, void* dst, size_t row_bytes, const uint32_t* parents, uint32_t groups, uint32_t beams, uint32_t n_out, Launch* l) {
     if (!src || !dst || !parents) return set_error(FK_ERR_INVALID, "beam_reorder: null pointer");
@@ -429,12 +560,15 @@ fk_status plan_beam_reorder(const void* src, void* dst, size_t row_bytes, const 
         return set_error(FK_ERR_INVALID, "beam_reorder: src and dst must be one buffer with n_out == beams, or not overlap");
     const DeviceFacts* dev;
     FK_TRY(device_facts(&dev));
-    const uint32_t width = (s0 | d0 | row_bytes) % 16 == 0 ? 16 : (s0 | d0 | row_bytes) % 4 == 0 ? 4 : 1;
+    const bool in_place = s0 == d0;
+    const uint32_t rows = in_place ? n_out : std::min(n_out, 8u);
+    const uint32_t width = (s0 | d0 | row_bytes) % 16 == 0 && rows <= 16 ? 16 : (s0 | d0 | row_bytes) % 4 == 0 ? 4 : 1;
     ReorderArgs a{src, dst, row_bytes / width, parents, beams, n_out};
     if ((a.columns + 255) / 256 > 0x7fffffffu) return set_error(FK_ERR_UNSUPPORTED, "beam_reorder: rows too long");
-    l->func = width == 16 ? reinterpret_cast<const void*>(&beam_reorder_kernel<uint4, kBeamMax>)
-              : width == 4 ? reinterpret_cast<const void*>(&beam_reorder_kernel<uint32_t, kBeamMax>) : reinterpret_cast<const void*>(&beam_reorder_kernel<uint8_t, kBeamMax>);
-    l->grid = dim3((uint32_t)((a.columns + 255) / 256), groups, 1);
+    uint32_t held = 1;
+    l->func = width == 16 ? reorder_form<fk_u32x4_t, 2, 4, 8, 16>(rows, &held)
+              : width == 4 ? reorder_form<uint32_t, 2, 4, 8, 16, 32, kBeamMax>(rows, &held) : reorder_form<uint8_t, 4, 16, kBeamMax>(rows, &held);
+    l->grid = dim3((uint32_t)((a.columns + 255) / 256), groups, (n_out + held - 1) / held);
     l->block = dim3(256, 1, 1);
     l->set_args(a);
     return FK_OK;

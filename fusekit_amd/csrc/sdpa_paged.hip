@@ -5,6 +5,8 @@
 // with p the row's position and c(x) = x, or softcap * tanh(x / softcap).
 #include <math.h>
 
+#include <algorithm>
+
 #include "fk_host.hpp"
 #include "mma32_device.hpp"
 #include "paged_device.hpp"
@@ -853,7 +855,10 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
         {{reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, true>)},
          {reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, true>)}}};
     l->func = p.few ? few[D == 128][softcap > 0.f][batch->max_rows * (n_heads / n_kv) > 8u] : tile[D == 128][softcap > 0.f];
-    l->grid = dim3((uint32_t)(p.slots ? p.slots : p.tiles), 1, 1);
+    // (no more blocks than there can be items: one that finds none costs what it takes to look)
+    const uint32_t step = p.few ? kFewRound : kTileStep, most = (batch->max_len + step - 1u) / step, splits = (most + p.min_steps - 1u) / p.min_steps;
+    const uint64_t items = p.slots ? std::min<uint64_t>(p.slots, p.tiles * splits) : p.tiles;
+    l->grid = dim3((uint32_t)items, 1, 1);
     l->block = dim3(256, 1, 1);
     l->shmem = p.few ? few_lds_bytes(D) : tile_lds_bytes(D);
     if ((int)l->shmem > dev->max_dyn_lds) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: LDS tile does not fit");
