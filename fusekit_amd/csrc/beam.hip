@@ -71,7 +71,7 @@ __device__ __forceinline__ uint32_t bound_of_best(uint32_t mine, uint32_t k, uin
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = all[lane + 64u * i];
     auto count = [&](uint32_t x, uint32_t at) { return (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(x >= at)); };
-    if (k <= 24u) {
+    if (__builtin_expect(k <= 24u, 1)) {
         const uint32_t a = v[0] > v[1] ? v[0] : v[1], b = v[2] > v[3] ? v[2] : v[3], m = a > b ? a : b;
 #pragma unroll
         for (int bit = BITS - 1; bit >= LOW; --bit)
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
     if (!over) {
         const uint16_t* x = a.logits + (size_t)row * a.row_stride + from;
         uint32_t w[VEC * 4];
-        if (left >= PIECE) {
+        if (__builtin_expect(left >= PIECE, 1)) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const loose v = *reinterpret_cast<const loose*>(x + ((uint32_t)i * 256u + tid) * 8u);
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
             }
             sum = wave_sum_wide(sum);
             sum *= 1.0 - 0.69314718055994531 * ((double)ref * (double)kBeamLog2E - (double)r);
-            if (pass != 0 || sum == sum) break;
+            if (__builtin_expect(pass != 0 || sum == sum, 1)) break;
             // a NaN among them: it counts as -inf (and an infinity's sum stays what it is)
 #pragma unroll
             for (int i = 0; i < VEC * 4; ++i) {
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
         const uint32_t n = counts[0] + counts[1] + counts[2] + counts[3];
         const bool fits = counts[0] <= kBeamPart && counts[1] <= kBeamPart && counts[2] <= kBeamPart && counts[3] <= kBeamPart;
         uint32_t* const out = a.best + ((size_t)row * a.pieces + piece) * k;
-        if (fits && n <= 64u) {   // one wave, an entry a lane
+        if (__builtin_expect(fits && n <= 64u, 1)) {   // one wave, an entry a lane
             if (wave == 0) {
                 const uint32_t c0 = counts[0], c1 = c0 + counts[1], c2 = c1 + counts[2];
                 const uint32_t at = lane < c0 ? lane : lane < c1 ? kBeamPart + lane - c0 : lane < c2 ? 2u * kBeamPart + lane - c1 : 3u * kBeamPart + lane - c2;
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
                 if (lane < n && rank < k) __hip_atomic_store(&out[rank], key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 if (lane >= n && lane < k) __hip_atomic_store(&out[lane], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
-        } else if (fits) {
+        } else if (__builtin_expect(fits, 1)) {
             for (uint32_t c = lane; c < mine; c += 64u) {
                 const uint32_t key = list[wave * kBeamPart + c];
                 uint32_t rank = 0;
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
     __syncthreads();
     if (tid == 0) flag = atomicAdd(&a.arrived[g * kBeamCounterStep], 1u) == a.beams * a.pieces - 1u ? 1u : 0u;
     __syncthreads();
-    if (!flag) return;
+    if (__builtin_expect(!flag, 1)) return;
     if (tid == 0) __hip_atomic_store(&a.arrived[g * kBeamCounterStep], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const uint32_t total = a.beams * a.pieces * k;
     const uint32_t* const group_best = a.best + (size_t)g * total;
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
             if (b >= a.beams) break;
             float m = wave_max(m4[0]), ref = m == -INFINITY ? 0.f : m;   // the sum is relative to m, which is the wave's
             double s = lane < a.pieces ? s4[0] * (double)__builtin_amdgcn_exp2f((m4[0] - ref) * kBeamLog2E) : 0.0;
-            for (uint32_t p0 = 64u; p0 < a.pieces; p0 += 64u) {
+            for (uint32_t p0 = 64u; __builtin_expect(p0 < a.pieces, 0); p0 += 64u) {
                 float mp;
                 double sp;
                 sums_of(b, p0 + lane, mp, sp);
@@ -390,7 +390,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
         a.out_beams[(size_t)g * k + at] = (uint32_t)(flat >> 32);
         a.out_tokens[(size_t)g * k + at] = (uint32_t)flat;
     };
-    if (fits) {
+    if (__builtin_expect(fits, 1)) {
         for (uint32_t c = lane; c < found_here; c += 64u) {
             const double v = values[wave * kBeamPart + c];
             const uint64_t flat = flats[wave * kBeamPart + c];
@@ -404,7 +404,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
                 }
             if (rank < k) put(rank, v, flat);
         }
-        if (n >= k || tid != 0) return;
+        if (__builtin_expect(n >= k || tid != 0, 1)) return;
         // fewer than k above -inf: the lowest places that are not among them
         uint64_t at = 0;
         auto next = [&] { at = (uint32_t)at + 1u < a.vocab ? at + 1u : ((at >> 32) + 1u) << 32; };
