@@ -83,22 +83,27 @@ __device__ __forceinline__ void paged_row(const SdpaPagedArgs& a, uint32_t seq, 
 }
 
 // ---- which piece of the work a block does ----
-// The columns of a sequence and KV head are its new rows times the query heads of a group, place * group + head; COLS of them are a tile.
-// A tile walks its positions in steps of STEP; where all tiles of the launch are fewer than `target` the steps are cut over several items.
-// Every wave finds its block's item by itself from the batch's arrays, 64 sequences with one request: lengths stay on the device.
+// The columns of a sequence and KV head are its new rows times the query heads of a group, place * group + head; 128 of them are a tile, and a
+// sequence of 16 or fewer goes by itself.  A tile walks its positions in steps of 64 (single tokens in rounds of 128); where all tiles of the
+// launch are fewer than `target` the steps are cut over several items.  Every wave finds its block's item by itself from the batch's arrays,
+// 64 sequences with one request: lengths stay on the device.
+constexpr uint32_t kTileCols = 128, kTileStep = 64;
+constexpr uint32_t kFewCols = 16, kFewStep = 32, kFewRound = 4 * kFewStep;
 struct PagedItem {
     uint32_t seq, kvh, tile, split, n_splits;
     PagedSeq s;
     bool any;
 };
-template <uint32_t COLS, uint32_t STEP>
+template <bool FEW>   // a launch of single tokens only
 __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t index, uint32_t lane) {
+    constexpr uint32_t STEP = FEW ? kFewRound : kTileStep;
     const uint32_t n_kv = a.b.n_kv;
-    auto tiles_of = [&](const PagedSeq& s) { return (uint32_t)(((uint64_t)s.rows * a.group + COLS - 1u) / COLS); };
+    auto tiles_of = [&](const PagedSeq& s) { return FEW ? (s.rows ? 1u : 0u) : (uint32_t)(((uint64_t)s.rows * a.group + kTileCols - 1u) / kTileCols); };
     auto steps_of = [&](const PagedSeq& s) {   // of a tile of the sequence, at most
         uint32_t seen = s.len;
         if (a.window) {
-            const uint64_t w = (uint64_t)a.window + (s.rows < COLS / a.group + 1u ? s.rows : COLS / a.group + 1u) + STEP - 1u;
+            const uint32_t span = FEW ? kFewCols : kTileCols / a.group + 1u;   // rows of a tile
+            const uint64_t w = (uint64_t)a.window + (s.rows < span ? s.rows : span) + STEP - 1u;
             seen = w < seen ? (uint32_t)w : seen;
         }
         return (seen + STEP - 1u) / STEP;
@@ -161,21 +166,20 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
     }
     return it;
 }
+constexpr int kPastCaches = 16;   // (sc1: what another block wrote, or is to read)
 
 // ---- tiles of 128 columns ----
 // A block is four waves of 32 columns on the same 64 positions a step.  The products and the softmax are those of the causal attention of one
 // sequence over a contiguous cache (sdpa_prefill.hip: S^T = K Q^T, a lane owns one query; O^T += V^T P^T with the score registers as they lie; V^T
 // through ds_read_b64_tr_b16; probabilities formed between the matrix instructions).  A wave requests 16 rows of K and of V a step, which lie
 // in one page: one page id, loaded two steps ahead into a scalar register.
-constexpr uint32_t kTileCols = 128, kTileStep = 64;
 constexpr uint32_t tile_lds_bytes(uint32_t d) {
     const uint32_t stage = 2u * 2u * kTileStep * d * 2u, outb = kTileCols * (d + 4u) * 4u;
     return (stage > outb ? stage : outb) + 16u;   // and a word for the block
 }
-constexpr int kPastCaches = 16;   // (sc1: what another block wrote, or is to read)
 
 template <int D, bool CAP>
-__global__ __launch_bounds__(256, 2) void sdpa_paged_tile_kernel(const SdpaPagedArgs a) {
+__device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedItem& it, uint32_t lane) {
     constexpr int KB = D / 16, DT = D / 32, VP = D / 8;
     constexpr uint32_t ROW = D * 2u, TILE = kTileStep * ROW, STAGE = 2u * TILE;      // bytes: a row, K (or V) of a step, both
     constexpr uint32_t RPI = 1024u / ROW;                                            // rows of one wave's request
@@ -183,9 +187,7 @@ __global__ __launch_bounds__(256, 2) void sdpa_paged_tile_kernel(const SdpaPaged
     extern __shared__ uint4 lds_raw[];
     unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_raw);
 
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kb = lane >> 5, nl = lane & 31u;
-    const PagedItem it = paged_item<kTileCols, kTileStep>(a, blockIdx.x, lane);
-    if (!it.any) return;
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kb = lane >> 5, nl = lane & 31u;
     const uint32_t G = a.group, columns = it.s.rows * G;   // (below 2^31: the host has checked)
     auto limit_of = [&](uint32_t place) { return it.s.len + place + 1u > it.s.rows ? it.s.len + place + 1u - it.s.rows : 0u; };   // positions a row may see end here
     auto low_of = [&](uint32_t limit) { return a.window && limit > a.window ? limit - a.window : 0u; };                           // and begin here
@@ -359,6 +361,7 @@ __global__ __launch_bounds__(256, 2) void sdpa_paged_tile_kernel(const SdpaPaged
         static_for<4>([&](auto w) __attribute__((always_inline)) { probabilities(std::integral_constant<int, 0>{}, w); });
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_nop 1");
+        __builtin_amdgcn_s_setprio(1);   // (ahead of the other block's wave, whose softmax fits between: 446 -> 429 us of two chunks of 2048 rows)
         static_for<4>([&](auto c) __attribute__((always_inline)) {
             static_for<DT>([&](auto i) __attribute__((always_inline)) {
                 const pf_u32x2_t lo = __builtin_bit_cast(pf_u32x2_t, vf[c()][i()][0]), hi = __builtin_bit_cast(pf_u32x2_t, vf[c()][i()][1]);
@@ -371,6 +374,7 @@ __global__ __launch_bounds__(256, 2) void sdpa_paged_tile_kernel(const SdpaPaged
             });
             asm volatile("s_nop 1");
         });
+        __builtin_amdgcn_s_setprio(0);
     }
     settle_matrix_ops();
 #pragma unroll
@@ -476,14 +480,13 @@ __global__ __launch_bounds__(256, 2) void sdpa_paged_tile_kernel(const SdpaPaged
 // instruction of its own.  A wave owns its steps of 32 positions and their place in LDS: it waits for no other wave until the block's waves
 // meet, its keys are requested again as soon as they are in registers, its values behind the second product.  Two blocks a CU keep 128 KB in
 // flight.  Bound by the bytes.
-constexpr uint32_t kFewCols = 16, kFewStep = 32, kFewRound = 4 * kFewStep;
 constexpr uint32_t few_lds_bytes(uint32_t d) {
     const uint32_t stages = 4u * kFewStep * d * 4u, meet = 4u * kFewCols * (d + 4u) * 4u + 2u * 4u * kFewCols * 4u;
     return (stages > meet ? stages : meet) + 16u;   // and two words for the block
 }
 
-template <int D, bool CAP, bool WIDE>
-__global__ __launch_bounds__(256, 2) void sdpa_paged_few_kernel(const SdpaPagedArgs a) {
+template <int D, bool CAP, bool WIDE, uint32_t SLOT_COLS>
+__device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedItem& it, uint32_t lane) {
     constexpr uint32_t ROW = D * 2u, P = D / 8u, KT = kFewStep * ROW, STAGE = 2u * KT, RPI = 1024u / ROW;   // pieces of a row; rows of a request
     constexpr int REQ = (int)(KT / 1024u), KS = D / 32, DT = D / 16, PARTS = WIDE ? 2 : 1;
     constexpr uint32_t QT = WIDE ? 16u : 8u;
@@ -491,9 +494,7 @@ __global__ __launch_bounds__(256, 2) void sdpa_paged_few_kernel(const SdpaPagedA
     extern __shared__ uint4 lds_raw[];
     unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_raw);
 
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
-    const PagedItem it = paged_item<kFewCols, kFewRound>(a, blockIdx.x, lane);
-    if (!it.any) return;
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
     const uint32_t G = a.group, columns = it.s.rows * G;
     auto limit_of = [&](uint32_t place) { return it.s.len + place + 1u > it.s.rows ? it.s.len + place + 1u - it.s.rows : 0u; };
     auto low_of = [&](uint32_t limit) { return a.window && limit > a.window ? limit - a.window : 0u; };
@@ -704,7 +705,7 @@ __global__ __launch_bounds__(256, 2) void sdpa_paged_few_kernel(const SdpaPagedA
     }
     __syncthreads();
     const bool whole = n_active == 1u;
-    constexpr uint32_t SLOT = kFewCols * (D + 2u) * 4u;
+    constexpr uint32_t SLOT = SLOT_COLS * (D + 2u) * 4u;
     const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials, 0, (int)(a.slots * SLOT), 0x27000);
     auto store = [&](uint32_t c, uint32_t d, const float4& o, float l) {
         const float f = l > 0.f || l != l ? 1.0f / l : 0.f;   // (a row that sees nothing: zeros)
@@ -782,6 +783,23 @@ __global__ __launch_bounds__(256, 2) void sdpa_paged_few_kernel(const SdpaPagedA
         if ((again & 1u) && c % 4u == wave) paged_row<D>(a, it.seq, it.s, c / G, it.kvh * G + c % G, lane);
 }
 
+// Chunks and single tokens together: each sequence by its kind, in one launch, so that what is bound by the matrix units runs beside what is bound by the
+// bytes.
+template <int D, bool CAP>
+__global__ __launch_bounds__(256, 2) void sdpa_paged_kernel(const SdpaPagedArgs a) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const PagedItem it = paged_item<false>(a, blockIdx.x, lane);
+    if (!it.any) return;
+    if (it.s.rows * a.group <= kFewCols) paged_few<D, CAP, true, kTileCols>(a, it, lane);
+    else paged_tile<D, CAP>(a, it, lane);
+}
+template <int D, bool CAP, bool WIDE>
+__global__ __launch_bounds__(256, 2) void sdpa_paged_few_kernel(const SdpaPagedArgs a) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const PagedItem it = paged_item<true>(a, blockIdx.x, lane);
+    if (it.any) paged_few<D, CAP, WIDE, kFewCols>(a, it, lane);
+}
+
 namespace {
 
 // How a launch is cut: fewer tiles than `target` are cut along their positions, into items of `min_steps` steps at least.
@@ -796,12 +814,14 @@ PagedPlan paged_plan(bool few, uint32_t n_heads, uint32_t n_kv, uint32_t head_di
     PagedPlan p;
     const uint32_t cols = few ? kFewCols : kTileCols;
     p.few = few;
-    p.target = few ? 1024 : 448;
+    p.target = few ? 1024 : 512;
     p.min_steps = few ? 2 : 4;
     p.tiles = few ? (uint64_t)n_seqs * n_kv : ((uint64_t)rows * (n_heads / n_kv) / cols + n_seqs) * n_kv;
     p.slot_bytes = (size_t)cols * (head_dim + 2) * 4;
     // (an item more for every tile: what is cut into items of equal work has one that is not full)
-    p.slots = p.tiles <= p.target ? (uint32_t)p.tiles + p.target : 0;
+    const uint32_t most = few ? 2048 : 896;   // slots: 64 MB at the most
+    p.slots = p.tiles <= most / 2 ? std::min((uint32_t)p.tiles + p.target, most) : 0;
+    p.target = p.slots ? p.slots - (uint32_t)p.tiles : p.target;
     p.bytes = kPagedCounterBytes + p.slots * p.slot_bytes;
     return p;
 }
@@ -847,8 +867,8 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     a.counters = static_cast<uint32_t*>(workspace);
     a.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kPagedCounterBytes);
     a.slots = p.slots; a.target = p.target; a.min_steps = p.min_steps;
-    const void* tile[2][2] = {{reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<64, false>), reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<64, true>)},
-                              {reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<128, false>), reinterpret_cast<const void*>(&sdpa_paged_tile_kernel<128, true>)}};
+    const void* tile[2][2] = {{reinterpret_cast<const void*>(&sdpa_paged_kernel<64, false>), reinterpret_cast<const void*>(&sdpa_paged_kernel<64, true>)},
+                              {reinterpret_cast<const void*>(&sdpa_paged_kernel<128, false>), reinterpret_cast<const void*>(&sdpa_paged_kernel<128, true>)}};
     const void* few[2][2][2] = {
         {{reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, false, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, false, true>)},
          {reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, true, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, true, true>)}},
