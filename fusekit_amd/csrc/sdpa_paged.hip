@@ -83,12 +83,13 @@ __device__ __forceinline__ void paged_row(const SdpaPagedArgs& a, uint32_t seq, 
 }
 
 // ---- which piece of the work a block does ----
-// The columns of a sequence and KV head are its new rows times the query heads of a group, place * group + head; 128 of them are a tile, and a
-// sequence of 16 or fewer goes by itself.  A tile walks its positions in steps of 64 (single tokens in rounds of 128); where all tiles of the
+// The columns of a sequence and KV head are its new rows times the query heads of a group, place * group + head; 128 of them are a tile, of a
+// sequence of up to kFewMost 16.  A tile walks its positions in steps of 64 (single tokens in rounds of 128); where all tiles of the
 // launch are fewer than `target` the steps are cut over several items.  Every wave finds its block's item by itself from the batch's arrays,
 // 64 sequences with one request: lengths stay on the device.
 constexpr uint32_t kTileCols = 128, kTileStep = 64;
-constexpr uint32_t kFewCols = 16, kFewStep = 32, kFewRound = 4 * kFewStep;
+constexpr uint32_t kFewCols = 16, kFewMost = 32, kFewStep = 32, kFewRound = 4 * kFewStep;
+constexpr uint32_t kMostSplits = 64;   // items of a tile
 struct PagedItem {
     uint32_t seq, kvh, tile, split, n_splits;
     PagedSeq s;
@@ -98,11 +99,14 @@ template <bool FEW>   // a launch of single tokens only
 __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t index, uint32_t lane) {
     constexpr uint32_t STEP = FEW ? kFewRound : kTileStep;
     const uint32_t n_kv = a.b.n_kv;
-    auto tiles_of = [&](const PagedSeq& s) { return FEW ? (s.rows ? 1u : 0u) : (uint32_t)(((uint64_t)s.rows * a.group + kTileCols - 1u) / kTileCols); };
+    auto tiles_of = [&](const PagedSeq& s) {   // (rows times heads of a group: below 2^31, the host has checked)
+        const uint32_t columns = s.rows * a.group, width = FEW || columns <= kFewMost ? kFewCols : kTileCols;
+        return (columns + width - 1u) / width;
+    };
     auto steps_of = [&](const PagedSeq& s) {   // of a tile of the sequence, at most
         uint32_t seen = s.len;
         if (a.window) {
-            const uint32_t span = FEW ? kFewCols : kTileCols / a.group + 1u;   // rows of a tile
+            const uint32_t span = (FEW ? kFewCols : kTileCols) / a.group + 2u;   // rows of a tile, at most
             const uint64_t w = (uint64_t)a.window + (s.rows < span ? s.rows : span) + STEP - 1u;
             seen = w < seen ? (uint32_t)w : seen;
         }
@@ -138,7 +142,7 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
         if (a.b.n_seqs > 64u) mine = read(at);
         const uint32_t tiles = tiles_of(mine);
         uint32_t splits = cut ? (steps_of(mine) + unit - 1u) / unit : 1u;
-        splits = splits < 1u ? 1u : splits;
+        splits = splits < 1u ? 1u : splits > kMostSplits ? kMostSplits : splits;
         const uint32_t items = tiles * splits * n_kv;
         uint32_t upto = items;   // with those of the lanes before
 #pragma unroll
@@ -396,8 +400,8 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
                 make_float4(oacc[i][4 * g + 0] * f, oacc[i][4 * g + 1] * f, oacc[i][4 * g + 2] * f, oacc[i][4 * g + 3] * f);
     wave_lds_order();
     // rows of this wave's columns whose sums are not finite, done again one by one (bit c: column e0 + c)
-    auto store_row = [&](uint32_t col, uint32_t pc, const float4& lo, const float4& hi) {
-        const uint32_t ec = e0 + col, pl = ec / G, hd = it.kvh * G + (ec - pl * G);
+    auto store_row = [&](uint32_t ec, uint32_t pc, const float4& lo, const float4& hi) {
+        const uint32_t pl = ec / G, hd = it.kvh * G + (ec - pl * G);
         *reinterpret_cast<uint4*>(a.out + (size_t)(it.s.row0 + pl) * a.out_stride + (size_t)hd * D + pc * 8u) =
             make_uint4(pack_bf16(lo.x, lo.y), pack_bf16(lo.z, lo.w), pack_bf16(hi.x, hi.y), pack_bf16(hi.z, hi.w));
     };
@@ -412,7 +416,7 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
             const bool in = col < live;
             const float4 lo = *reinterpret_cast<const float4*>(ob + (in ? col : 0u) * OS + pc * 8u);
             const float4 hi = *reinterpret_cast<const float4*>(ob + (in ? col : 0u) * OS + pc * 8u + 4u);
-            if (in) store_row(col, pc, lo, hi);
+            if (in) store_row(e0 + col, pc, lo, hi);
             unsigned long long odd = __builtin_amdgcn_ballot_w64(in && !(finite(lo) && finite(hi)));
             for (; odd; odd &= odd - 1u) again |= 1ull << ((base + (uint32_t)__builtin_ctzll(odd)) / (uint32_t)VP);
         }
@@ -439,34 +443,64 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
         if (!*last) return;
         if (tid == 0) __hip_atomic_store(&a.counters[base], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc(a.partials, 0, (int)(a.slots * (uint32_t)(kTileCols * (D + 2u) * 4u)), 0x27000);
-        constexpr uint32_t SLOT = kTileCols * (D + 2u) * 4u;
-        for (uint32_t b0 = 0; b0 < live * (uint32_t)VP; b0 += 64u) {
-            const uint32_t idx = b0 + lane, col = idx / (uint32_t)VP, pc = idx % (uint32_t)VP;
-            const bool in = col < live;
-            const uint32_t c = wave * 32u + (in ? col : 0u);
-            float M = -INFINITY, l = 0.f;
-            float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
-            for (uint32_t i = 0; i < n_active; ++i) {
-                const uint32_t at = (base + i * n_kv) * SLOT;
-                const pf_u32x2_t ml = __builtin_bit_cast(pf_u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(all, (int)(at + (kTileCols * D + c * 2u) * 4u), 0, kPastCaches));
-                const pf_u32x4_t u0 = __builtin_bit_cast(pf_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(all, (int)(at + (c * D + pc * 8u) * 4u), 0, kPastCaches));
-                const pf_u32x4_t u1 = __builtin_bit_cast(pf_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(all, (int)(at + (c * D + pc * 8u + 4u) * 4u), 0, kPastCaches));
-                const float mi = __uint_as_float(ml[0]), Mn = fmaxf(M, mi), ref = Mn == -INFINITY ? 0.f : Mn;
-                const float w0 = __builtin_amdgcn_exp2f(M - ref), w1 = __builtin_amdgcn_exp2f(mi - ref);
-                M = Mn;
-                l = l * w0 + __uint_as_float(ml[1]) * w1;
-                lo = make_float4(fmaf(__uint_as_float(u0[0]), w1, lo.x * w0), fmaf(__uint_as_float(u0[1]), w1, lo.y * w0),
-                                 fmaf(__uint_as_float(u0[2]), w1, lo.z * w0), fmaf(__uint_as_float(u0[3]), w1, lo.w * w0));
-                hi = make_float4(fmaf(__uint_as_float(u1[0]), w1, hi.x * w0), fmaf(__uint_as_float(u1[1]), w1, hi.y * w0),
-                                 fmaf(__uint_as_float(u1[2]), w1, hi.z * w0), fmaf(__uint_as_float(u1[3]), w1, hi.w * w0));
+        constexpr uint32_t SLOT = kTileCols * (D + 2u) * 4u, PAIR = 2, AHEAD = 4;   // pieces of a thread at once, partials requested together
+        const uint32_t pieces = (e_last - e_tile + 1u) * (uint32_t)VP;              // of the tile, over all threads
+        volatile uint32_t* const odd = reinterpret_cast<volatile uint32_t*>(lds);   // a bit for a column: its sums are not finite
+        if (tid < 4u) odd[tid] = 0;
+        __syncthreads();
+#pragma unroll 1
+        for (uint32_t b0 = 0; b0 < pieces; b0 += 256u * PAIR) {
+            uint32_t col[PAIR], pc[PAIR];
+            float M[PAIR], l[PAIR];
+            float o[PAIR][8];
+#pragma unroll
+            for (uint32_t p = 0; p < PAIR; ++p) {
+                const uint32_t idx = b0 + p * 256u + tid;
+                col[p] = (idx < pieces ? idx : 0u) / (uint32_t)VP;
+                pc[p] = idx % (uint32_t)VP;
+                M[p] = -INFINITY;
+                l[p] = 0.f;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) o[p][r] = 0.f;
             }
-            const float r = l > 0.f || l != l ? 1.0f / l : 0.f;
-            lo = make_float4(lo.x * r, lo.y * r, lo.z * r, lo.w * r);
-            hi = make_float4(hi.x * r, hi.y * r, hi.z * r, hi.w * r);
-            if (in) store_row(col, pc, lo, hi);
-            unsigned long long odd = __builtin_amdgcn_ballot_w64(in && !(finite(lo) && finite(hi)));
-            for (; odd; odd &= odd - 1u) again |= 1ull << ((b0 + (uint32_t)__builtin_ctzll(odd)) / (uint32_t)VP);
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < n_active; i0 += AHEAD) {
+                pf_u32x2_t ml[AHEAD][PAIR];
+                pf_u32x4_t u[AHEAD][PAIR][2];
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i)
+#pragma unroll
+                    for (uint32_t p = 0; p < PAIR; ++p) {
+                        const uint32_t at = (base + (i0 + i < n_active ? i0 + i : i0) * n_kv) * SLOT;
+                        ml[i][p] = __builtin_bit_cast(pf_u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(all, (int)(at + (kTileCols * D + col[p] * 2u) * 4u), 0, kPastCaches));
+                        u[i][p][0] = __builtin_bit_cast(pf_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(all, (int)(at + (col[p] * D + pc[p] * 8u) * 4u), 0, kPastCaches));
+                        u[i][p][1] = __builtin_bit_cast(pf_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(all, (int)(at + (col[p] * D + pc[p] * 8u + 4u) * 4u), 0, kPastCaches));
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i)
+#pragma unroll
+                    for (uint32_t p = 0; p < PAIR; ++p) {
+                        const float mi = i0 + i < n_active ? __uint_as_float(ml[i][p][0]) : -INFINITY, li = i0 + i < n_active ? __uint_as_float(ml[i][p][1]) : 0.f;
+                        const float Mn = fmaxf(M[p], mi), ref = Mn == -INFINITY ? 0.f : Mn;
+                        const float w0 = __builtin_amdgcn_exp2f(M[p] - ref), w1 = __builtin_amdgcn_exp2f(mi - ref);
+                        M[p] = Mn;
+                        l[p] = l[p] * w0 + li * w1;
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) o[p][r] = fmaf(__uint_as_float(u[i][p][r / 4][r % 4]), i0 + i < n_active ? w1 : 0.f, o[p][r] * w0);
+                    }
+            }
+#pragma unroll
+            for (uint32_t p = 0; p < PAIR; ++p) {
+                if (b0 + p * 256u + tid >= pieces) continue;
+                const float r = l[p] > 0.f || l[p] != l[p] ? 1.0f / l[p] : 0.f;
+                const float4 lo = make_float4(o[p][0] * r, o[p][1] * r, o[p][2] * r, o[p][3] * r), hi = make_float4(o[p][4] * r, o[p][5] * r, o[p][6] * r, o[p][7] * r);
+                store_row(e_tile + col[p], pc[p], lo, hi);
+                if (!(finite(lo) && finite(hi))) atomicOr(const_cast<uint32_t*>(&odd[col[p] >> 5]), 1u << (col[p] & 31u));
+            }
         }
+        __syncthreads();
+        again = odd[wave];
     }
     for (; again; again &= again - 1u) {
         const uint32_t ec = e0 + (uint32_t)__builtin_ctzll(again), pl = ec / G;
@@ -495,10 +529,10 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
     unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_raw);
 
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
-    const uint32_t G = a.group, columns = it.s.rows * G;
+    const uint32_t G = a.group, e0 = it.tile * kFewCols, left_cols = it.s.rows * G - e0, columns = left_cols < kFewCols ? left_cols : kFewCols;   // of this tile
     auto limit_of = [&](uint32_t place) { return it.s.len + place + 1u > it.s.rows ? it.s.len + place + 1u - it.s.rows : 0u; };
     auto low_of = [&](uint32_t limit) { return a.window && limit > a.window ? limit - a.window : 0u; };
-    const uint32_t kv_end = __builtin_amdgcn_readfirstlane(limit_of(it.s.rows - 1u)), lim_lo = __builtin_amdgcn_readfirstlane(limit_of(0));
+    const uint32_t kv_end = __builtin_amdgcn_readfirstlane(limit_of((e0 + columns - 1u) / G)), lim_lo = __builtin_amdgcn_readfirstlane(limit_of(e0 / G));
     const uint32_t low_lo = __builtin_amdgcn_readfirstlane(low_of(lim_lo)), low_hi = __builtin_amdgcn_readfirstlane(low_of(kv_end));
     const uint32_t round0 = low_lo / kFewRound, rounds = (kv_end + kFewRound - 1u) / kFewRound - (kv_end ? round0 : 0u);
     const uint32_t per = (rounds + it.n_splits - 1u) / it.n_splits;
@@ -510,10 +544,10 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
     const uint32_t n_steps = __builtin_amdgcn_readfirstlane(end > first ? (end - first + kFewRound - 1u) / kFewRound : 0u);
 
     const uint32_t mine = n % QT < columns ? n % QT : columns - 1u;   // (columns past the last repeat it and store nothing)
-    const uint32_t place = mine / G, q_limit = limit_of(place), q_low = low_of(q_limit);
+    const uint32_t place = (e0 + mine) / G, q_limit = limit_of(place), q_low = low_of(q_limit);
     pf_bf16x8_t qf[KS];
     {
-        const uint16_t* qr = a.q + (size_t)(it.s.row0 + place) * a.q_stride + (size_t)(it.kvh * G + (mine - place * G)) * D + g * 8u;
+        const uint16_t* qr = a.q + (size_t)(it.s.row0 + place) * a.q_stride + (size_t)(it.kvh * G + (e0 + mine - place * G)) * D + g * 8u;
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const pf_bf16x8_t*>(qr + s * 32);
     }
@@ -710,8 +744,8 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
     auto store = [&](uint32_t c, uint32_t d, const float4& o, float l) {
         const float f = l > 0.f || l != l ? 1.0f / l : 0.f;   // (a row that sees nothing: zeros)
         const float t = (__builtin_fabsf(o.x) + __builtin_fabsf(o.y)) + (__builtin_fabsf(o.z) + __builtin_fabsf(o.w));
-        const uint32_t pl = c / G;
-        *reinterpret_cast<uint2*>(a.out + (size_t)(it.s.row0 + pl) * a.out_stride + (size_t)(it.kvh * G + (c - pl * G)) * D + d) =
+        const uint32_t pl = (e0 + c) / G;
+        *reinterpret_cast<uint2*>(a.out + (size_t)(it.s.row0 + pl) * a.out_stride + (size_t)(it.kvh * G + (e0 + c - pl * G)) * D + d) =
             make_uint2(pack_bf16(o.x * f, o.y * f), pack_bf16(o.z * f, o.w * f));
         if (!(t * f < INFINITY)) atomicOr(const_cast<uint32_t*>(&word[1]), 1u << c);
     };
@@ -743,44 +777,58 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
         }
     }
     if (!whole) {   // the item that arrives last merges the sequence's, in their order
-        const uint32_t n_kv = a.b.n_kv, base = blockIdx.x - it.split * n_kv;
+        const uint32_t stride = a.b.n_kv, base = blockIdx.x - it.split * stride;   // the slot of the tile's first item
         wait_memory_ops_done();
         __syncthreads();
         if (tid == 0) word[0] = atomicAdd(&a.counters[base], 1u) == n_active - 1u ? 1u : 0u;
         __syncthreads();
         if (!word[0]) return;
         if (tid == 0) __hip_atomic_store(&a.counters[base], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        for (uint32_t i = tid; i < columns * (D / 4u); i += 256u) {
-            const uint32_t c = i / (D / 4u), d = (i % (D / 4u)) * 4u;
-            float M = -INFINITY, l = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            constexpr uint32_t AHEAD = 8;   // partials requested together
-            for (uint32_t b0 = 0; b0 < n_active; b0 += AHEAD) {
-                pf_u32x2_t ml[AHEAD];
-                pf_u32x4_t u[AHEAD];
+        // a wave a column: every partial of it is requested before the first is looked at
+        constexpr uint32_t LP = D / 4u, SPR = 64u / LP;   // lanes of a partial, partials of a request
+        for (uint32_t c = wave; c < columns; c += 4u) {
+            const pf_u32x2_t ml = __builtin_bit_cast(pf_u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(
+                mem, (int)((base + (lane < n_active ? lane : 0u) * stride) * SLOT + (kFewCols * D + c * 2u) * 4u), 0, kPastCaches));
+            auto merge = [&](auto count) __attribute__((always_inline)) {
+                constexpr uint32_t N = decltype(count)::value / SPR;
+                pf_u32x4_t u[N];
 #pragma unroll
-                for (uint32_t k = 0; k < AHEAD; ++k) {
-                    const uint32_t at = (base + (b0 + k < n_active ? b0 + k : n_active - 1u) * n_kv) * SLOT;
-                    ml[k] = __builtin_bit_cast(pf_u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(mem, (int)(at + (kFewCols * D + c * 2u) * 4u), 0, kPastCaches));
-                    u[k] = __builtin_bit_cast(pf_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(mem, (int)(at + (c * D + d) * 4u), 0, kPastCaches));
+                for (uint32_t i = 0; i < N; ++i) {
+                    const uint32_t k = i * SPR + lane / LP;
+                    u[i] = __builtin_bit_cast(pf_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                        mem, (int)((base + (k < n_active ? k : 0u) * stride) * SLOT + (c * D + (lane % LP) * 4u) * 4u), 0, kPastCaches));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                const float m = lane < n_active ? __uint_as_float(ml[0]) : -INFINITY, M = wave_max(m);
+                const float w_mine = __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.f : M));
+                const float l = wave_sum(lane < n_active ? __uint_as_float(ml[1]) * w_mine : 0.f);
+                float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (uint32_t i = 0; i < N; ++i) {
+                    const uint32_t k = i * SPR + lane / LP;
+                    const float w = __int_as_float(__builtin_amdgcn_ds_bpermute((int)(k * 4u), __float_as_int(w_mine)));
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[r] = k < n_active ? fmaf(__uint_as_float(u[i][r]), w, o[r]) : o[r];
                 }
 #pragma unroll
-                for (uint32_t k = 0; k < AHEAD; ++k) {
-                    if (b0 + k >= n_active) break;
-                    const float mk = __uint_as_float(ml[k][0]), Mn = fmaxf(M, mk), ref = Mn == -INFINITY ? 0.f : Mn;
-                    const float w0 = __builtin_amdgcn_exp2f(M - ref), w1 = __builtin_amdgcn_exp2f(mk - ref);
-                    M = Mn;
-                    l = l * w0 + __uint_as_float(ml[k][1]) * w1;
-                    o = make_float4(fmaf(__uint_as_float(u[k][0]), w1, o.x * w0), fmaf(__uint_as_float(u[k][1]), w1, o.y * w0),
-                                    fmaf(__uint_as_float(u[k][2]), w1, o.z * w0), fmaf(__uint_as_float(u[k][3]), w1, o.w * w0));
+                for (int r = 0; r < 4; ++r) {   // the partials that a request brought side by side
+                    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[r]), __float_as_uint(o[r]), false, false);
+                    o[r] = __uint_as_float(h[0]) + __uint_as_float(h[1]);
+                    if constexpr (SPR == 4) {
+                        const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(o[r]), __float_as_uint(o[r]), false, false);
+                        o[r] = __uint_as_float(q[0]) + __uint_as_float(q[1]);
+                    }
                 }
-            }
-            store(c, d, o, l);
+                if (lane < LP) store(c, lane * 4u, make_float4(o[0], o[1], o[2], o[3]), l);
+            };
+            if (n_active <= 8u) merge(std::integral_constant<uint32_t, 8>{});
+            else if (n_active <= 24u) merge(std::integral_constant<uint32_t, 24>{});
+            else merge(std::integral_constant<uint32_t, kMostSplits>{});
         }
     }
     __syncthreads();
     for (uint32_t again = word[1], c = 0; again; again >>= 1, ++c)
-        if ((again & 1u) && c % 4u == wave) paged_row<D>(a, it.seq, it.s, c / G, it.kvh * G + c % G, lane);
+        if ((again & 1u) && c % 4u == wave) paged_row<D>(a, it.seq, it.s, (e0 + c) / G, it.kvh * G + (e0 + c) % G, lane);
 }
 
 // Chunks and single tokens together: each sequence by its kind, in one launch, so that what is bound by the matrix units runs beside what is bound by the
@@ -790,7 +838,7 @@ __global__ __launch_bounds__(256, 2) void sdpa_paged_kernel(const SdpaPagedArgs 
     const uint32_t lane = threadIdx.x & 63u;
     const PagedItem it = paged_item<false>(a, blockIdx.x, lane);
     if (!it.any) return;
-    if (it.s.rows * a.group <= kFewCols) paged_few<D, CAP, true, kTileCols>(a, it, lane);
+    if (it.s.rows * a.group <= kFewMost) paged_few<D, CAP, true, kTileCols>(a, it, lane);
     else paged_tile<D, CAP>(a, it, lane);
 }
 template <int D, bool CAP, bool WIDE>
@@ -814,9 +862,11 @@ PagedPlan paged_plan(bool few, uint32_t n_heads, uint32_t n_kv, uint32_t head_di
     PagedPlan p;
     const uint32_t cols = few ? kFewCols : kTileCols;
     p.few = few;
-    p.target = few ? 1024 : 512;
-    p.min_steps = few ? 2 : 4;
-    p.tiles = few ? (uint64_t)n_seqs * n_kv : ((uint64_t)rows * (n_heads / n_kv) / cols + n_seqs) * n_kv;
+    p.target = few ? 768 : 640;
+    p.min_steps = few ? 1 : 8;
+    // (a sequence of up to kFewMost columns has tiles of 16 also among chunks)
+    const uint64_t columns = (uint64_t)rows * (n_heads / n_kv);
+    p.tiles = few ? (columns / kFewCols + n_seqs) * n_kv : (columns / kTileCols + (uint64_t)n_seqs * (kFewMost / kFewCols)) * n_kv;
     p.slot_bytes = (size_t)cols * (head_dim + 2) * 4;
     // (an item more for every tile: what is cut into items of equal work has one that is not full)
     const uint32_t most = few ? 2048 : 896;   // slots: 64 MB at the most
@@ -857,7 +907,7 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     size_t need = 0;
     FK_TRY(sdpa_paged_workspace_bytes(n_heads, n_kv, D, batch->n_seqs, batch->rows, batch->max_len, &need));
     if (workspace_bytes < need) return set_error(FK_ERR_INVALID, "sdpa_paged: workspace too small");
-    const PagedPlan p = paged_plan(batch->max_rows * (n_heads / n_kv) <= kFewCols, n_heads, n_kv, D, batch->n_seqs, batch->rows);
+    const PagedPlan p = paged_plan(batch->max_rows * (n_heads / n_kv) <= kFewMost, n_heads, n_kv, D, batch->n_seqs, batch->rows);
     if (p.tiles + p.target > 0x7fffffffull) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: too many rows");
     const DeviceFacts* dev;
     FK_TRY(device_facts(&dev));
