@@ -92,10 +92,12 @@ constexpr uint32_t kFewCols = 16, kFewMost = 32, kFewStep = 32, kFewRound = 4 * 
 constexpr uint32_t kMostSplits = 64;   // items of a tile
 struct PagedItem {
     uint32_t seq, kvh, tile, split, n_splits;
+    uint32_t base;   // the index of the tile's first item; its others follow n_kv apart
     PagedSeq s;
     bool any;
 };
-template <bool FEW>   // a launch of single tokens only
+// FEW: a launch of single tokens only.  TILES: `index` counts tiles, not items.
+template <bool FEW, bool TILES = false>
 __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t index, uint32_t lane) {
     constexpr uint32_t STEP = FEW ? kFewRound : kTileStep;
     const uint32_t n_kv = a.b.n_kv;
@@ -137,40 +139,64 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
     unit = unit < a.min_steps ? a.min_steps : unit;
     PagedItem it;
     it.any = false;
-    uint32_t left = index;
+    uint32_t left = index, before = 0;   // items of the sequences before
     for (uint32_t at = 0; at < a.b.n_seqs; at += 64u) {
         if (a.b.n_seqs > 64u) mine = read(at);
         const uint32_t tiles = tiles_of(mine);
-        uint32_t splits = cut ? (steps_of(mine) + unit - 1u) / unit : 1u;
+        uint32_t splits = cut ? (steps_of(mine) + (FEW ? unit - 1u : 0u)) / unit : 1u;
         splits = splits < 1u ? 1u : splits > kMostSplits ? kMostSplits : splits;
         const uint32_t items = tiles * splits * n_kv;
-        uint32_t upto = items;   // with those of the lanes before
+        auto with_those_before = [&](uint32_t upto) {
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t v = __shfl_up(upto, o, 64);
-            upto += lane >= (uint32_t)o ? v : 0u;
-        }
-        const unsigned long long past = __builtin_amdgcn_ballot_w64(upto > left);
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t v = __shfl_up(upto, o, 64);
+                upto += lane >= (uint32_t)o ? v : 0u;
+            }
+            return upto;
+        };
+        const uint32_t upto = with_those_before(items), count = TILES ? tiles * n_kv : items, counted = TILES ? with_those_before(count) : upto;
+        const unsigned long long past = __builtin_amdgcn_ballot_w64(counted > left);
         if (!past) {
-            left -= (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+            left -= (uint32_t)__builtin_amdgcn_readlane((int)counted, 63);
+            before += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
             continue;
         }
         const int who = (int)__builtin_ctzll(past);
         auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, who); };
-        left -= of(upto) - of(items);
+        left -= of(counted) - of(count);
+        before += of(upto) - of(items);
         it.seq = at + (uint32_t)who;
         it.s = PagedSeq{of(mine.row0), of(mine.rows), of(mine.len), of(mine.bad)};
         it.n_splits = of(splits);
         it.kvh = left % n_kv;
         left /= n_kv;
-        it.split = left % it.n_splits;
-        it.tile = of(tiles) - 1u - left / it.n_splits;   // the longest first
+        it.split = TILES ? 0u : left % it.n_splits;
+        left = TILES ? left : left / it.n_splits;
+        it.tile = of(tiles) - 1u - left;   // the longest first
+        it.base = before + left * it.n_splits * n_kv + it.kvh;
         it.any = true;
         break;
     }
     return it;
 }
 constexpr int kPastCaches = 16;   // (sc1: what another block wrote, or is to read)
+
+// What a tile's columns e_tile .. e_last see, in steps of STEP positions, and how its items share them: item i takes `per` steps from step0 + i * per.
+struct PagedRange {
+    uint32_t kv_end, step0, steps, per, n_active;   // n_active: items that have steps, one at least
+};
+template <uint32_t STEP>
+__device__ __forceinline__ PagedRange paged_range(const SdpaPagedArgs& a, const PagedItem& it, uint32_t e_tile, uint32_t e_last) {
+    auto limit_of = [&](uint32_t place) { return it.s.len + place + 1u > it.s.rows ? it.s.len + place + 1u - it.s.rows : 0u; };
+    PagedRange r;
+    r.kv_end = __builtin_amdgcn_readfirstlane(limit_of(e_last / a.group));
+    const uint32_t first = limit_of(e_tile / a.group);
+    r.step0 = __builtin_amdgcn_readfirstlane((a.window && first > a.window ? first - a.window : 0u) / STEP);
+    r.steps = (r.kv_end + STEP - 1u) / STEP - (r.kv_end ? r.step0 : 0u);
+    r.per = (r.steps + it.n_splits - 1u) / it.n_splits;
+    r.n_active = r.per ? (r.steps + r.per - 1u) / r.per : 1u;
+    return r;
+}
 
 // ---- tiles of 128 columns ----
 // A block is four waves of 32 columns on the same 64 positions a step.  The products and the softmax are those of the causal attention of one
@@ -179,7 +205,7 @@ constexpr int kPastCaches = 16;   // (sc1: what another block wrote, or is to re
 // in one page: one page id, loaded two steps ahead into a scalar register.
 constexpr uint32_t tile_lds_bytes(uint32_t d) {
     const uint32_t stage = 2u * 2u * kTileStep * d * 2u, outb = kTileCols * (d + 4u) * 4u;
-    return (stage > outb ? stage : outb) + 16u;   // and a word for the block
+    return stage > outb ? stage : outb;
 }
 
 template <int D, bool CAP>
@@ -196,14 +222,11 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
     auto limit_of = [&](uint32_t place) { return it.s.len + place + 1u > it.s.rows ? it.s.len + place + 1u - it.s.rows : 0u; };   // positions a row may see end here
     auto low_of = [&](uint32_t limit) { return a.window && limit > a.window ? limit - a.window : 0u; };                           // and begin here
     const uint32_t e_tile = it.tile * kTileCols, e_last = columns - e_tile < kTileCols ? columns - 1u : e_tile + kTileCols - 1u;
-    const uint32_t kv_end = __builtin_amdgcn_readfirstlane(limit_of(e_last / G));
-    const uint32_t step0 = __builtin_amdgcn_readfirstlane(low_of(limit_of(e_tile / G)) / kTileStep);
-    const uint32_t all_steps = (kv_end + kTileStep - 1u) / kTileStep - (kv_end ? step0 : 0u);
-    const uint32_t per = (all_steps + it.n_splits - 1u) / it.n_splits;
-    const uint32_t n_active = per ? (all_steps + per - 1u) / per : 1u;   // items of this tile that have steps (one at least)
+    const PagedRange range = paged_range<kTileStep>(a, it, e_tile, e_last);
+    const uint32_t kv_end = range.kv_end, n_active = range.n_active;
     if (it.split >= n_active) return;
-    const uint32_t begin = __builtin_amdgcn_readfirstlane(step0 + it.split * per);
-    const uint32_t stop = __builtin_amdgcn_readfirstlane(it.split + 1u == n_active ? step0 + all_steps : begin + per);
+    const uint32_t begin = __builtin_amdgcn_readfirstlane(range.step0 + it.split * range.per);
+    const uint32_t stop = __builtin_amdgcn_readfirstlane(it.split + 1u == n_active ? range.step0 + range.steps : begin + range.per);
 
     // this lane's column; a wave's columns past the last repeat it, and a wave without columns does the last one's loads and nothing else
     const uint32_t e0 = e_tile + wave * 32u;
@@ -399,113 +422,140 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
             *reinterpret_cast<float4*>(ob + nl * OS + (uint32_t)(i * 32 + 8 * g) + 4u * kb) =
                 make_float4(oacc[i][4 * g + 0] * f, oacc[i][4 * g + 1] * f, oacc[i][4 * g + 2] * f, oacc[i][4 * g + 3] * f);
     wave_lds_order();
-    // rows of this wave's columns whose sums are not finite, done again one by one (bit c: column e0 + c)
-    auto store_row = [&](uint32_t ec, uint32_t pc, const float4& lo, const float4& hi) {
-        const uint32_t pl = ec / G, hd = it.kvh * G + (ec - pl * G);
-        *reinterpret_cast<uint4*>(a.out + (size_t)(it.s.row0 + pl) * a.out_stride + (size_t)hd * D + pc * 8u) =
-            make_uint4(pack_bf16(lo.x, lo.y), pack_bf16(lo.z, lo.w), pack_bf16(hi.x, hi.y), pack_bf16(hi.z, hi.w));
-    };
-    auto finite = [](const float4& v) {
-        const float t = __builtin_fabsf(v.x) + __builtin_fabsf(v.y) + __builtin_fabsf(v.z) + __builtin_fabsf(v.w);
-        return t < INFINITY;
-    };
-    unsigned long long again = 0;
-    if (whole) {
-        for (uint32_t base = 0; base < live * (uint32_t)VP; base += 64u) {
-            const uint32_t idx = base + lane, col = idx / (uint32_t)VP, pc = idx % (uint32_t)VP;
-            const bool in = col < live;
-            const float4 lo = *reinterpret_cast<const float4*>(ob + (in ? col : 0u) * OS + pc * 8u);
-            const float4 hi = *reinterpret_cast<const float4*>(ob + (in ? col : 0u) * OS + pc * 8u + 4u);
-            if (in) store_row(e0 + col, pc, lo, hi);
-            unsigned long long odd = __builtin_amdgcn_ballot_w64(in && !(finite(lo) && finite(hi)));
-            for (; odd; odd &= odd - 1u) again |= 1ull << ((base + (uint32_t)__builtin_ctzll(odd)) / (uint32_t)VP);
-        }
-    } else {
-        const uint32_t slot = blockIdx.x;
-        float* const part = a.partials + (size_t)slot * (kTileCols * (D + 2u));
-        const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(part, 0, (int)(kTileCols * (D + 2u) * 4u), 0x27000);
+    if (!whole) {   // the item's part, for paged_merge
+        const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials + (size_t)blockIdx.x * (kTileCols * (D + 2u)), 0, (int)(kTileCols * (D + 2u) * 4u), 0x27000);
         for (uint32_t idx = lane; idx < live * (uint32_t)(D / 4); idx += 64u) {
             const uint32_t col = idx / (uint32_t)(D / 4), pc = idx % (uint32_t)(D / 4);
             const pf_u32x4_t v = *reinterpret_cast<const pf_u32x4_t*>(ob + col * OS + pc * 4u);
-            __builtin_amdgcn_raw_buffer_store_b128(v, mem, (int)(((wave * 32u + col) * D + pc * 4u) * 4u), 0, kPastCaches);
+            __builtin_amdgcn_raw_buffer_store_b128(v, mem, (int)(((wave * 32u + col) * D + pc * 4u) * 4u), 0, 0);
         }
         if (kb == 0 && nl < live) {
             const pf_u32x2_t ml = {__float_as_uint(m_run), __float_as_uint(l_run)};
-            __builtin_amdgcn_raw_buffer_store_b64(ml, mem, (int)((kTileCols * D + (wave * 32u + nl) * 2u) * 4u), 0, kPastCaches);
+            __builtin_amdgcn_raw_buffer_store_b64(ml, mem, (int)((kTileCols * D + (wave * 32u + nl) * 2u) * 4u), 0, 0);
         }
-        // the item that arrives last merges the tile's, in their order
-        volatile uint32_t* const last = reinterpret_cast<volatile uint32_t*>(lds + tile_lds_bytes(D) - 16u);   // (LDS starts with the stages: their addresses are absolute)
-        const uint32_t n_kv = a.b.n_kv, base = slot - it.split * n_kv;   // the slot of the tile's first item
-        wait_memory_ops_done();
-        __syncthreads();
-        if (tid == 0) *last = atomicAdd(&a.counters[base], 1u) == n_active - 1u ? 1u : 0u;
-        __syncthreads();
-        if (!*last) return;
-        if (tid == 0) __hip_atomic_store(&a.counters[base], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc(a.partials, 0, (int)(a.slots * (uint32_t)(kTileCols * (D + 2u) * 4u)), 0x27000);
-        constexpr uint32_t SLOT = kTileCols * (D + 2u) * 4u, PAIR = 2, AHEAD = 4;   // pieces of a thread at once, partials requested together
-        const uint32_t pieces = (e_last - e_tile + 1u) * (uint32_t)VP;              // of the tile, over all threads
-        volatile uint32_t* const odd = reinterpret_cast<volatile uint32_t*>(lds);   // a bit for a column: its sums are not finite
-        if (tid < 4u) odd[tid] = 0;
-        __syncthreads();
-#pragma unroll 1
-        for (uint32_t b0 = 0; b0 < pieces; b0 += 256u * PAIR) {
-            uint32_t col[PAIR], pc[PAIR];
-            float M[PAIR], l[PAIR];
-            float o[PAIR][8];
-#pragma unroll
-            for (uint32_t p = 0; p < PAIR; ++p) {
-                const uint32_t idx = b0 + p * 256u + tid;
-                col[p] = (idx < pieces ? idx : 0u) / (uint32_t)VP;
-                pc[p] = idx % (uint32_t)VP;
-                M[p] = -INFINITY;
-                l[p] = 0.f;
-#pragma unroll
-                for (int r = 0; r < 8; ++r) o[p][r] = 0.f;
-            }
-#pragma unroll 1
-            for (uint32_t i0 = 0; i0 < n_active; i0 += AHEAD) {
-                pf_u32x2_t ml[AHEAD][PAIR];
-                pf_u32x4_t u[AHEAD][PAIR][2];
-#pragma unroll
-                for (uint32_t i = 0; i < AHEAD; ++i)
-#pragma unroll
-                    for (uint32_t p = 0; p < PAIR; ++p) {
-                        const uint32_t at = (base + (i0 + i < n_active ? i0 + i : i0) * n_kv) * SLOT;
-                        ml[i][p] = __builtin_bit_cast(pf_u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(all, (int)(at + (kTileCols * D + col[p] * 2u) * 4u), 0, kPastCaches));
-                        u[i][p][0] = __builtin_bit_cast(pf_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(all, (int)(at + (col[p] * D + pc[p] * 8u) * 4u), 0, kPastCaches));
-                        u[i][p][1] = __builtin_bit_cast(pf_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(all, (int)(at + (col[p] * D + pc[p] * 8u + 4u) * 4u), 0, kPastCaches));
-                    }
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (uint32_t i = 0; i < AHEAD; ++i)
-#pragma unroll
-                    for (uint32_t p = 0; p < PAIR; ++p) {
-                        const float mi = i0 + i < n_active ? __uint_as_float(ml[i][p][0]) : -INFINITY, li = i0 + i < n_active ? __uint_as_float(ml[i][p][1]) : 0.f;
-                        const float Mn = fmaxf(M[p], mi), ref = Mn == -INFINITY ? 0.f : Mn;
-                        const float w0 = __builtin_amdgcn_exp2f(M[p] - ref), w1 = __builtin_amdgcn_exp2f(mi - ref);
-                        M[p] = Mn;
-                        l[p] = l[p] * w0 + li * w1;
-#pragma unroll
-                        for (int r = 0; r < 8; ++r) o[p][r] = fmaf(__uint_as_float(u[i][p][r / 4][r % 4]), i0 + i < n_active ? w1 : 0.f, o[p][r] * w0);
-                    }
-            }
-#pragma unroll
-            for (uint32_t p = 0; p < PAIR; ++p) {
-                if (b0 + p * 256u + tid >= pieces) continue;
-                const float r = l[p] > 0.f || l[p] != l[p] ? 1.0f / l[p] : 0.f;
-                const float4 lo = make_float4(o[p][0] * r, o[p][1] * r, o[p][2] * r, o[p][3] * r), hi = make_float4(o[p][4] * r, o[p][5] * r, o[p][6] * r, o[p][7] * r);
-                store_row(e_tile + col[p], pc[p], lo, hi);
-                if (!(finite(lo) && finite(hi))) atomicOr(const_cast<uint32_t*>(&odd[col[p] >> 5]), 1u << (col[p] & 31u));
-            }
-        }
-        __syncthreads();
-        again = odd[wave];
+        return;
+    }
+    unsigned long long again = 0;   // columns of this wave whose sums are not finite, done again one by one
+    for (uint32_t base = 0; base < live * (uint32_t)VP; base += 64u) {
+        const uint32_t idx = base + lane, col = idx / (uint32_t)VP, pc = idx % (uint32_t)VP;
+        const bool in = col < live;
+        const float4 lo = *reinterpret_cast<const float4*>(ob + (in ? col : 0u) * OS + pc * 8u);
+        const float4 hi = *reinterpret_cast<const float4*>(ob + (in ? col : 0u) * OS + pc * 8u + 4u);
+        const uint32_t ec = e0 + col, pl = ec / G;
+        if (in)
+            *reinterpret_cast<uint4*>(a.out + (size_t)(it.s.row0 + pl) * a.out_stride + (size_t)(it.kvh * G + (ec - pl * G)) * D + pc * 8u) =
+                make_uint4(pack_bf16(lo.x, lo.y), pack_bf16(lo.z, lo.w), pack_bf16(hi.x, hi.y), pack_bf16(hi.z, hi.w));
+        const float t = (__builtin_fabsf(lo.x) + __builtin_fabsf(lo.y)) + (__builtin_fabsf(lo.z) + __builtin_fabsf(lo.w)) +
+                        (__builtin_fabsf(hi.x) + __builtin_fabsf(hi.y)) + (__builtin_fabsf(hi.z) + __builtin_fabsf(hi.w));
+        unsigned long long odd = __builtin_amdgcn_ballot_w64(in && !(t < INFINITY));
+        for (; odd; odd &= odd - 1u) again |= 1ull << ((base + (uint32_t)__builtin_ctzll(odd)) / (uint32_t)VP);
     }
     for (; again; again &= again - 1u) {
         const uint32_t ec = e0 + (uint32_t)__builtin_ctzll(again), pl = ec / G;
         paged_row<D>(a, it.seq, it.s, pl, it.kvh * G + (ec - pl * G), lane);
     }
+}
+
+// A wave's merge of the columns c0, c0 + step, ... below `end` from the parts of n items (64 at most) that lie `stride` slots apart: GROUP parts of each of
+// T columns are requested together.  put(c, d, four sums, the sum of the probabilities) by the lanes that hold them; done(c) by all lanes.
+template <int D, int CACHE, uint32_t GROUP, uint32_t T, typename Put, typename Done>
+__device__ __forceinline__ void paged_merge_columns(const __amdgpu_buffer_rsrc_t& mem, uint32_t base, uint32_t stride, uint32_t slot_bytes, uint32_t ml_at, uint32_t c0,
+                                                    uint32_t end, uint32_t step, uint32_t n, uint32_t lane, Put&& put, Done&& done) {
+    constexpr uint32_t LP = D / 4u, SPR = 64u / LP, N = GROUP / SPR;   // lanes of a part, parts of a request, requests of a column
+    for (uint32_t c = c0; c < end; c += T * step) {
+        pf_u32x2_t ml[T];
+        pf_u32x4_t u[T][N];
+        auto request = [&](uint32_t from) __attribute__((always_inline)) {
+#pragma unroll
+            for (uint32_t t = 0; t < T; ++t) {
+                const uint32_t ct = c + t * step < end ? c + t * step : c;
+#pragma unroll
+                for (uint32_t i = 0; i < N; ++i) {
+                    const uint32_t k = from + i * SPR + lane / LP;
+                    u[t][i] = __builtin_bit_cast(pf_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(mem, (int)((base + (k < n ? k : 0u) * stride) * slot_bytes + (ct * D + (lane % LP) * 4u) * 4u), 0, CACHE));
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (uint32_t t = 0; t < T; ++t) {
+            const uint32_t ct = c + t * step < end ? c + t * step : c;
+            ml[t] = __builtin_bit_cast(pf_u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(mem, (int)((base + (lane < n ? lane : 0u) * stride) * slot_bytes + ml_at + ct * 8u), 0, CACHE));
+        }
+        request(0);
+        float w_mine[T], l[T], o[T][4];
+#pragma unroll
+        for (uint32_t t = 0; t < T; ++t) {
+            const float m = lane < n ? __uint_as_float(ml[t][0]) : -INFINITY, M = wave_max(m);
+            w_mine[t] = __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.f : M));
+            l[t] = wave_sum(lane < n ? __uint_as_float(ml[t][1]) * w_mine[t] : 0.f);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[t][r] = 0.f;
+        }
+        for (uint32_t from = 0;;) {
+#pragma unroll
+            for (uint32_t t = 0; t < T; ++t)
+#pragma unroll
+                for (uint32_t i = 0; i < N; ++i) {
+                    const uint32_t k = from + i * SPR + lane / LP;
+                    const float w = __int_as_float(__builtin_amdgcn_ds_bpermute((int)(k * 4u), __float_as_int(w_mine[t])));
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[t][r] = k < n ? fmaf(__uint_as_float(u[t][i][r]), w, o[t][r]) : o[t][r];
+                }
+            if ((from += GROUP) >= n) break;
+            request(from);
+        }
+#pragma unroll
+        for (uint32_t t = 0; t < T; ++t) {
+            if (c + t * step >= end) break;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {   // the parts that a request brought side by side
+                const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[t][r]), __float_as_uint(o[t][r]), false, false);
+                o[t][r] = __uint_as_float(h[0]) + __uint_as_float(h[1]);
+                if constexpr (SPR == 4) {
+                    const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(o[t][r]), __float_as_uint(o[t][r]), false, false);
+                    o[t][r] = __uint_as_float(q[0]) + __uint_as_float(q[1]);
+                }
+            }
+            if (lane < LP) put(c + t * step, lane * 4u, make_float4(o[t][0], o[t][1], o[t][2], o[t][3]), l[t]);
+            done(c + t * step);
+        }
+    }
+}
+
+// The parts of cut tiles of 128 columns joined, in a launch of its own: a block takes 16 columns of a tile, a wave one at a time.  (By the tile's last
+// item, as single tokens are, one CU reads all parts, 66 KB each: a chunk of 64 rows behind 8000 positions, 16 parts a tile, 45 us.)
+constexpr uint32_t kMergeCols = 16;
+template <int D>
+__global__ __launch_bounds__(256) void sdpa_paged_merge_kernel(const SdpaPagedArgs a) {
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const PagedItem it = paged_item<false, true>(a, blockIdx.x / (kTileCols / kMergeCols), lane);
+    if (!it.any) return;
+    const uint32_t G = a.group, columns = it.s.rows * G, e_tile = it.tile * kTileCols, c0 = blockIdx.x % (kTileCols / kMergeCols) * kMergeCols;
+    if (columns <= kFewMost || e_tile + c0 >= columns) return;
+    const PagedRange range = paged_range<kTileStep>(a, it, e_tile, columns - e_tile < kTileCols ? columns - 1u : e_tile + kTileCols - 1u);
+    if (range.n_active == 1u) return;
+    constexpr uint32_t SLOT = kTileCols * (D + 2u) * 4u;
+    const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials, 0, (int)(a.slots * SLOT), 0x27000);
+    const uint32_t left = columns - e_tile, end = left < c0 + kMergeCols ? left : c0 + kMergeCols;
+    bool odd = false;
+    auto put = [&](uint32_t c, uint32_t d, const float4& o, float l) {
+        const float f = l > 0.f || l != l ? 1.0f / l : 0.f;   // (a row that sees nothing: zeros)
+        const float t = (__builtin_fabsf(o.x) + __builtin_fabsf(o.y)) + (__builtin_fabsf(o.z) + __builtin_fabsf(o.w));
+        const uint32_t e = e_tile + c, place = e / G;
+        *reinterpret_cast<uint2*>(a.out + (size_t)(it.s.row0 + place) * a.out_stride + (size_t)(it.kvh * G + (e - place * G)) * D + d) =
+            make_uint2(pack_bf16(o.x * f, o.y * f), pack_bf16(o.z * f, o.w * f));
+        odd = !(t * f < INFINITY);
+    };
+    auto done = [&](uint32_t c) {
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd) != 0, 0)) {
+            const uint32_t e = e_tile + c, place = e / G;
+            paged_row<D>(a, it.seq, it.s, place, it.kvh * G + (e - place * G), lane);
+            odd = false;
+        }
+    };
+    if (range.n_active <= 8u) paged_merge_columns<D, 0, 8, 2>(mem, it.base, a.b.n_kv, SLOT, kTileCols * D * 4u, c0 + wave, end, 4u, range.n_active, lane, put, done);
+    else paged_merge_columns<D, 0, 16, 1>(mem, it.base, a.b.n_kv, SLOT, kTileCols * D * 4u, c0 + wave, end, 4u, range.n_active, lane, put, done);
 }
 
 // ---- single tokens: at most 16 columns of a sequence and KV head ----
@@ -532,14 +582,12 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
     const uint32_t G = a.group, e0 = it.tile * kFewCols, left_cols = it.s.rows * G - e0, columns = left_cols < kFewCols ? left_cols : kFewCols;   // of this tile
     auto limit_of = [&](uint32_t place) { return it.s.len + place + 1u > it.s.rows ? it.s.len + place + 1u - it.s.rows : 0u; };
     auto low_of = [&](uint32_t limit) { return a.window && limit > a.window ? limit - a.window : 0u; };
-    const uint32_t kv_end = __builtin_amdgcn_readfirstlane(limit_of((e0 + columns - 1u) / G)), lim_lo = __builtin_amdgcn_readfirstlane(limit_of(e0 / G));
-    const uint32_t low_lo = __builtin_amdgcn_readfirstlane(low_of(lim_lo)), low_hi = __builtin_amdgcn_readfirstlane(low_of(kv_end));
-    const uint32_t round0 = low_lo / kFewRound, rounds = (kv_end + kFewRound - 1u) / kFewRound - (kv_end ? round0 : 0u);
-    const uint32_t per = (rounds + it.n_splits - 1u) / it.n_splits;
-    const uint32_t n_active = per ? (rounds + per - 1u) / per : 1u;
+    const PagedRange range = paged_range<kFewRound>(a, it, e0, e0 + columns - 1u);
+    const uint32_t kv_end = range.kv_end, n_active = range.n_active, lim_lo = __builtin_amdgcn_readfirstlane(limit_of(e0 / G));
+    const uint32_t low_hi = __builtin_amdgcn_readfirstlane(low_of(kv_end));
     if (it.split >= n_active) return;
-    const uint32_t first = (round0 + it.split * per) * kFewRound + wave * kFewStep;
-    uint32_t end = (round0 + (it.split + 1u) * per) * kFewRound;
+    const uint32_t first = (range.step0 + it.split * range.per) * kFewRound + wave * kFewStep;
+    uint32_t end = (range.step0 + (it.split + 1u) * range.per) * kFewRound;
     end = __builtin_amdgcn_readfirstlane(end < kv_end ? end : kv_end);
     const uint32_t n_steps = __builtin_amdgcn_readfirstlane(end > first ? (end - first + kFewRound - 1u) / kFewRound : 0u);
 
@@ -777,54 +825,16 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
         }
     }
     if (!whole) {   // the item that arrives last merges the sequence's, in their order
-        const uint32_t stride = a.b.n_kv, base = blockIdx.x - it.split * stride;   // the slot of the tile's first item
+        const uint32_t stride = a.b.n_kv, base = it.base;
         wait_memory_ops_done();
         __syncthreads();
         if (tid == 0) word[0] = atomicAdd(&a.counters[base], 1u) == n_active - 1u ? 1u : 0u;
         __syncthreads();
         if (!word[0]) return;
         if (tid == 0) __hip_atomic_store(&a.counters[base], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        // a wave a column: every partial of it is requested before the first is looked at
-        constexpr uint32_t LP = D / 4u, SPR = 64u / LP;   // lanes of a partial, partials of a request
-        for (uint32_t c = wave; c < columns; c += 4u) {
-            const pf_u32x2_t ml = __builtin_bit_cast(pf_u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(
-                mem, (int)((base + (lane < n_active ? lane : 0u) * stride) * SLOT + (kFewCols * D + c * 2u) * 4u), 0, kPastCaches));
-            auto merge = [&](auto count) __attribute__((always_inline)) {
-                constexpr uint32_t N = decltype(count)::value / SPR;
-                pf_u32x4_t u[N];
-#pragma unroll
-                for (uint32_t i = 0; i < N; ++i) {
-                    const uint32_t k = i * SPR + lane / LP;
-                    u[i] = __builtin_bit_cast(pf_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                        mem, (int)((base + (k < n_active ? k : 0u) * stride) * SLOT + (c * D + (lane % LP) * 4u) * 4u), 0, kPastCaches));
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                const float m = lane < n_active ? __uint_as_float(ml[0]) : -INFINITY, M = wave_max(m);
-                const float w_mine = __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.f : M));
-                const float l = wave_sum(lane < n_active ? __uint_as_float(ml[1]) * w_mine : 0.f);
-                float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (uint32_t i = 0; i < N; ++i) {
-                    const uint32_t k = i * SPR + lane / LP;
-                    const float w = __int_as_float(__builtin_amdgcn_ds_bpermute((int)(k * 4u), __float_as_int(w_mine)));
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[r] = k < n_active ? fmaf(__uint_as_float(u[i][r]), w, o[r]) : o[r];
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {   // the partials that a request brought side by side
-                    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[r]), __float_as_uint(o[r]), false, false);
-                    o[r] = __uint_as_float(h[0]) + __uint_as_float(h[1]);
-                    if constexpr (SPR == 4) {
-                        const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(o[r]), __float_as_uint(o[r]), false, false);
-                        o[r] = __uint_as_float(q[0]) + __uint_as_float(q[1]);
-                    }
-                }
-                if (lane < LP) store(c, lane * 4u, make_float4(o[0], o[1], o[2], o[3]), l);
-            };
-            if (n_active <= 8u) merge(std::integral_constant<uint32_t, 8>{});
-            else if (n_active <= 24u) merge(std::integral_constant<uint32_t, 24>{});
-            else merge(std::integral_constant<uint32_t, kMostSplits>{});
-        }
+        auto none = [](uint32_t) {};
+        if (n_active <= 8u) paged_merge_columns<D, kPastCaches, 8, 4>(mem, base, stride, SLOT, kFewCols * D * 4u, wave, columns, 4u, n_active, lane, store, none);
+        else paged_merge_columns<D, kPastCaches, 32, 1>(mem, base, stride, SLOT, kFewCols * D * 4u, wave, columns, 4u, n_active, lane, store, none);
     }
     __syncthreads();
     for (uint32_t again = word[1], c = 0; again; again >>= 1, ++c)
@@ -862,15 +872,14 @@ PagedPlan paged_plan(bool few, uint32_t n_heads, uint32_t n_kv, uint32_t head_di
     PagedPlan p;
     const uint32_t cols = few ? kFewCols : kTileCols;
     p.few = few;
-    p.target = few ? 768 : 640;
-    p.min_steps = few ? 1 : 8;
+    p.target = few ? 768 : 512;
+    p.min_steps = few ? 1 : 4;
     // (a sequence of up to kFewMost columns has tiles of 16 also among chunks)
     const uint64_t columns = (uint64_t)rows * (n_heads / n_kv);
     p.tiles = few ? (columns / kFewCols + n_seqs) * n_kv : (columns / kTileCols + (uint64_t)n_seqs * (kFewMost / kFewCols)) * n_kv;
     p.slot_bytes = (size_t)cols * (head_dim + 2) * 4;
-    // (an item more for every tile: what is cut into items of equal work has one that is not full)
     const uint32_t most = few ? 2048 : 896;   // slots: 64 MB at the most
-    p.slots = p.tiles <= most / 2 ? std::min((uint32_t)p.tiles + p.target, most) : 0;
+    p.slots = p.tiles <= most / 2 ? std::min((uint32_t)p.tiles + p.target, most) : 0;   // (rounding leaves an item more for every tile)
     p.target = p.slots ? p.slots - (uint32_t)p.tiles : p.target;
     p.bytes = kPagedCounterBytes + p.slots * p.slot_bytes;
     return p;
@@ -925,15 +934,28 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
         {{reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, true>)},
          {reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, true>)}}};
     l->func = p.few ? few[D == 128][softcap > 0.f][batch->max_rows * (n_heads / n_kv) > 8u] : tile[D == 128][softcap > 0.f];
+    // Positions that a tile can see, in steps.  Chunks of up to 8 steps are not cut: the merge costs what it saves (a prompt of 512 rows, 32 / 8 heads x
+    // 128: 18 us whole, 24 in halves).
+    const uint32_t step = p.few ? kFewRound : kTileStep, span = (p.few ? kFewCols : kTileCols) / a.group + 2u;
+    const uint64_t seen = window ? std::min<uint64_t>(batch->max_len, (uint64_t)window + std::min(batch->max_rows, span) + step) : batch->max_len;
+    const uint32_t most = (uint32_t)((seen + step - 1u) / step), splits = (most + p.min_steps - 1u) / p.min_steps;
+    const bool cut = p.slots && (p.few ? splits > 1u : most > 8u);
+    if (!cut) a.slots = 0;
     // (no more blocks than there can be items: one that finds none costs what it takes to look)
-    const uint32_t step = p.few ? kFewRound : kTileStep, most = (batch->max_len + step - 1u) / step, splits = (most + p.min_steps - 1u) / p.min_steps;
-    const uint64_t items = p.slots ? std::min<uint64_t>(p.slots, p.tiles * splits) : p.tiles;
-    l->grid = dim3((uint32_t)items, 1, 1);
+    l->grid = dim3((uint32_t)(cut ? std::min<uint64_t>(p.slots, p.tiles * splits) : p.tiles), 1, 1);
     l->block = dim3(256, 1, 1);
-    l->shmem = p.few ? few_lds_bytes(D) : tile_lds_bytes(D);
+    l->shmem = p.few ? few_lds_bytes(D) : std::max(tile_lds_bytes(D), few_lds_bytes(D));
     if ((int)l->shmem > dev->max_dyn_lds) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: LDS tile does not fit");
     FK_TRY(raise_dynamic_lds(l->func, l->shmem));
     l->set_args(a);
+    if (!p.few && cut) {
+        Launch m;
+        m.func = D == 64 ? reinterpret_cast<const void*>(&sdpa_paged_merge_kernel<64>) : reinterpret_cast<const void*>(&sdpa_paged_merge_kernel<128>);
+        m.grid = dim3((uint32_t)p.tiles * (kTileCols / kMergeCols), 1, 1);
+        m.block = dim3(256, 1, 1);
+        m.set_args(a);
+        l->then.push_back(m);
+    }
     return FK_OK;
 }
 
