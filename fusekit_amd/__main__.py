@@ -4,6 +4,9 @@
   generate --model DIR --ids 1,2,3 [--max-tokens N] [--capacity C]
                                          greedy decode of an mlx-lm format checkpoint (token ids in,
                                          token ids out; no tokenizer is bundled)
+  generate --model DIR --ids 1,2,3 --beams N [--eos T]
+                                         beam search over a paged cache (dense decoders): the N likeliest continuations
+                                         and the sums of their log probabilities
   export-random --out DIR [--bits 4] [--layers 2] [--moe] ...
                                          write a small random-init model in the mlx-lm file layout (--moe: a
                                          mixture-of-experts model in the deepseek_v2 layout; generate / patch
@@ -32,6 +35,8 @@ def main() -> int:
     g.add_argument("--max-tokens", type=int, default=32)
     g.add_argument("--capacity", type=int, default=1024)
     g.add_argument("--artifact", default=None, help="directory written by `patch`")
+    g.add_argument("--beams", type=int, default=0, help="beam search with this many beams (1 to 64)")
+    g.add_argument("--eos", type=int, default=None, help="with --beams: the token that ends a continuation")
     pa = sub.add_parser("patch")
     pa.add_argument("--model", required=True)
     pa.add_argument("--out", default=None)
@@ -85,6 +90,8 @@ def main() -> int:
         from .artifact import ArtifactRuntime, write_artifact
         from .checkpoint import load_moe_checkpoint
         from .moe_decoder import MoeRuntime
+        if args.cmd == "generate" and args.beams:
+            ap.error("--beams: beam search runs dense decoders")
         cfg, w = load_moe_checkpoint(args.model, capacity=args.capacity)
         if args.cmd == "patch":
             rt = MoeRuntime(cfg, w)
@@ -112,6 +119,17 @@ def main() -> int:
         print(json.dumps({"artifact": out, "tasks": len(rt.tasks), "variants": [f"prefill_m{m}" for m in ms]}))
         return 0
     prompt = [int(t) for t in args.ids.split(",") if t.strip()]
+    if args.beams:
+        from .paged import PagedDecoder
+        if args.artifact:
+            ap.error("--beams runs from the checkpoint, not from an artifact")
+        rows = 16
+        # the prompt's pages, and for every beam those of its own tokens and of its tail before and after a step
+        pages = -(-len(prompt) // rows) + 2 * args.beams * (-(-args.max_tokens // rows) + 2)
+        dec = PagedDecoder(cfg, w, pages, rows, max_rows=max(64, min(512, len(prompt))), max_seqs=args.beams)
+        found = dec.beam_search(prompt, args.beams, args.max_tokens, args.eos)
+        print(json.dumps({"beams": [{"tokens": t, "log_probability": round(p, 5)} for t, p in found]}))
+        return 0
     if args.artifact:
         from .artifact import ArtifactRuntime
         art = ArtifactRuntime(args.artifact, w)

@@ -514,7 +514,7 @@ fk_status plan_beam_select(const uint16_t* logits, size_t row_stride, const floa
 struct ReorderArgs {
     const void* src;
     void* dst;
-    size_t columns;
+    size_t src_stride, dst_stride, columns;   // in values of T
     const uint32_t* parents;
     uint32_t beams, n_out;
 };
@@ -523,19 +523,19 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(const ReorderArgs a) 
     const size_t c = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (c >= a.columns) return;
     const uint32_t g = blockIdx.y, first = blockIdx.z * N;
-    const T* src = static_cast<const T*>(a.src) + (size_t)g * a.beams * a.columns + c;
-    T* dst = static_cast<T*>(a.dst) + ((size_t)g * a.n_out + first) * a.columns + c;
+    const T* src = static_cast<const T*>(a.src) + (size_t)g * a.beams * a.src_stride + c;
+    T* dst = static_cast<T*>(a.dst) + ((size_t)g * a.n_out + first) * a.dst_stride + c;
     const uint32_t* parents = a.parents + (size_t)g * a.n_out + first;
     const uint32_t rows = a.n_out - first;
     T v[N];
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i) {
         const uint32_t p = parents[i < rows ? i : rows - 1u];
-        v[i] = src[(size_t)(p < a.beams ? p : a.beams - 1u) * a.columns];
+        v[i] = src[(size_t)(p < a.beams ? p : a.beams - 1u) * a.src_stride];
     }
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i)
-        if (i < rows) dst[(size_t)i * a.columns] = v[i];
+        if (i < rows) dst[(size_t)i * a.dst_stride] = v[i];
 }
 
 namespace {
@@ -548,22 +548,26 @@ const void* reorder_form(uint32_t rows, uint32_t* held) {
 }
 }  // namespace
 
-fk_status plan_beam_reorder(const void* src, void* dst, size_t row_bytes, const uint32_t* parents, uint32_t groups, uint32_t beams, uint32_t n_out, Launch* l) {
+fk_status plan_beam_reorder(const void* src, size_t src_stride, void* dst, size_t dst_stride, size_t row_bytes, const uint32_t* parents, uint32_t groups,
+                            uint32_t beams, uint32_t n_out, Launch* l) {
     if (!src || !dst || !parents) return set_error(FK_ERR_INVALID, "beam_reorder: null pointer");
     if (row_bytes == 0 || groups == 0 || beams == 0 || n_out == 0) return set_error(FK_ERR_INVALID, "beam_reorder: empty shape");
     if (beams > kBeamMax || n_out > kBeamMax) return set_error(FK_ERR_UNSUPPORTED, "beam_reorder: beams up to 64");
     if (groups > 65535) return set_error(FK_ERR_UNSUPPORTED, "beam_reorder: more than 65535 groups");
+    if (src_stride < row_bytes || dst_stride < row_bytes) return set_error(FK_ERR_INVALID, "beam_reorder: a row stride is shorter than the row");
     if ((uintptr_t)parents & 3u) return set_error(FK_ERR_INVALID, "beam_reorder: parents must be 4-byte aligned");
-    if (row_bytes > (SIZE_MAX >> 1) / ((size_t)groups * kBeamMax)) return set_error(FK_ERR_UNSUPPORTED, "beam_reorder: state too large");
-    const uintptr_t s0 = (uintptr_t)src, d0 = (uintptr_t)dst, sn = (size_t)groups * beams * row_bytes, dn = (size_t)groups * n_out * row_bytes;
-    if (s0 == d0 ? n_out != beams : (s0 < d0 + dn && d0 < s0 + sn))
-        return set_error(FK_ERR_INVALID, "beam_reorder: src and dst must be one buffer with n_out == beams, or not overlap");
+    if (std::max(src_stride, dst_stride) > (SIZE_MAX >> 1) / ((size_t)groups * kBeamMax)) return set_error(FK_ERR_UNSUPPORTED, "beam_reorder: state too large");
+    const uintptr_t s0 = (uintptr_t)src, d0 = (uintptr_t)dst;
+    const size_t sn = ((size_t)groups * beams - 1) * src_stride + row_bytes, dn = ((size_t)groups * n_out - 1) * dst_stride + row_bytes;
+    const bool in_place = s0 == d0;
+    if (in_place ? n_out != beams || src_stride != dst_stride : (s0 < d0 + dn && d0 < s0 + sn))
+        return set_error(FK_ERR_INVALID, "beam_reorder: src and dst must be the same rows, n_out then being beams, or not overlap");
     const DeviceFacts* dev;
     FK_TRY(device_facts(&dev));
-    const bool in_place = s0 == d0;
     const uint32_t rows = in_place ? n_out : std::min(n_out, 8u);
-    const uint32_t width = (s0 | d0 | row_bytes) % 16 == 0 && rows <= 16 ? 16 : (s0 | d0 | row_bytes) % 4 == 0 ? 4 : 1;
-    ReorderArgs a{src, dst, row_bytes / width, parents, beams, n_out};
+    const uintptr_t all = s0 | d0 | row_bytes | src_stride | dst_stride;
+    const uint32_t width = all % 16 == 0 && rows <= 16 ? 16 : all % 4 == 0 ? 4 : 1;
+    ReorderArgs a{src, dst, src_stride / width, dst_stride / width, row_bytes / width, parents, beams, n_out};
     if ((a.columns + 255) / 256 > 0x7fffffffu) return set_error(FK_ERR_UNSUPPORTED, "beam_reorder: rows too long");
     uint32_t held = 1;
     l->func = width == 16 ? reorder_form<fk_u32x4_t, 2, 4, 8, 16>(rows, &held)

@@ -1040,10 +1040,10 @@ fk_status fk_beam_select(const uint16_t* logits, size_t row_stride, const float*
     return run_launch(l, (hipStream_t)s);
 }
 
-fk_status fk_beam_reorder(const void* src, void* dst, size_t row_bytes, const uint32_t* parents, uint32_t groups, uint32_t beams, uint32_t n_out,
-                          fk_stream s) {
+fk_status fk_beam_reorder(const void* src, size_t src_stride, void* dst, size_t dst_stride, size_t row_bytes, const uint32_t* parents,
+                          uint32_t groups, uint32_t beams, uint32_t n_out, fk_stream s) {
     Launch l;
-    FK_TRY(plan_beam_reorder(src, dst, row_bytes, parents, groups, beams, n_out, &l));
+    FK_TRY(plan_beam_reorder(src, src_stride, dst, dst_stride, row_bytes, parents, groups, beams, n_out, &l));
     return run_launch(l, (hipStream_t)s);
 }
 

@@ -413,8 +413,8 @@ fk_status beam_select_workspace_bytes(uint32_t groups, uint32_t beams, uint32_t 
 fk_status plan_beam_select(const uint16_t* logits, size_t row_stride, const float* scores, const uint32_t* finished, uint32_t pad_token,
                            uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k, float* out_scores, uint32_t* out_beams,
                            uint32_t* out_tokens, void* workspace, size_t workspace_bytes, Launch* out);
-fk_status plan_beam_reorder(const void* src, void* dst, size_t row_bytes, const uint32_t* parents, uint32_t groups, uint32_t beams,
-                            uint32_t n_out, Launch* out);
+fk_status plan_beam_reorder(const void* src, size_t src_stride, void* dst, size_t dst_stride, size_t row_bytes, const uint32_t* parents,
+                            uint32_t groups, uint32_t beams, uint32_t n_out, Launch* out);
 fk_status plan_step_init(uint32_t* step_counter, uint32_t* offset, uint32_t* kv_len, Launch* out,
                          float* rope_tab = nullptr, uint32_t rope_dims = 0, float base_log2 = 0.f);
 fk_status plan_fill_u32(void* p, uint32_t value, size_t count, Launch* out);

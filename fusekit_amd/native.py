@@ -723,9 +723,11 @@ def beam_select(logits, row_stride, scores, finished, pad_token, groups, beams, 
                              _addr(out_scores), _addr(out_beams), _addr(out_tokens), _addr(workspace), workspace_bytes, _addr(stream)))
 
 
-def beam_reorder(src, dst, row_bytes, parents, groups, beams, n_out, stream=None):
-    """dst[g, i] = src[g, parents[g, i]], rows of row_bytes (fk_beam_reorder); dst may be src where n_out == beams."""
-    check(lib.fk_beam_reorder(_addr(src), _addr(dst), row_bytes, _addr(parents), groups, beams, n_out, _addr(stream)))
+def beam_reorder(src, dst, row_bytes, parents, groups, beams, n_out, stream=None, src_stride=None, dst_stride=None):
+    """dst[g, i] = src[g, parents[g, i]], rows of row_bytes, side by side unless strides say otherwise (fk_beam_reorder); dst may be src where
+    n_out == beams."""
+    check(lib.fk_beam_reorder(_addr(src), row_bytes if src_stride is None else src_stride, _addr(dst), row_bytes if dst_stride is None else dst_stride,
+                              row_bytes, _addr(parents), groups, beams, n_out, _addr(stream)))
 
 
 def copy(dst, src, nbytes, stream=None):
@@ -826,7 +828,7 @@ _SIGNATURES = {
     "fk_xcd_kslice_meta": "puupp", "fk_xcd_check": "pp", "fk_route_order": "puupp", "fk_set_gemv_policy": "uu",
     "fk_rope_frequencies": "udidddupp", "fk_rope_paged_store": "pupupupuuppfuipBPp", "fk_sdpa_paged_workspace_bytes": "uuuuuup",
     "fk_sdpa_paged": "pupuuffuBPpzp", "fk_paged_check": "pp", "fk_pages_copy": "puzuzpup", "fk_beam_select_workspace_bytes": "uuuup",
-    "fk_beam_select": "pzppuuuuuppppzp", "fk_beam_reorder": "ppzpuuup",
+    "fk_beam_select": "pzppuuuuuppppzp", "fk_beam_reorder": "pzpzzpuuup",
     "fk_set_qgemm_wide": "i", "fk_set_gemv_flat_only": "i", "fk_stream_sync": "p",
 }
 

@@ -657,12 +657,13 @@ fk_status fk_beam_select(const uint16_t *logits, size_t row_stride, const float 
                          uint32_t pad_token, uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k,
                          float *out_scores, uint32_t *out_beams, uint32_t *out_tokens, void *workspace,
                          size_t workspace_bytes, fk_stream s);
-/* Rows of per-beam state follow the beams that were chosen: dst[g * n_out + i] = src[g * beams + parents[g * n_out + i]], rows of
- * row_bytes (any number).  dst may be src where n_out == beams (rows are then exchanged in place); otherwise the two
+/* Rows of per-beam state follow the beams that were chosen: dst row g * n_out + i becomes src row g * beams + parents[g * n_out + i], rows of
+ * row_bytes (any number) that lie src_stride / dst_stride bytes apart (a column of a history, part of a wider state).  dst
+ * may be src where n_out == beams and the strides are the same (rows are then exchanged in place); otherwise what the two span
  * must not overlap.  parents: device u32 [groups, n_out]; an index beyond the group's beams takes the last one.  beams,
  * n_out up to 64. */
-fk_status fk_beam_reorder(const void *src, void *dst, size_t row_bytes, const uint32_t *parents, uint32_t groups, uint32_t beams,
-                          uint32_t n_out, fk_stream s);
+fk_status fk_beam_reorder(const void *src, size_t src_stride, void *dst, size_t dst_stride, size_t row_bytes, const uint32_t *parents,
+                          uint32_t groups, uint32_t beams, uint32_t n_out, fk_stream s);
 
 /* E   x = T(embed[token] * out_scale), dense bf16 or MLX-affine table.  Replaces
  *     src/codegen/kernels/embed_lookup_decode.rs:17-108. */

@@ -152,3 +152,23 @@ def test_reorder_takes_the_last_beam_for_an_index_beyond(fk):
     fk.beam_reorder(s, s, 128, p, 1, 4, 4)
     fk.sync()
     assert bool((s.to_numpy(np.uint32, src.shape) == src[:, [3, 3, 3, 0]]).all())
+
+
+@pytest.mark.parametrize("row,src_stride,dst_stride", [(4, 4, 400), (4, 36, 4), (16, 48, 160), (7, 9, 30), (64, 128, 64)])
+@pytest.mark.parametrize("groups,n_beams,n_out", [(1, 4, 4), (3, 5, 5), (2, 3, 20)])
+def test_reorder_rows_that_lie_apart(fk, row, src_stride, dst_stride, groups, n_beams, n_out):
+    src = rng(row).integers(0, 256, (groups, n_beams, src_stride), dtype=np.uint8)
+    old = rng(row + 1).integers(0, 256, (groups, n_out, dst_stride), dtype=np.uint8)
+    parents = rng(n_out).integers(0, n_beams, (groups, n_out)).astype(np.uint32)
+    s, d, p = fk.DeviceBuffer.from_numpy(src), fk.DeviceBuffer.from_numpy(old), fk.DeviceBuffer.from_numpy(parents)
+    fk.beam_reorder(s, d, row, p, groups, n_beams, n_out, src_stride=src_stride, dst_stride=dst_stride)
+    fk.sync()
+    ref = old.copy()
+    ref[:, :, :row] = np.take_along_axis(src, parents[:, :, None].astype(np.int64), 1)[:, :, :row]
+    assert bool((d.to_numpy(np.uint8, old.shape) == ref).all())
+    if n_out == n_beams:                       # in place, what lies between the rows stays
+        fk.beam_reorder(s, s, row, p, groups, n_beams, n_out, src_stride=src_stride, dst_stride=src_stride)
+        fk.sync()
+        ref = src.copy()
+        ref[:, :, :row] = np.take_along_axis(src, parents[:, :, None].astype(np.int64), 1)[:, :, :row]
+        assert bool((s.to_numpy(np.uint8, src.shape) == ref).all())

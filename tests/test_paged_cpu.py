@@ -131,11 +131,91 @@ def test_select(change):
 
 @pytest.mark.parametrize("change", [dict(src=None), dict(dst=None), dict(parents=None), dict(row=0), dict(groups=0), dict(beams=0), dict(out=0),
                                     dict(beams=65), dict(out=65), dict(groups=70000), dict(parents=A + 2), dict(dst=A, out=3), dict(dst=A + 100),
-                                    dict(dst=A - 100), dict(row=1 << 60)], ids=str)
+                                    dict(dst=A - 100), dict(row=1 << 60), dict(src_stride=63), dict(dst_stride=60), dict(dst=A, dst_stride=128),
+                                    dict(dst=A + 64, src_stride=256, dst_stride=256), dict(src_stride=2048)], ids=str)
 def test_reorder(change):
-    v = dict(src=A, dst=A + 8192, row=64, parents=A, groups=2, beams=4, out=4)
+    v = dict(src=A, dst=A + 8192, row=64, parents=A, groups=2, beams=4, out=4, stream=None, src_stride=None, dst_stride=None)
     v.update(change)
     refused(lambda: fk.beam_reorder(*v.values()))
+
+
+def make(n_pages=8, page_rows=4):
+    from fusekit_amd.paged import PageAllocator
+    return PageAllocator(n_pages, page_rows)
+
+
+def test_allocator_takes_shares_and_gives_back():
+    from fusekit_amd.paged import OutOfPages
+    a = make()
+    s, t = a.new(), a.new()
+    assert a.extend([s, t], [6, 0]) == [] and s.pages == [0, 1] and s.length == 6 and t.pages == []
+    f = a.fork(s)
+    assert f.pages == s.pages and a.users[0] == 2
+    # both write into the shared tail page: the first copies it, the second then has it to itself
+    assert a.extend([f, s], [1, 1]) == [(1, 2)] and f.pages == [0, 2] and s.pages == [0, 1]
+    assert a.extend([s], [2]) == [] and s.pages == [0, 1, 3]                       # 7 + 2 positions: a page more, nothing shared is written
+    g = a.fork(f)
+    a.extend([f], [1])                                                             # (its tail page was shared)
+    assert f.pages == [0, 4] and g.pages == [0, 2]
+    h = a.fork(f)
+    assert a.extend([h], [1]) == [] and h.pages == [0, 4, 5] and a.users[4] == 2   # a full tail page stays shared
+    before = (a.users.copy(), a.free_pages, list(s.pages), s.length)
+    with pytest.raises(OutOfPages):
+        a.extend([s, t], [4, 8])
+    assert (a.users == before[0]).all() and (a.free_pages, s.pages, s.length) == before[1:]
+    for x in (s, f, g, h, t):
+        a.release(x)
+    assert a.free_pages == 8 and not a.users.any()
+
+
+def test_allocator_copies_are_what_pages_copy_takes():
+    """Sources are never destinations, and no destination comes twice, whatever is forked."""
+    a, rng = make(200, 4), np.random.Generator(np.random.PCG64(1))
+    live = [a.new()]
+    a.extend(live, [7])
+    for _ in range(200):
+        parents = rng.integers(0, len(live), 5)
+        children = [a.fork(live[p]) for p in parents]
+        for s in live:
+            a.release(s)
+        live = children
+        pairs = a.extend(live, rng.integers(0, 6, 5))
+        src, dst = {p for p, _ in pairs}, [q for _, q in pairs]
+        assert len(set(dst)) == len(dst) and not src & set(dst)
+        held = [p for s in live for p in s.pages]
+        assert all(a.users[p] == held.count(p) for p in set(held)) and a.free_pages == 200 - len(set(held))
+        if max(s.length for s in live) > 60:
+            for s in live:
+                a.truncate(s, min(s.length, 5))
+            assert all(-(-s.length // 4) == len(s.pages) for s in live)
+
+
+def test_allocator_compacts():
+    a = make(10, 4)
+    s = [a.new() for _ in range(5)]
+    a.extend(s, [8] * 5)
+    f = a.fork(s[4])
+    a.release(s[0])
+    a.release(s[2])
+    pairs = a.compact()
+    assert sorted(p for x in (s[1], s[3], s[4]) for p in x.pages) == list(range(6)) and f.pages == s[4].pages
+    assert {q for _, q in pairs} == {0, 1, 4, 5} and {p for p, _ in pairs} == {6, 7, 8, 9} and a.compact() == [] and a.free_pages == 4
+    a.extend([s[1]], [4])
+    assert s[1].pages[-1] == 6
+
+
+def test_allocator_refusals():
+    a = make()
+    s, other = a.new(), make().new()
+    a.extend([s], [5])
+    for bad in (lambda: make(0, 4), lambda: make(4, 0), lambda: a.extend([s, s], [1, 1]), lambda: a.extend([s], [1, 2]), lambda: a.extend([s], [-1]),
+                lambda: a.extend([other], [1]), lambda: a.fork(other), lambda: a.release(other), lambda: a.truncate(s, 6), lambda: a.truncate(s, -1)):
+        with pytest.raises(ValueError):
+            bad()
+    a.release(s)
+    for bad in (lambda: a.release(s), lambda: a.fork(s), lambda: a.extend([s], [1]), lambda: a.table([s], 4)):
+        with pytest.raises(ValueError):
+            bad()
 
 
 def test_sound_calls_ask_for_the_device():
