@@ -211,6 +211,11 @@ fk_status plan_rope_paged_store(const uint16_t* q, uint32_t q_stride, const uint
         return set_error(FK_ERR_INVALID, "rope_paged_store: pointers must be 16-byte aligned");
     if (((uintptr_t)q_norm | (uintptr_t)k_norm) & 1u) return set_error(FK_ERR_INVALID, "rope_paged_store: norms must be 2-byte aligned");
     if (!(eps >= 0.f)) return set_error(FK_ERR_INVALID, "rope_paged_store: eps must not be negative");
+    const size_t qw = (size_t)n_heads * D, kw = (size_t)n_kv * D;
+    if (!(q_out == q && q_out_stride == q_stride) && rows_overlap(q, q_stride, qw, q_out, q_out_stride, qw, batch->rows))
+        return set_error(FK_ERR_INVALID, "rope_paged_store: q_out must be q, with its stride, or not overlap it");
+    if (rows_overlap(k, k_stride, kw, q_out, q_out_stride, qw, batch->rows) || rows_overlap(v, v_stride, kw, q_out, q_out_stride, qw, batch->rows))
+        return set_error(FK_ERR_INVALID, "rope_paged_store: q_out overlaps k or v");
     const DeviceFacts* dev;
     FK_TRY(device_facts(&dev));
     a.q = q; a.k = k; a.v = v; a.q_out = q_out; a.q_norm = q_norm; a.k_norm = k_norm;

@@ -18,6 +18,16 @@ struct PagedArgs {
 // Checks a batch and a pool and makes the argument block of them (host).
 fk_status paged_args(const char* what, const fk_paged_batch* batch, const fk_page_pool* pool, PagedArgs* out);
 
+// Whether rows of `a_width` and `b_width` values that lie `a_stride` and `b_stride` apart share a byte, `rows` of each: column blocks of one wider row
+// do not (host).
+inline bool rows_overlap(const uint16_t* a, size_t a_stride, size_t a_width, const uint16_t* b, size_t b_stride, size_t b_width, size_t rows) {
+    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b, a1 = a0 + 2 * ((rows - 1) * a_stride + a_width), b1 = b0 + 2 * ((rows - 1) * b_stride + b_width);
+    if (a1 <= b0 || b1 <= a0) return false;
+    if (a_stride != b_stride) return true;
+    const uintptr_t apart = a0 < b0 ? (b0 - a0) % (2 * a_stride) : (a0 - b0) % (2 * a_stride);   // of a row's start behind the other's
+    return apart < 2 * (a0 < b0 ? a_width : b_width) || apart + 2 * (a0 < b0 ? b_width : a_width) > 2 * a_stride;
+}
+
 __device__ __forceinline__ void paged_fault(const PagedArgs& b, uint32_t bit) {
     if (b.fault) __hip_atomic_fetch_or(b.fault, bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }

@@ -911,7 +911,13 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     if ((q_stride | out_stride) % 8) return set_error(FK_ERR_INVALID, "sdpa_paged: strides must be multiples of 8 elements");
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15u) return set_error(FK_ERR_INVALID, "sdpa_paged: pointers must be 16-byte aligned");
     if (!(scale > 0.f) || !std::isfinite(scale)) return set_error(FK_ERR_INVALID, "sdpa_paged: scale must be positive");
+    if (!(scale * kLog2E < 3e38f)) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: scale too large");
     if (!(softcap >= 0.f) || !std::isfinite(softcap)) return set_error(FK_ERR_INVALID, "sdpa_paged: softcap must not be negative");
+    // (the kernels' tanh is off by 2^-23 of the cap, which is what a probability's exponent is then off by)
+    if (softcap > 1024.f || (softcap > 0.f && !std::isfinite(2.0f * scale * kLog2E / softcap)))
+        return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: softcap up to 1024, and not so small that scale / softcap overflows (0: none)");
+    if (rows_overlap(q, q_stride, (size_t)n_heads * D, out, out_stride, (size_t)n_heads * D, batch->rows))
+        return set_error(FK_ERR_INVALID, "sdpa_paged: out overlaps q");
     if ((uint64_t)batch->max_rows * (n_heads / n_kv) > 0x7fffffffull) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: too many rows of a sequence");
     size_t need = 0;
     FK_TRY(sdpa_paged_workspace_bytes(n_heads, n_kv, D, batch->n_seqs, batch->rows, batch->max_len, &need));

@@ -614,7 +614,7 @@ fk_status fk_rope_frequencies(uint32_t dims, double theta, int scaling, double f
                               uint32_t trained, double *d_freq, fk_stream s);
 /* R   for a batch over pages: rotates the first rope_dims of every q and k head of every new row at its position and
  *     appends k and v to the sequence's pages; the counterpart of fk_qkv_rope_store_rows.  q, k, v rows lie *_stride
- *     elements apart (column blocks of one packed row, for instance), q_out rows q_out_stride (q_out may be q).
+ *     elements apart (column blocks of one packed row, for instance), q_out rows q_out_stride (q_out may be q, else it overlaps none).
  *     interleaved: pairs (2 i, 2 i + 1), else (i, i + rope_dims / 2).  q_norm / k_norm [head_dim] (each may be NULL) first
  *     apply the per-head RMSNorm; everything up to the stored bf16 value is fp32 with one rounding, and the angle is formed
  *     and reduced in 64 bits (at 100 000 positions an fp32 angle is off by some 4e-3).  rope_dims a multiple of 16 up to
@@ -626,11 +626,14 @@ fk_status fk_rope_paged_store(const uint16_t *q, uint32_t q_stride, const uint16
                               int interleaved, const double *d_freq, const fk_paged_batch *batch,
                               const fk_page_pool *pool, fk_stream s);
 /* K4  for a batch over pages: row r of a sequence, at position p, attends to positions max(0, p - window + 1) .. p
- *     (window 0: from 0), n_heads / n_kv query heads to a KV head.  Scores q.k * scale, with softcap > 0
- *     softcap * tanh(score / softcap); fp32 scores, softmax and sums, one rounding of the output.  A row that sees
+ *     (window 0: from 0), n_heads / n_kv query heads to a KV head.  Scores q.k * scale, with softcap > 0 (up to 1024)
+ *     softcap * tanh(score / softcap); fp32 scores, softmax and sums, the probabilities of chunks in bf16 for the second
+ *     product (of up to 32 (row, head) pairs a KV head in 16 bits), one rounding of the output.  A row that sees
  *     nothing (a length below the new rows) is set to zeros.  K and V behind a sequence's length, and pages that hold none
  *     of its positions, may hold anything.  q, out: rows q_stride / out_stride elements apart, heads of a row adjacent;
- *     strides multiples of 8, pointers 16-byte aligned.  One launch serves chunks of prompts and single tokens together.
+ *     strides multiples of 8, pointers 16-byte aligned; out must not overlap q.  One call serves chunks of prompts and
+ *     single tokens together; a row's result does not depend on the other sequences but for the order in which its
+ *     positions are added up (how finely a long context is cut goes by the whole batch).
  *     workspace: fk_sdpa_paged_workspace_bytes() bytes (below 64 MB), zeroed before the first launch and left ready by each;
  *     launches that share it must not overlap, those of graphs included. */
 fk_status fk_sdpa_paged_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t n_seqs, uint32_t rows,

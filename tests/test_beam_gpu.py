@@ -52,6 +52,11 @@ def test_beams_and_k(fk, groups, n_beams, k):
     check(fk, *make(k, groups, n_beams, 3001), groups, n_beams, k)
 
 
+def test_more_lists_than_are_held_at_once(fk):
+    check(fk, *make(4, 2, 64, 70001), 2, 64, 64)
+    check(fk, *make(4, 1, 64, 70001, std=0.05), 1, 64, 64)    # ties, too
+
+
 def test_large_vocabulary(fk):
     check(fk, *make(5, 2, 8, 260003), 2, 8, 16)
     check(fk, *make(6, 1, 1, 151936), 1, 1, 1)

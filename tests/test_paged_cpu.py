@@ -5,7 +5,7 @@ import pytest
 
 import fusekit_amd.native as fk
 
-A = 0x10000   # an aligned address that nothing reads
+A, B, C = 0x10000, 0x100000, 0x200000   # aligned addresses that nothing reads
 
 
 def batch(**change):
@@ -34,14 +34,14 @@ def refused(call):
 
 
 def attend(b=None, p=None, **change):
-    v = dict(q=A, q_stride=256, out=A, out_stride=256, n_heads=4, scale=0.125, softcap=0.0, window=0, workspace=A, workspace_bytes=64 << 20)
+    v = dict(q=B, q_stride=256, out=C, out_stride=256, n_heads=4, scale=0.125, softcap=0.0, window=0, workspace=A, workspace_bytes=64 << 20)
     v.update(change)
     fk.sdpa_paged(v["q"], v["q_stride"], v["out"], v["out_stride"], v["n_heads"], v["scale"], v["softcap"], v["window"], b or batch(), p or pool(),
                   v["workspace"], v["workspace_bytes"])
 
 
 def store(b=None, p=None, **change):
-    v = dict(q=A, q_stride=512, k=A, k_stride=512, v=A, v_stride=512, q_out=A, q_out_stride=256, n_heads=4, q_norm=None, k_norm=None, eps=1e-6,
+    v = dict(q=B, q_stride=512, k=B + 512, k_stride=512, v=B + 768, v_stride=512, q_out=C, q_out_stride=256, n_heads=4, q_norm=None, k_norm=None, eps=1e-6,
              rope_dims=64, interleaved=0, freq=A)
     v.update(change)
     fk.rope_paged_store(*v.values(), b or batch(), p or pool())
@@ -62,7 +62,8 @@ def test_pools(change):
 @pytest.mark.parametrize("change", [dict(q=None), dict(out=None), dict(workspace=None), dict(n_heads=0), dict(n_heads=3), dict(n_heads=65536 * 2),
                                     dict(q_stride=255), dict(q_stride=260), dict(out_stride=248), dict(q=A + 2), dict(out=A + 8), dict(workspace=A + 4),
                                     dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(softcap=-1.0),
-                                    dict(softcap=float("nan")), dict(softcap=float("inf")), dict(workspace_bytes=0)], ids=str)
+                                    dict(softcap=float("nan")), dict(softcap=float("inf")), dict(softcap=1025.0), dict(softcap=1e-40), dict(scale=3e38), dict(workspace_bytes=0),
+                                    dict(out=B), dict(out=B + 512 * 3), dict(out=B + 2 * 128), dict(out=B - 512), dict(out=B + 2 * 256, q_stride=512, out_stride=264)], ids=str)
 def test_attention(change):
     refused(lambda: attend(**change))
 
@@ -70,7 +71,8 @@ def test_attention(change):
 @pytest.mark.parametrize("change", [dict(q=None), dict(k=None), dict(v=None), dict(q_out=None), dict(n_heads=0), dict(rope_dims=8), dict(rope_dims=80),
                                     dict(rope_dims=128), dict(freq=None), dict(freq=A + 4), dict(q_stride=248), dict(q_stride=260), dict(k_stride=120),
                                     dict(v_stride=130), dict(q_out_stride=255), dict(q=A + 2), dict(k=A + 8), dict(v=A + 4), dict(q_out=A + 2),
-                                    dict(q_norm=A + 1), dict(k_norm=A + 1), dict(eps=-1.0), dict(eps=float("nan"))], ids=str)
+                                    dict(q_norm=A + 1), dict(k_norm=A + 1), dict(eps=-1.0), dict(eps=float("nan")),
+                                    dict(q_out=B), dict(q_out=B + 16, q_out_stride=512), dict(q_out=B + 512, q_out_stride=512), dict(q_out=B + 1024 * 3)], ids=str)
 def test_rope_store(change):
     refused(lambda: store(**change))
 
@@ -221,7 +223,7 @@ def test_allocator_refusals():
 def test_sound_calls_ask_for_the_device():
     if fk.has_device():
         pytest.skip("a HIP device is present: the addresses are not real")
-    for call in (attend, store, lambda: fk.rope_frequencies(64, 1e4, A), lambda: fk.pages_copy(A, 2, 640, 10, 64, [[0, 1], [0, 2]]),
+    for call in (attend, store, lambda: store(q_out=B, q_out_stride=512), lambda: attend(q_stride=1024, out=B + 512, out_stride=1024), lambda: fk.rope_frequencies(64, 1e4, A), lambda: fk.pages_copy(A, 2, 640, 10, 64, [[0, 1], [0, 2]]),
                  lambda: fk.beam_select(A, 100, A, A, 3, 2, 4, 100, 8, A, A, A, A, 1 << 20), lambda: fk.beam_reorder(A, A, 64, A, 2, 4, 4)):
         with pytest.raises(fk.FusekitError) as e:
             call()

@@ -66,7 +66,7 @@ def test_window(fk, window, rows, lens):
     check_attention(fk, Paged(rows, lens, 2, 128, 64, seed=window), 8, window=window)
 
 
-@pytest.mark.parametrize("softcap", [0.5, 5.0, 50.0])
+@pytest.mark.parametrize("softcap", [0.5, 5.0, 50.0, 1024.0])
 @pytest.mark.parametrize("window", [0, 70])
 def test_softcap(fk, softcap, window):
     check_attention(fk, Paged([40, 1, 1], [200, 90, 700], 2, 128, 32, seed=1), 8, softcap=softcap, window=window)
