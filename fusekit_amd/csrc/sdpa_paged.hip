@@ -310,20 +310,24 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
         const uint32_t kv0 = step * kTileStep;
         if (kv0 >= last_limit || kv0 + kTileStep <= first_low) continue;   // nothing that a row of this wave sees
         const unsigned char *ks = lds + stage * STAGE, *vs = ks + TILE;
-        // all of a product's fragments are asked for before its first matrix instruction
-        pf_u32x4_t kf[KB][2];
-#pragma unroll
-        for (int j = 0; j < KB; ++j)
+        // (two of the eight pairs of fragments ahead of their matrix instructions; all of them first took 1 % longer of two chunks of 2048 rows, 2 % with a window)
+        pf_u32x4_t kf[3][2];
+        auto read_k = [&](auto j) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const uint32_t row = (uint32_t)t * 32u + nl;
-                kf[j][t] = *reinterpret_cast<const pf_u32x4_t*>(ks + row * ROW + (((uint32_t)(2 * j) + kb) ^ k_swizzle(row)) * 16u);
+                kf[j() % 3][t] = *reinterpret_cast<const pf_u32x4_t*>(ks + row * ROW + (((uint32_t)(2 * j()) + kb) ^ k_swizzle(row)) * 16u);
             }
+        };
+        read_k(std::integral_constant<int, 0>{});
+        read_k(std::integral_constant<int, 1>{});
         __builtin_amdgcn_sched_barrier(0);
         pf_f32x16_t s[2];
         static_for<KB>([&](auto j) __attribute__((always_inline)) {
-            mfma32_scores<j() == 0>(s[0], kf[j()][0], qreg[j()]);
-            mfma32_scores<j() == 0>(s[1], kf[j()][1], qreg[j()]);
+            if constexpr (j() + 2 < KB) read_k(std::integral_constant<int, j() + 2>{});
+            __builtin_amdgcn_sched_barrier(0);
+            mfma32_scores<j() == 0>(s[0], kf[j() % 3][0], qreg[j()]);
+            mfma32_scores<j() == 0>(s[1], kf[j() % 3][1], qreg[j()]);
         });
         __builtin_amdgcn_sched_barrier(0);
         pf_s16x4_t vf[4][DT][2];
@@ -383,7 +387,9 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
             const float p0 = __builtin_amdgcn_exp2f(fmaf(s[at / 16][at % 16], scale2, -m_sub));
             const float p1 = __builtin_amdgcn_exp2f(fmaf(s[at / 16][at % 16 + 1], scale2, -m_sub));
             l_run += p0 + p1;
-            pb[c()][w()] = pack_bf16(p0, p1);
+            uint32_t both = pack_bf16(p0, p1);
+            asm volatile("" : "+v"(both), "+v"(l_run));   // (made here: the compiler would gather them in one place)
+            pb[c()][w()] = both;
         };
         static_for<4>([&](auto w) __attribute__((always_inline)) { probabilities(std::integral_constant<int, 0>{}, w); });
         __builtin_amdgcn_sched_barrier(0);
