@@ -137,13 +137,15 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
     const float share = work / (float)a.target;
     uint32_t unit = share < 0x1p30f ? (uint32_t)ceilf(share) : 1u << 30;
     unit = unit < a.min_steps ? a.min_steps : unit;
+    const float of_steps = 1.0f / fmaxf(share, (float)a.min_steps);
     PagedItem it;
     it.any = false;
     uint32_t left = index, before = 0;   // items of the sequences before
     for (uint32_t at = 0; at < a.b.n_seqs; at += 64u) {
         if (a.b.n_seqs > 64u) mine = read(at);
         const uint32_t tiles = tiles_of(mine);
-        uint32_t splits = cut ? (steps_of(mine) + (FEW ? unit - 1u : 0u)) / unit : 1u;
+        // (tiles: as many as fit; an integer share gave a chunk of 512 rows behind 3000 384 items instead of 512)
+        uint32_t splits = !cut ? 1u : FEW ? (steps_of(mine) + unit - 1u) / unit : (uint32_t)fmaf((float)steps_of(mine), of_steps, 0x1p-10f);
         splits = splits < 1u ? 1u : splits > kMostSplits ? kMostSplits : splits;
         const uint32_t items = tiles * splits * n_kv;
         auto with_those_before = [&](uint32_t upto) {
