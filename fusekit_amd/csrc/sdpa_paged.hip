@@ -125,7 +125,7 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
     PagedSeq mine = read(0);
     for (uint32_t at = 0;;) {
         const float t = (float)tiles_of(mine) * (float)n_kv;
-        work += t * (float)steps_of(mine);
+        work = fmaf(t, (float)steps_of(mine), work);   // (the merge forms the same value)
         pairs += t;
         if ((at += 64u) >= a.b.n_seqs) break;
         mine = read(at);

@@ -161,10 +161,8 @@ class PagedDecoder:
         if self.rope_dims:
             self.freq = DeviceBuffer(8 * (self.rope_dims // 2 + 1))
             native.rope_frequencies(self.rope_dims, c.theta, self.freq, **(rope or {}), stream=stream)
-        self.stride = n_pages                                                      # a sequence may hold every page
-        # tokens, row starts, lengths and page tables of a batch, sent in one piece
-        self._at = np.cumsum([0, R, S + 1, S, S * self.stride])
-        self.batch_words = DeviceBuffer(4 * int(self._at[-1]))
+        # row starts, lengths, tokens and page tables of a batch, sent in one piece (a sequence may hold every page)
+        self.batch_words = DeviceBuffer(4 * (S + 1 + S + R + S * n_pages))
         self.fault = native.zeros(4)
         self.x, self.x2, self.xn = (DeviceBuffer(R * c.hidden * 2) for _ in range(3))
         self.q, self.att = DeviceBuffer(R * c.n_q * 2), DeviceBuffer(R * c.n_q * 2)
@@ -193,21 +191,20 @@ class PagedDecoder:
         R = sum(rows)
         if not 0 < n <= self.max_seqs or R > self.max_rows or min(rows) < 1:
             raise ValueError("a batch has sequences with tokens, no more than max_seqs and max_rows")
+        flat = [t for ts in tokens for t in ts]
+        if min(flat) < 0 or max(flat) >= c.vocab:
+            raise ValueError("a token outside of the vocabulary")
         copies = self.pages.extend(seqs, rows)
         self.copy_pages(copies)
-        words = np.zeros(int(self._at[-1]), np.uint32)
-        words[:R] = [t for ts in tokens for t in ts]
         starts = np.concatenate([[0], np.cumsum(rows)])
-        words[self._at[1]:self._at[1] + n + 1] = starts
-        words[self._at[2]:self._at[2] + n] = [s.length for s in seqs]
-        table = int(self._at[3])
-        words[table:table + n * self.stride] = self.pages.table(seqs, self.stride).ravel()
+        stride = max(len(s.pages) for s in seqs)
+        words = np.concatenate([starts, [s.length for s in seqs], flat, self.pages.table(seqs, stride).ravel()]).astype(np.uint32)
         if st is not None:
             native.sync(st)                                    # (the upload below does not wait for another stream's batch)
-        self.batch_words.upload(words[:table + n * self.stride])
-        at = [self.batch_words.ptr + 4 * int(a) for a in self._at]
-        b = native.PagedBatch(at[1], at[2], at[3], self.stride, n, R, max(rows), max(s.length for s in seqs), self.fault)
-        native.embed_lookup_rows(w.mats["embed_tokens"], at[0], R, c.embed_scale, self.x, st)
+        self.batch_words.upload(words)
+        at = [self.batch_words.ptr + 4 * i for i in (0, n + 1, 2 * n + 1, 2 * n + 1 + R)]
+        b = native.PagedBatch(at[0], at[1], at[3], stride, n, R, max(rows), max(s.length for s in seqs), self.fault)
+        native.embed_lookup_rows(w.mats["embed_tokens"], at[2], R, c.embed_scale, self.x, st)
         scale = float(c.head_dim) ** -0.5
         for l in range(c.n_layers):
             p = f"layers.{l}."

@@ -173,3 +173,21 @@ def test_command(fk, tmp_path):
     beams = json.loads(r.stdout.strip().splitlines()[-1])["beams"]
     assert len(beams) == 3 and all(len(b["tokens"]) == 4 for b in beams)
     assert beams[0]["log_probability"] >= beams[1]["log_probability"] >= beams[2]["log_probability"]
+
+
+@pytest.mark.parametrize("tokens", [[1, 1003], [-1], [2 ** 32]])
+def test_tokens_outside_of_the_vocabulary_change_nothing(fk, models, tokens):
+    cfg, d = paged(models, "norms")
+    s = d.pages.new()
+    with pytest.raises(ValueError):
+        d.forward([(s, tokens)])
+    assert s.length == 0 and d.pages.free_pages == 64
+
+
+def test_a_large_pool_sends_only_the_pages_of_the_batch(fk, models):
+    cfg, d = paged(models, "norms", n_pages=5000)
+    a, b = d.pages.new(), d.pages.new()
+    tokens = rng(8).integers(0, cfg.vocab, 40).tolist()
+    got = d.forward([(a, tokens), (b, tokens[:3])]).to_numpy(np.uint16)[:2 * cfg.vocab].reshape(2, -1)
+    for row, t in zip(got, (tokens, tokens[:3])):
+        assert rel_l2(row, wide(logits_of(models, "norms", t))) <= BAR
