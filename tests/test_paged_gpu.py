@@ -307,3 +307,47 @@ def test_pages_copy(fk, planes, n_pages, page_bytes, pairs, gap):
         v[dst] = v[src]
     assert bool((d.to_numpy(np.uint8) == ref).all())
     fk.pages_copy(d, planes, stride, n_pages, page_bytes, [])
+
+
+def test_pages_beyond_32_bits(fk):
+    """Pages around 4 GB, 2^32 values and at the pool's end: attention of a chunk and of single tokens, the append, copies."""
+    p = Paged([40, 1, 3], [200, 130, 70], 2, 128, 64, seed=30)
+    page_bytes, far = p.k[0].nbytes, 2 ** 33 // p.k[0].nbytes + 40
+    ids = np.concatenate([2 ** 32 // page_bytes + np.arange(-2, 2), 2 ** 33 // page_bytes + np.arange(-2, 2), far - 1 - np.arange(p.n_pages)]).astype(np.uint32)
+    pools = [fk.DeviceBuffer(far * page_bytes) for _ in range(2)]
+    for buf, pages in zip(pools, (p.k, p.v)):
+        for i in range(p.n_pages):
+            buf.upload(pages[i], int(ids[i]) * page_bytes)
+    table = np.where(p.table < p.n_pages, ids[np.minimum(p.table, p.n_pages - 1)], 0xFFFFFFFF).astype(np.uint32)
+    d = [fk.DeviceBuffer.from_numpy(a) for a in (p.row_start, p.kv_len, table)]
+    n, n_heads = sum(p.rows), 8
+    q = normal_bf16(31, (n, n_heads, 128))
+    ref, size = attention(p, q, n_heads, 128 ** -0.5)
+    pool = fk.PagePool(pools[0], pools[1], far, 64, 2, 128)
+    for keep in (slice(0, 3), slice(1, 3)):                   # with the chunk; single tokens and three rows, tiles of 16
+        rows = np.array(p.rows[keep])
+        start = fk.DeviceBuffer.from_numpy(np.concatenate([[0], np.cumsum(rows)]).astype(np.uint32))
+        first, m = sum(p.rows[:keep.start]), int(rows.sum())
+        batch = fk.PagedBatch(start, d[1].ptr + 4 * keep.start, d[2].ptr + 4 * keep.start * p.stride, p.stride, len(rows), m, int(rows.max()), 200, None)
+        out, ws = fk.zeros(m * n_heads * 256), fk.zeros(fk.sdpa_paged_workspace_bytes(n_heads, 2, 128, len(rows), m, 200))
+        fk.sdpa_paged(fk.DeviceBuffer.from_numpy(q[first:first + m]), n_heads * 128, out, n_heads * 128, n_heads, 128 ** -0.5, 0.0, 0, batch, pool, ws, ws.nbytes)
+        fk.sync()
+        got, r, s = wide(out.to_numpy(np.uint16, (m, n_heads, 128))), ref[first:first + m], size[first:first + m]
+        assert bool((np.abs(got - r) <= 2.0 ** -8 * np.abs(r) + (2.0 ** -8 + 2.0 ** -11) * s).all())
+    kv = normal_bf16(32, (n, 2, 128))
+    dk, dq = fk.DeviceBuffer.from_numpy(kv), fk.DeviceBuffer.from_numpy(q)
+    batch = fk.PagedBatch(d[0], d[1], d[2], p.stride, 3, n, 40, 200, None)
+    fk.rope_paged_store(dq, n_heads * 128, dk, 256, dk, 256, dq, n_heads * 128, n_heads, None, None, 1e-6, 0, False, None, batch, pool)
+    at = 0
+    for i, (r, length) in enumerate(zip(p.rows, p.lens)):
+        page, slot = p.where(i, np.arange(length - r, length))
+        p.k[page, :, slot] = p.v[page, :, slot] = kv[at:at + r]
+        at += r
+    near = np.array([[ids[0], 1], [ids[p.n_pages - 1], 2 ** 32 // page_bytes + 5]], np.uint32)
+    for buf, pages in zip(pools, (p.k, p.v)):
+        fk.pages_copy(buf, 1, far * page_bytes, far, page_bytes, near)
+        fk.sync()
+        for i in range(p.n_pages):
+            assert bool((buf.to_numpy(np.uint16, p.k[0].shape, int(ids[i]) * page_bytes) == pages[i]).all())
+        for src, dst in ((0, near[0, 1]), (p.n_pages - 1, near[1, 1])):
+            assert bool((buf.to_numpy(np.uint16, p.k[0].shape, int(dst) * page_bytes) == pages[src]).all())
