@@ -27,6 +27,11 @@ constexpr size_t kBeamCounterBytes = (size_t)4 * kBeamCounterStep * kBeamGroups;
 // values reach and few more; found by bisection over its 16 bits with ballots.  What reaches it is collected in LDS and ranked by counting.
 // Only a piece full of ties has more than fit there: its k largest are then taken one by one.  Logits are compared two at a time as 16-bit
 // integers: with a negative one's magnitude negated, bf16 values are in order (and -0 is 0).
+//
+// 16 x 8 rows of 151851 in 21 us, 1.85 TB/s.  A block waits for its piece (3 us while all ask at once), then for the bound, the list and the counter after
+// one another (another 3); 2432 blocks are one round of 2048 and a fifth of a second, and the last group's merge is 5 us.  4 rows of 32000 in 9 us: 4 to
+// the last arrival, 5 of merge.  Pieces of 4096, 6144, 8192, 10240, 12288 and 16384 tokens take 27, 22, 21, 22, 23 and 37 us of the former; of
+// 8192 instead of 2048 10.3 us of the latter.
 struct BeamArgs {
     const uint16_t* logits;
     size_t row_stride;
@@ -463,7 +468,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
     }
 }
 
-// Pieces of 8192 tokens where that makes two blocks a CU, else of 2048.
+// Pieces of 8192 tokens where that makes two blocks a CU, else of 2048 (measured above).
 static uint32_t beam_piece(uint32_t groups, uint32_t beams, uint32_t vocab) { return (uint64_t)groups * beams * ((vocab + 8191u) / 8192u) >= 512u ? 8192u : 2048u; }
 
 fk_status beam_select_workspace_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k, size_t* bytes) {
@@ -510,7 +515,8 @@ fk_status plan_beam_select(const uint16_t* logits, size_t row_stride, const floa
 // ---- rows of state that follow the beams ----
 // A thread takes one column of a group and N of its output rows: it requests them all before it writes one.  In place N covers all rows (of 16-byte
 // columns up to 16: more would not stay in registers, and go by words); apart, eight rows a thread and a part of the grid for each eight.
-// Bound by the bytes; the two columns that a wave's rows share a line in cost nothing that shows.
+// Bound by the bytes; the two columns that a wave's rows share a line in cost nothing that shows.  64 rows of 2.4 MB in 49 us, 6.3 TB/s read and written (what
+// the last-level cache holds of them counts); 4 rows of 8 KB in 2.6.
 struct ReorderArgs {
     const void* src;
     void* dst;

@@ -205,6 +205,10 @@ __device__ __forceinline__ PagedRange paged_range(const SdpaPagedArgs& a, const 
 // sequence over a contiguous cache (sdpa_prefill.hip: S^T = K Q^T, a lane owns one query; O^T += V^T P^T with the score registers as they lie; V^T
 // through ds_read_b64_tr_b16; probabilities formed between the matrix instructions).  A wave requests 16 rows of K and of V a step, which lie
 // in one page: one page id, loaded two steps ahead into a scalar register.
+// Two chunks of 2048 rows behind some 3000 positions, 32 / 8 heads x 128: 430 us, 1000 TFLOP/s (a large bf16 product of the vendor's library reaches 1150 to 1380
+// on the same card).  The matrix unit works in 42 % of the cycles, the vector unit about as long.  What holds the rate is the card's power as much as that:
+// tiles of 256 columns with the softmax of one step between the products of another took a fifth fewer cycles at a clock a fifth lower (1.94 -> 1.54 GHz),
+// 428 us for 439, and lost a third where tiles are few; tiles of 64 columns, two waves sharing 32 columns' positions, lost 15 % on a chunk of 512 rows behind 3000.
 constexpr uint32_t tile_lds_bytes(uint32_t d) {
     const uint32_t stage = 2u * 2u * kTileStep * d * 2u, outb = kTileCols * (d + 4u) * 4u;
     return stage > outb ? stage : outb;
@@ -389,9 +393,7 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
             const float p0 = __builtin_amdgcn_exp2f(fmaf(s[at / 16][at % 16], scale2, -m_sub));
             const float p1 = __builtin_amdgcn_exp2f(fmaf(s[at / 16][at % 16 + 1], scale2, -m_sub));
             l_run += p0 + p1;
-            uint32_t both = pack_bf16(p0, p1);
-            asm volatile("" : "+v"(both), "+v"(l_run));   // (made here: the compiler would gather them in one place)
-            pb[c()][w()] = both;
+            pb[c()][w()] = pack_bf16(p0, p1);
         };
         static_for<4>([&](auto w) __attribute__((always_inline)) { probabilities(std::integral_constant<int, 0>{}, w); });
         __builtin_amdgcn_sched_barrier(0);
@@ -571,7 +573,8 @@ __global__ __launch_bounds__(256) void sdpa_paged_merge_kernel(const SdpaPagedAr
 // columns), a probability as the sum of two bf16 values, hi + lo, which leaves 2^-17 of it: of up to 8 columns in the columns 8 on, of more in an
 // instruction of its own.  A wave owns its steps of 32 positions and their place in LDS: it waits for no other wave until the block's waves
 // meet, its keys are requested again as soon as they are in registers, its values behind the second product.  Two blocks a CU keep 128 KB in
-// flight.  Bound by the bytes.
+// flight.  Bound by the bytes: 64 tokens over 620 MB of keys and values 119 us, 5.2 TB/s (a copy on the card reaches 4.75 read and written).  One token
+// over 613 positions, 14 / 2 heads x 64: 7 us, which is what finding the item, one round and the merge take after one another.
 constexpr uint32_t few_lds_bytes(uint32_t d) {
     const uint32_t stages = 4u * kFewStep * d * 4u, meet = 4u * kFewCols * (d + 4u) * 4u + 2u * 4u * kFewCols * 4u;
     return (stages > meet ? stages : meet) + 16u;   // and two words for the block
