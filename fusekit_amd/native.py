@@ -695,10 +695,10 @@ def paged_check(fault, stream=None) -> None:
 
 def pages_copy(base, n_planes, plane_stride, n_pages, page_bytes, pairs, stream=None) -> None:
     """Page pairs[i][0] to page pairs[i][1] in every plane of a pool (fk_pages_copy); pairs: host numbers [n, 2]."""
-    p = pairs if pairs.__class__ is np.ndarray and pairs.dtype == np.uint32 and pairs.flags.c_contiguous else _page_pairs(pairs)
+    p = pairs if pairs.__class__ is np.ndarray and pairs.dtype == np.uint32 else _page_pairs(pairs)
     if p.ndim != 2 or p.shape[1] != 2:
         raise InvalidArgument(FK_ERR_INVALID, "pages_copy: pairs must be [n, 2]")
-    check(lib.fk_pages_copy(_addr(base), n_planes, plane_stride, n_pages, page_bytes, p.ctypes.data, p.shape[0], _addr(stream)))
+    check(lib.fk_pages_copy(_addr(base), n_planes, plane_stride, n_pages, page_bytes, p.tobytes(), p.shape[0], _addr(stream)))   # (bytes: an array's address costs 1 us)
 
 
 def _page_pairs(pairs) -> np.ndarray:
@@ -707,7 +707,7 @@ def _page_pairs(pairs) -> np.ndarray:
         return np.zeros((0, 2), np.uint32)
     if p.dtype.kind not in "iu" or p.min() < 0 or p.max() > 0xFFFFFFFF:
         raise InvalidArgument(FK_ERR_INVALID, "pages_copy: pairs must be page ids")
-    return np.ascontiguousarray(p, dtype=np.uint32)
+    return p.astype(np.uint32)
 
 
 def beam_select_workspace_bytes(groups, beams, vocab, k) -> int:
