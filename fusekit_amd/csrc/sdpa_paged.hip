@@ -97,18 +97,18 @@ struct PagedItem {
     bool any;
 };
 // FEW: a launch of single tokens only.  TILES: `index` counts tiles, not items.
-template <bool FEW, bool TILES = false>
+template <bool FEW, uint32_t COLS, bool TILES = false>
 __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t index, uint32_t lane) {
     constexpr uint32_t STEP = FEW ? kFewRound : kTileStep;
     const uint32_t n_kv = a.b.n_kv;
     auto tiles_of = [&](const PagedSeq& s) {   // (rows times heads of a group: below 2^31, the host has checked)
-        const uint32_t columns = s.rows * a.group, width = FEW || columns <= kFewMost ? kFewCols : kTileCols;
+        const uint32_t columns = s.rows * a.group, width = columns <= kFewMost ? kFewCols : COLS;
         return (columns + width - 1u) / width;
     };
     auto steps_of = [&](const PagedSeq& s) {   // of a tile of the sequence, at most
         uint32_t seen = s.len;
         if (a.window) {
-            const uint32_t span = (FEW ? kFewCols : kTileCols) / a.group + 2u;   // rows of a tile, at most
+            const uint32_t span = COLS / a.group + 2u;   // rows of a tile, at most
             const uint64_t w = (uint64_t)a.window + (s.rows < span ? s.rows : span) + STEP - 1u;
             seen = w < seen ? (uint32_t)w : seen;
         }
@@ -200,42 +200,87 @@ __device__ __forceinline__ PagedRange paged_range(const SdpaPagedArgs& a, const 
     return r;
 }
 
+// What a wave hands on of 32 columns, `live` of them, et the first: outputs, or where the tile is cut the sums as they are, the reference and the sum of the
+// probabilities into this item's slot (`c0`: the first column's place there).  ob: [32][D + 4] in LDS, outputs or sums.
+template <int D>
+__device__ __forceinline__ void paged_hand_on(const SdpaPagedArgs& a, const PagedItem& it, const float* ob, uint32_t et, uint32_t c0, uint32_t live, bool whole, float m,
+                                              float l, uint32_t lane) {
+    constexpr uint32_t OS = D + 4, VP = D / 8;
+    const uint32_t G = a.group;
+    if (!whole) {
+        const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials + (size_t)blockIdx.x * (kTileCols * (D + 2u)), 0, (int)(kTileCols * (D + 2u) * 4u), 0x27000);
+        for (uint32_t idx = lane; idx < live * (uint32_t)(D / 4); idx += 64u) {
+            const uint32_t col = idx / (uint32_t)(D / 4), pc = idx % (uint32_t)(D / 4);
+            const pf_u32x4_t v = *reinterpret_cast<const pf_u32x4_t*>(ob + col * OS + pc * 4u);
+            __builtin_amdgcn_raw_buffer_store_b128(v, mem, (int)(((c0 + col) * D + pc * 4u) * 4u), 0, 0);
+        }
+        if (lane < live) {   // (the lanes below 32 hold all of a column's l)
+            const pf_u32x2_t ml = {__float_as_uint(m), __float_as_uint(l)};
+            __builtin_amdgcn_raw_buffer_store_b64(ml, mem, (int)((kTileCols * D + (c0 + lane) * 2u) * 4u), 0, 0);
+        }
+        return;
+    }
+    uint32_t again = 0;   // columns whose sums are not finite, done again one by one
+    for (uint32_t base = 0; base < live * VP; base += 64u) {
+        const uint32_t idx = base + lane, col = idx / VP, pc = idx % VP;
+        const bool in = col < live;
+        const float4 lo = *reinterpret_cast<const float4*>(ob + (in ? col : 0u) * OS + pc * 8u);
+        const float4 hi = *reinterpret_cast<const float4*>(ob + (in ? col : 0u) * OS + pc * 8u + 4u);
+        const uint32_t ec = et + col, pl = ec / G;
+        if (in)
+            *reinterpret_cast<uint4*>(a.out + (size_t)(it.s.row0 + pl) * a.out_stride + (size_t)(it.kvh * G + (ec - pl * G)) * D + pc * 8u) =
+                make_uint4(pack_bf16(lo.x, lo.y), pack_bf16(lo.z, lo.w), pack_bf16(hi.x, hi.y), pack_bf16(hi.z, hi.w));
+        const float t = (__builtin_fabsf(lo.x) + __builtin_fabsf(lo.y)) + (__builtin_fabsf(lo.z) + __builtin_fabsf(lo.w)) +
+                        (__builtin_fabsf(hi.x) + __builtin_fabsf(hi.y)) + (__builtin_fabsf(hi.z) + __builtin_fabsf(hi.w));
+        unsigned long long odd = __builtin_amdgcn_ballot_w64(in && !(t < INFINITY));
+        for (; odd; odd &= odd - 1u) again |= 1u << ((base + (uint32_t)__builtin_ctzll(odd)) / VP);
+    }
+    for (; again; again &= again - 1u) {
+        const uint32_t ec = et + (uint32_t)__builtin_ctz(again), pl = ec / G;
+        paged_row<D>(a, it.seq, it.s, pl, it.kvh * G + (ec - pl * G), lane);
+    }
+}
+
 // ---- tiles of 128 columns ----
-// A block is four waves of 32 columns on the same 64 positions a step.  The products and the softmax are those of the causal attention of one
+// A block is four waves of 32 columns on the same 64 positions a step (SPLIT 1).  The products and the softmax are those of the causal attention of one
 // sequence over a contiguous cache (sdpa_prefill.hip: S^T = K Q^T, a lane owns one query; O^T += V^T P^T with the score registers as they lie; V^T
-// through ds_read_b64_tr_b16; probabilities formed between the matrix instructions).  A wave requests 16 rows of K and of V a step, which lie
-// in one page: one page id, loaded two steps ahead into a scalar register.
+// through ds_read_b64_tr_b16; probabilities formed between the matrix instructions).  A wave requests 16 rows of K and of V a step (SPLIT
+// times), which lie in one page: one page id, loaded two steps ahead into a scalar register.
 // Two chunks of 2048 rows behind some 3000 positions, 32 / 8 heads x 128: 430 us, 1000 TFLOP/s (a large bf16 product of the vendor's library reaches 1150 to 1380
-// on the same card).  The matrix unit works in 42 % of the cycles, the vector unit about as long.  What holds the rate is the card's power as much as that:
+// on the same card).  The matrix unit works in half of the cycles, the vector unit as long.  What holds the rate is the card's power as much as that:
 // tiles of 256 columns with the softmax of one step between the products of another took a fifth fewer cycles at a clock a fifth lower (1.94 -> 1.54 GHz),
-// 428 us for 439, and lost a third where tiles are few; tiles of 64 columns, two waves sharing 32 columns' positions, lost 15 % on a chunk of 512 rows behind 3000.
-constexpr uint32_t tile_lds_bytes(uint32_t d) {
-    const uint32_t stage = 2u * 2u * kTileStep * d * 2u, outb = kTileCols * (d + 4u) * 4u;
+// 428 us for 439, and lost a third where tiles are few.
+// SPLIT 2: tiles of 64 columns and 128 positions a step, for launches that leave CUs to themselves; two waves share 32 columns, 64 positions a step each,
+// and join at the end (the planner has the rule and its figures).
+constexpr uint32_t tile_lds_bytes(uint32_t d, uint32_t split) {
+    const uint32_t stage = split * 2u * 2u * kTileStep * d * 2u, outb = 4u * 32u * (d + 4u + 2u) * 4u;
     return stage > outb ? stage : outb;
 }
 
-template <int D, bool CAP>
+template <int D, bool CAP, uint32_t SPLIT>
 __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedItem& it, uint32_t lane) {
     constexpr int KB = D / 16, DT = D / 32, VP = D / 8;
-    constexpr uint32_t ROW = D * 2u, TILE = kTileStep * ROW, STAGE = 2u * TILE;      // bytes: a row, K (or V) of a step, both
+    constexpr uint32_t COLS = kTileCols / SPLIT, STEP = kTileStep * SPLIT;           // of a block: columns, positions a step
+    constexpr uint32_t ROW = D * 2u, TILE = STEP * ROW, STAGE = 2u * TILE;           // bytes: a row, K (or V) of a step, both
     constexpr uint32_t RPI = 1024u / ROW;                                            // rows of one wave's request
-    constexpr int REQ = 16 / (int)RPI;                                               // requests of a wave, matrix and step
+    constexpr int REQ = 16 / (int)RPI;                                               // requests of 16 rows of a matrix
     extern __shared__ uint4 lds_raw[];
     unsigned char* const lds = reinterpret_cast<unsigned char*>(lds_raw);
 
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kb = lane >> 5, nl = lane & 31u;
     const uint32_t G = a.group, columns = it.s.rows * G;   // (below 2^31: the host has checked)
+    const uint32_t column_tile = SPLIT == 1 ? wave : wave & 1u, my_half = SPLIT == 1 ? 0u : wave >> 1;
     auto limit_of = [&](uint32_t place) { return it.s.len + place + 1u > it.s.rows ? it.s.len + place + 1u - it.s.rows : 0u; };   // positions a row may see end here
     auto low_of = [&](uint32_t limit) { return a.window && limit > a.window ? limit - a.window : 0u; };                           // and begin here
-    const uint32_t e_tile = it.tile * kTileCols, e_last = columns - e_tile < kTileCols ? columns - 1u : e_tile + kTileCols - 1u;
-    const PagedRange range = paged_range<kTileStep>(a, it, e_tile, e_last);
+    const uint32_t e_tile = it.tile * COLS, e_last = columns - e_tile < COLS ? columns - 1u : e_tile + COLS - 1u;
+    const PagedRange range = paged_range<STEP>(a, it, e_tile, e_last);
     const uint32_t kv_end = range.kv_end, n_active = range.n_active;
     if (it.split >= n_active) return;
     const uint32_t begin = __builtin_amdgcn_readfirstlane(range.step0 + it.split * range.per);
     const uint32_t stop = __builtin_amdgcn_readfirstlane(it.split + 1u == n_active ? range.step0 + range.steps : begin + range.per);
 
     // this lane's column; a wave's columns past the last repeat it, and a wave without columns does the last one's loads and nothing else
-    const uint32_t e0 = e_tile + wave * 32u;
+    const uint32_t e0 = e_tile + column_tile * 32u;
     const uint32_t live = e0 <= e_last ? (e_last - e0 < 31u ? e_last - e0 + 1u : 32u) : 0u;
     const uint32_t e = live ? e0 + (nl < live ? nl : live - 1u) : e_last;
     const uint32_t place = e / G, head = it.kvh * G + (e - place * G);
@@ -257,25 +302,37 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
     typedef const uint32_t __attribute__((address_space(4)))* scalar_ptr;
     const uintptr_t table = (uintptr_t)(a.b.table + (size_t)__builtin_amdgcn_readfirstlane(it.seq) * a.b.table_stride);
     uint32_t bad = 0;
-    auto span_of = [&](uint32_t step) { return step * kTileStep + wave * 16u; };   // the first of this wave's 16 rows of a step
-    auto page_of = [&](uint32_t step) {                                             // (past the range: the last position's)
-        const uint32_t span = span_of(step), at = span < kv_end ? span : kv_end - 1u;
-        return *(scalar_ptr)(table + (size_t)(at >> shift) * 4u);
+    struct Pages {
+        uint32_t id[SPLIT];
     };
-    auto issue = [&](uint32_t step, uint32_t page, uint32_t stage) {
-        if (page >= a.b.n_pages) {
-            page = 0;
-            bad = FK_PAGED_BAD_PAGE;
-        }
-        const uint32_t span = span_of(step), at = span < kv_end ? span : kv_end - 1u, left = kv_end - 1u - at;
-        const size_t off = (((size_t)page * a.b.n_kv + it.kvh) * (in_page + 1u) + (at & in_page)) * ROW;
-        const unsigned char *ks = reinterpret_cast<const unsigned char*>(a.k) + off, *vs = reinterpret_cast<const unsigned char*>(a.v) + off;
+    auto span_of = [&](uint32_t step, uint32_t g) { return step * STEP + (wave * SPLIT + g) * 16u; };   // the first of 16 rows of a step that this wave requests
+    auto pages_of = [&](uint32_t step) {                                                                 // (past the range: the last position's)
+        Pages p;
 #pragma unroll
-        for (int i = 0; i < REQ; ++i) {
-            const uint32_t r = (uint32_t)i * RPI + irow, row = wave * 16u + r, from = r < left ? r : left;   // (past the range: masked scores, zero probabilities)
-            const uint32_t to = stage * STAGE + (wave * (uint32_t)REQ + (uint32_t)i) * 1024u;
-            dma16(to, from * ROW + ((at_piece ^ k_swizzle(row)) * 16u), ks);
-            dma16(to + TILE, from * ROW + ((at_piece ^ v_swizzle(row)) * 16u), vs);
+        for (uint32_t g = 0; g < SPLIT; ++g) {
+            const uint32_t span = span_of(step, g), at = span < kv_end ? span : kv_end - 1u;
+            p.id[g] = *(scalar_ptr)(table + (size_t)(at >> shift) * 4u);
+        }
+        return p;
+    };
+    auto issue = [&](uint32_t step, const Pages& pages, uint32_t stage) {
+#pragma unroll
+        for (uint32_t g = 0; g < SPLIT; ++g) {
+            uint32_t page = pages.id[g];
+            if (page >= a.b.n_pages) {
+                page = 0;
+                bad = FK_PAGED_BAD_PAGE;
+            }
+            const uint32_t span = span_of(step, g), at = span < kv_end ? span : kv_end - 1u, left = kv_end - 1u - at;
+            const size_t off = (((size_t)page * a.b.n_kv + it.kvh) * (in_page + 1u) + (at & in_page)) * ROW;
+            const unsigned char *ks = reinterpret_cast<const unsigned char*>(a.k) + off, *vs = reinterpret_cast<const unsigned char*>(a.v) + off;
+#pragma unroll
+            for (int i = 0; i < REQ; ++i) {
+                const uint32_t r = (uint32_t)i * RPI + irow, from = r < left ? r : left;   // (past the range: masked scores, zero probabilities; a swizzle repeats every 16 rows)
+                const uint32_t to = stage * STAGE + ((wave * SPLIT + g) * (uint32_t)REQ + (uint32_t)i) * 1024u;
+                dma16(to, from * ROW + ((at_piece ^ k_swizzle(r)) * 16u), ks);
+                dma16(to + TILE, from * ROW + ((at_piece ^ v_swizzle(r)) * 16u), vs);
+            }
         }
     };
 
@@ -298,11 +355,11 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
     const float scale2 = CAP ? 1.0f : a.scale * kLog2E;                              // scores to exponents of two
     const float cap2 = a.softcap * kLog2E, turn2 = CAP ? 2.0f * a.scale * kLog2E / a.softcap : 0.f;
 
-    uint32_t page_next = 0;
+    Pages next = {};
     if (begin < stop) {
-        const uint32_t page = page_of(begin);
-        if (begin + 1u < stop) page_next = page_of(begin + 1u);
-        issue(begin, page, 0);
+        const Pages first = pages_of(begin);
+        if (begin + 1u < stop) next = pages_of(begin + 1u);
+        issue(begin, first, 0);
     }
     uint32_t stage = 0;
 #pragma unroll 1
@@ -310,12 +367,12 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
         wait_loads<0>();
         barrier();   // this step's rows are everybody's; the other stage has been read
         if (step + 1u < stop) {
-            issue(step + 1u, page_next, stage ^ 1u);
-            if (step + 2u < stop) page_next = page_of(step + 2u);
+            issue(step + 1u, next, stage ^ 1u);
+            if (step + 2u < stop) next = pages_of(step + 2u);
         }
-        const uint32_t kv0 = step * kTileStep;
+        const uint32_t kv0 = step * STEP + my_half * kTileStep;            // this wave's 64 positions
         if (kv0 >= last_limit || kv0 + kTileStep <= first_low) continue;   // nothing that a row of this wave sees
-        const unsigned char *ks = lds + stage * STAGE, *vs = ks + TILE;
+        const unsigned char *ks = lds + stage * STAGE + my_half * kTileStep * ROW, *vs = ks + TILE;
         // (two of the eight pairs of fragments ahead of their matrix instructions; all of them first took 1 % longer of two chunks of 2048 rows, 2 % with a window)
         pf_u32x4_t kf[3][2];
         auto read_k = [&](auto j) __attribute__((always_inline)) {
@@ -422,47 +479,48 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
     // ---- what the tile hands on: through this wave's own LDS rows, so that the stores are whole 16-byte pieces ----
     l_run = both_halves_sum(l_run);
     constexpr uint32_t OS = D + 4;
-    float* const ob = reinterpret_cast<float*>(lds_raw) + wave * 32u * OS;
+    float* const all = reinterpret_cast<float*>(lds_raw);
+    float* const ob = all + wave * 32u * OS;
     const bool whole = n_active == 1u;
-    const float f = whole ? (l_run > 0.f || l_run != l_run ? 1.0f / l_run : 0.f) : 1.0f;   // (a row that sees nothing: zeros)
+    const float f = whole && SPLIT == 1 ? (l_run > 0.f || l_run != l_run ? 1.0f / l_run : 0.f) : 1.0f;   // (a row that sees nothing: zeros)
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
             *reinterpret_cast<float4*>(ob + nl * OS + (uint32_t)(i * 32 + 8 * g) + 4u * kb) =
                 make_float4(oacc[i][4 * g + 0] * f, oacc[i][4 * g + 1] * f, oacc[i][4 * g + 2] * f, oacc[i][4 * g + 3] * f);
-    wave_lds_order();
-    if (!whole) {   // the item's part, for paged_merge
-        const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials + (size_t)blockIdx.x * (kTileCols * (D + 2u)), 0, (int)(kTileCols * (D + 2u) * 4u), 0x27000);
-        for (uint32_t idx = lane; idx < live * (uint32_t)(D / 4); idx += 64u) {
-            const uint32_t col = idx / (uint32_t)(D / 4), pc = idx % (uint32_t)(D / 4);
-            const pf_u32x4_t v = *reinterpret_cast<const pf_u32x4_t*>(ob + col * OS + pc * 4u);
-            __builtin_amdgcn_raw_buffer_store_b128(v, mem, (int)(((wave * 32u + col) * D + pc * 4u) * 4u), 0, 0);
+    if constexpr (SPLIT == 1) {
+        wave_lds_order();
+        paged_hand_on<D>(a, it, ob, e0, wave * 32u, live, whole, m_run, l_run, lane);
+    } else {   // the two waves of a column tile join their halves, 16 columns each
+        float* const ml = all + 4u * 32u * OS;   // [wave][column] reference, sum
+        if (kb == 0) *reinterpret_cast<float2*>(ml + (wave * 32u + nl) * 2u) = make_float2(m_run, l_run);
+        __syncthreads();
+        const uint32_t c0 = my_half * 16u, mine = live > c0 ? (live - c0 < 16u ? live - c0 : 16u) : 0u;
+        const float* const other = all + (wave ^ 2u) * 32u * OS;
+        auto join = [&](uint32_t c, float& w0, float& w1, float& m, float& l) {
+            const float2 x = *reinterpret_cast<const float2*>(ml + (wave * 32u + c) * 2u), y = *reinterpret_cast<const float2*>(ml + ((wave ^ 2u) * 32u + c) * 2u);
+            m = fmaxf(x.x, y.x);
+            const float ref = m == -INFINITY ? 0.f : m;
+            w0 = __builtin_amdgcn_exp2f(x.x - ref);
+            w1 = __builtin_amdgcn_exp2f(y.x - ref);
+            l = fmaf(x.y, w0, y.y * w1);
+        };
+        float w0, w1, m, l;
+        for (uint32_t idx = lane; idx < 16u * (D / 4u); idx += 64u) {
+            const uint32_t c = c0 + idx / (D / 4u), d = idx % (D / 4u) * 4u;
+            join(c, w0, w1, m, l);
+            if (whole) {
+                const float r = l > 0.f || l != l ? 1.0f / l : 0.f;
+                w0 *= r;
+                w1 *= r;
+            }
+            const float4 x = *reinterpret_cast<const float4*>(ob + c * OS + d), y = *reinterpret_cast<const float4*>(other + c * OS + d);
+            *reinterpret_cast<float4*>(ob + c * OS + d) = make_float4(fmaf(x.x, w0, y.x * w1), fmaf(x.y, w0, y.y * w1), fmaf(x.z, w0, y.z * w1), fmaf(x.w, w0, y.w * w1));
         }
-        if (kb == 0 && nl < live) {
-            const pf_u32x2_t ml = {__float_as_uint(m_run), __float_as_uint(l_run)};
-            __builtin_amdgcn_raw_buffer_store_b64(ml, mem, (int)((kTileCols * D + (wave * 32u + nl) * 2u) * 4u), 0, 0);
-        }
-        return;
-    }
-    unsigned long long again = 0;   // columns of this wave whose sums are not finite, done again one by one
-    for (uint32_t base = 0; base < live * (uint32_t)VP; base += 64u) {
-        const uint32_t idx = base + lane, col = idx / (uint32_t)VP, pc = idx % (uint32_t)VP;
-        const bool in = col < live;
-        const float4 lo = *reinterpret_cast<const float4*>(ob + (in ? col : 0u) * OS + pc * 8u);
-        const float4 hi = *reinterpret_cast<const float4*>(ob + (in ? col : 0u) * OS + pc * 8u + 4u);
-        const uint32_t ec = e0 + col, pl = ec / G;
-        if (in)
-            *reinterpret_cast<uint4*>(a.out + (size_t)(it.s.row0 + pl) * a.out_stride + (size_t)(it.kvh * G + (ec - pl * G)) * D + pc * 8u) =
-                make_uint4(pack_bf16(lo.x, lo.y), pack_bf16(lo.z, lo.w), pack_bf16(hi.x, hi.y), pack_bf16(hi.z, hi.w));
-        const float t = (__builtin_fabsf(lo.x) + __builtin_fabsf(lo.y)) + (__builtin_fabsf(lo.z) + __builtin_fabsf(lo.w)) +
-                        (__builtin_fabsf(hi.x) + __builtin_fabsf(hi.y)) + (__builtin_fabsf(hi.z) + __builtin_fabsf(hi.w));
-        unsigned long long odd = __builtin_amdgcn_ballot_w64(in && !(t < INFINITY));
-        for (; odd; odd &= odd - 1u) again |= 1ull << ((base + (uint32_t)__builtin_ctzll(odd)) / (uint32_t)VP);
-    }
-    for (; again; again &= again - 1u) {
-        const uint32_t ec = e0 + (uint32_t)__builtin_ctzll(again), pl = ec / G;
-        paged_row<D>(a, it.seq, it.s, pl, it.kvh * G + (ec - pl * G), lane);
+        join(c0 + (lane & 15u), w0, w1, m, l);
+        wave_lds_order();
+        paged_hand_on<D>(a, it, ob + c0 * OS, e0 + c0, column_tile * 32u + c0, mine, whole, m, l, lane);
     }
 }
 
@@ -539,7 +597,7 @@ constexpr uint32_t kMergeCols = 16;
 template <int D>
 __global__ __launch_bounds__(256) void sdpa_paged_merge_kernel(const SdpaPagedArgs a) {
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const PagedItem it = paged_item<false, true>(a, blockIdx.x / (kTileCols / kMergeCols), lane);
+    const PagedItem it = paged_item<false, kTileCols, true>(a, blockIdx.x / (kTileCols / kMergeCols), lane);
     if (!it.any) return;
     const uint32_t G = a.group, columns = it.s.rows * G, e_tile = it.tile * kTileCols, c0 = blockIdx.x % (kTileCols / kMergeCols) * kMergeCols;
     if (columns <= kFewMost || e_tile + c0 >= columns) return;
@@ -854,18 +912,18 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
 
 // Chunks and single tokens together: each sequence by its kind, in one launch, so that what is bound by the matrix units runs beside what is bound by the
 // bytes.
-template <int D, bool CAP>
+template <int D, bool CAP, uint32_t SPLIT>
 __global__ __launch_bounds__(256, 2) void sdpa_paged_kernel(const SdpaPagedArgs a) {
     const uint32_t lane = threadIdx.x & 63u;
-    const PagedItem it = paged_item<false>(a, blockIdx.x, lane);
+    const PagedItem it = paged_item<false, kTileCols / SPLIT>(a, blockIdx.x, lane);
     if (!it.any) return;
     if (it.s.rows * a.group <= kFewMost) paged_few<D, CAP, true, kTileCols>(a, it, lane);
-    else paged_tile<D, CAP>(a, it, lane);
+    else paged_tile<D, CAP, SPLIT>(a, it, lane);
 }
 template <int D, bool CAP, bool WIDE>
 __global__ __launch_bounds__(256, 2) void sdpa_paged_few_kernel(const SdpaPagedArgs a) {
     const uint32_t lane = threadIdx.x & 63u;
-    const PagedItem it = paged_item<true>(a, blockIdx.x, lane);
+    const PagedItem it = paged_item<true, kFewCols>(a, blockIdx.x, lane);
     if (it.any) paged_few<D, CAP, WIDE, kFewCols>(a, it, lane);
 }
 
@@ -943,25 +1001,35 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     a.counters = static_cast<uint32_t*>(workspace);
     a.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kPagedCounterBytes);
     a.slots = p.slots; a.target = p.target; a.min_steps = p.min_steps;
-    const void* tile[2][2] = {{reinterpret_cast<const void*>(&sdpa_paged_kernel<64, false>), reinterpret_cast<const void*>(&sdpa_paged_kernel<64, true>)},
-                              {reinterpret_cast<const void*>(&sdpa_paged_kernel<128, false>), reinterpret_cast<const void*>(&sdpa_paged_kernel<128, true>)}};
+    const void* tile[2][2][2] = {
+        {{reinterpret_cast<const void*>(&sdpa_paged_kernel<64, false, 1>), reinterpret_cast<const void*>(&sdpa_paged_kernel<64, false, 2>)},
+         {reinterpret_cast<const void*>(&sdpa_paged_kernel<64, true, 1>), reinterpret_cast<const void*>(&sdpa_paged_kernel<64, true, 2>)}},
+        {{reinterpret_cast<const void*>(&sdpa_paged_kernel<128, false, 1>), reinterpret_cast<const void*>(&sdpa_paged_kernel<128, false, 2>)},
+         {reinterpret_cast<const void*>(&sdpa_paged_kernel<128, true, 1>), reinterpret_cast<const void*>(&sdpa_paged_kernel<128, true, 2>)}}};
     const void* few[2][2][2] = {
         {{reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, false, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, false, true>)},
          {reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, true, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, true, true>)}},
         {{reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, true>)},
          {reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, true>)}}};
-    l->func = p.few ? few[D == 128][softcap > 0.f][batch->max_rows * (n_heads / n_kv) > 8u] : tile[D == 128][softcap > 0.f];
     // Positions that a tile can see, in steps.  Chunks of up to 8 steps are not cut: the merge costs what it saves (a prompt of 512 rows, 32 / 8 heads x
     // 128: 18 us whole, 24 in halves).
     const uint32_t step = p.few ? kFewRound : kTileStep, span = (p.few ? kFewCols : kTileCols) / a.group + 2u;
     const uint64_t seen = window ? std::min<uint64_t>(batch->max_len, (uint64_t)window + std::min(batch->max_rows, span) + step) : batch->max_len;
     const uint32_t most = (uint32_t)((seen + step - 1u) / step), splits = (most + p.min_steps - 1u) / p.min_steps;
-    const bool cut = p.slots && (p.few ? splits > 1u : most > 8u);
+    // Tiles of 64 columns and twice the positions a step where each has a CU to itself: a lone block's step takes 1.3 to 1.5 us, most of it waits that do not
+    // depend on what it holds, and half as many are left.  32 / 8 heads x 128, us in whole or cut tiles of 128 and in these: a fresh prompt of 512 rows 17.2,
+    // 14.5; of 256 11.6, 11.0; of 200 10.7, 11.0; 512 rows behind 1000 positions 31.8, 28.2; behind 1300 33.7, 32.1; behind 3000 45.8, 54; 384 behind 1100 27.7,
+    // 26.3; 256 behind 1000 24.0, 23.7; 128 behind 512 19.8, 15.7; behind 1000 21.2, 21.4; 64 behind 512 18.0, 15.4; behind 1000 19.1, 21.4.
+    // (at most so many tiles: a sequence of few columns has two, of more one beyond what all together fill)
+    const uint64_t filled = ((uint64_t)batch->rows * a.group + kTileCols / 2 - 1) / (kTileCols / 2), halves = (std::max<uint64_t>(filled, 2) + 2 * (uint64_t)(batch->n_seqs - 1)) * n_kv;
+    const bool split = !p.few && halves <= (uint64_t)dev->cus && most > 4u && most <= 12u + halves / 12u;
+    const bool cut = !split && p.slots && (p.few ? splits > 1u : most > 8u);
     if (!cut) a.slots = 0;
+    l->func = p.few ? few[D == 128][softcap > 0.f][batch->max_rows * (n_heads / n_kv) > 8u] : tile[D == 128][softcap > 0.f][split];
     // (no more blocks than there can be items: one that finds none costs what it takes to look)
-    l->grid = dim3((uint32_t)(cut ? std::min<uint64_t>(p.slots, p.tiles * splits) : p.tiles), 1, 1);
+    l->grid = dim3((uint32_t)(cut ? std::min<uint64_t>(p.slots, p.tiles * splits) : split ? halves : p.tiles), 1, 1);
     l->block = dim3(256, 1, 1);
-    l->shmem = p.few ? few_lds_bytes(D) : std::max(tile_lds_bytes(D), few_lds_bytes(D));
+    l->shmem = p.few ? few_lds_bytes(D) : std::max(tile_lds_bytes(D, split ? 2u : 1u), few_lds_bytes(D));
     if ((int)l->shmem > dev->max_dyn_lds) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: LDS tile does not fit");
     FK_TRY(raise_dynamic_lds(l->func, l->shmem));
     l->set_args(a);

@@ -351,3 +351,50 @@ def test_pages_beyond_32_bits(fk):
             assert bool((buf.to_numpy(np.uint16, p.k[0].shape, int(ids[i]) * page_bytes) == pages[i]).all())
         for src, dst in ((0, near[0, 1]), (p.n_pages - 1, near[1, 1])):
             assert bool((buf.to_numpy(np.uint16, p.k[0].shape, int(dst) * page_bytes) == pages[src]).all())
+
+
+# ---------------------------------------------------------------- a few hundred positions and few tiles: 64 columns, 128 positions a step
+
+@pytest.mark.parametrize("rows,lens", [([130], [300]), ([40], [700]), ([200, 1], [500, 700]), ([70, 33, 0, 2], [330, 400, 9, 77]), ([65], [321]), ([8], [300]), ([8, 8], [300, 290])])
+@pytest.mark.parametrize("n_heads,n_kv,dim,page_rows", [(8, 2, 128, 16), (14, 2, 64, 32), (6, 6, 64, 128), (8, 2, 128, 256)])
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (300, 0.0), (0, 20.0), (310, 30.0)])
+def test_few_tiles(fk, rows, lens, n_heads, n_kv, dim, page_rows, window, softcap):
+    p = Paged(rows, lens, n_kv, dim, page_rows, seed=40 + len(rows))
+    check_attention(fk, p, n_heads, softcap=softcap, window=window, rows=max(sum(rows), 40), max_rows=max(rows + [36]))
+
+
+@pytest.mark.parametrize("edge", [256, 257, 383, 384, 385, 448, 511, 512, 513])
+def test_few_tiles_at_the_edges_of_a_step(fk, edge):
+    for rows in (1, 33, edge if edge < 400 else 100):
+        check_attention(fk, Paged([max(rows, 17)], [edge], 1, 128, 32, seed=edge, spare_table=20), 4, max_len=700)
+
+
+@pytest.mark.parametrize("dim,page_rows", [(64, 16), (128, 64)])
+def test_infinities_and_nan_in_masked_places_of_few_tiles(fk, dim, page_rows):
+    for bad_bits in (0x7F80, 0xFF80, 0x7FC0):
+        p = Paged([50, 1], [400, 600], 2, dim, page_rows, seed=41)
+        for i, at in ((0, np.arange(395, 400)), (1, np.arange(0, 270))):      # the chunk's last five rows; before the window of the other
+            page, slot = p.where(i, at)
+            p.k[page, :, slot] = bad_bits
+            p.v[page, :, slot] = bad_bits
+        q, got, _ = attend(fk, p, 8, window=320)
+        with np.errstate(all="ignore"):
+            ref, size = attention(p, q, 8, dim ** -0.5, 0.0, 320)
+        fine = np.r_[0:45, 50]
+        off = np.abs(wide(got[fine]) - ref[fine]) - (2.0 ** -8 * np.abs(ref[fine]) + (2.0 ** -8 + 2.0 ** -11) * size[fine])
+        assert np.isfinite(wide(got[fine])).all() and off.max() <= 0, hex(bad_bits)
+        if bad_bits == 0x7FC0:
+            assert np.isnan(wide(got[45:50])).all()
+
+
+def test_few_tiles_bad_page(fk):
+    fault = fk.zeros(4)
+    p = Paged([60, 50], [300, 310], 2, 128, 16, seed=42)
+    p.table[0, 9] = p.n_pages + 3
+    q, got, _ = attend(fk, p, 8, fault=fault)
+    p.table[0, 9] = 0
+    ref, size = attention(p, q, 8, 128 ** -0.5)
+    other = slice(60, 110)
+    assert bool((np.abs(wide(got[other]) - ref[other]) <= 2.0 ** -8 * np.abs(ref[other]) + (2.0 ** -8 + 2.0 ** -11) * size[other]).all())
+    with pytest.raises(fk.InvalidArgument, match="page id"):
+        fk.paged_check(fault)
