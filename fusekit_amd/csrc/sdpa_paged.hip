@@ -29,8 +29,9 @@ struct SdpaPagedArgs {
     float scale, softcap;
     float* partials;       // [slots][columns of a tile][D], then (m, l) [slots][columns of a tile]
     uint32_t* counters;    // [slots], zero before the first launch, left zero
-    uint32_t slots;
+    uint32_t slots, slot_bytes;
     uint32_t target, min_steps;   // items that a launch is cut into where its tiles are fewer; the least steps of an item
+    uint32_t only_few;            // of chunks among single tokens: whole chunks, cut tokens
 };
 
 // ---- one row of one head by a wave: positions in the order they lie, what the row does not see is not touched ----
@@ -92,7 +93,8 @@ constexpr uint32_t kFewCols = 16, kFewMost = 32, kFewStep = 32, kFewRound = 4 * 
 constexpr uint32_t kMostSplits = 64;   // items of a tile
 struct PagedItem {
     uint32_t seq, kvh, tile, split, n_splits;
-    uint32_t base;   // the index of the tile's first item; its others follow n_kv apart
+    uint32_t base;   // the slot of the tile's first item, whose others follow n_kv apart
+    uint32_t slot;   // the item's own
     PagedSeq s;
     bool any;
 };
@@ -121,18 +123,29 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
         if (s.bad && i < a.b.n_seqs && index == 0) paged_fault(a.b, s.bad);
         return s;
     };
-    float work = 0.f, pairs = 0.f;
+    bool only_few = !FEW && !TILES && a.only_few != 0;   // (whole tiles have no slots)
+    auto whole = [&](const PagedSeq& s) { return only_few && s.rows * a.group > kFewMost; };
+    float work = 0.f, pairs = 0.f, wholes = 0.f, longest_whole = 0.f, longest_cut = 0.f;   // pairs: of tiles that may be cut
     PagedSeq mine = read(0);
     for (uint32_t at = 0;;) {
         const float t = (float)tiles_of(mine) * (float)n_kv;
         work = fmaf(t, (float)steps_of(mine), work);   // (the merge forms the same value)
-        pairs += t;
+        pairs += whole(mine) ? 0.f : t;
+        if (only_few) {
+            const float steps = mine.rows ? (float)steps_of(mine) : 0.f;
+            if (whole(mine)) {
+                wholes += t;
+                longest_whole = fmaxf(longest_whole, steps);
+            } else {
+                longest_cut = fmaxf(longest_cut, steps);
+            }
+        }
         if ((at += 64u) >= a.b.n_seqs) break;
         mine = read(at);
     }
     work = wave_sum(work);
     pairs = wave_sum(pairs);
-    const bool cut = pairs + (float)a.target <= (float)a.slots;
+    bool cut = pairs + (float)a.target <= (float)a.slots;
     // (of at least work / target steps: all items together are at most target + pairs)
     const float share = work / (float)a.target;
     uint32_t unit = share < 0x1p30f ? (uint32_t)ceilf(share) : 1u << 30;
@@ -140,12 +153,24 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
     const float of_steps = 1.0f / fmaxf(share, (float)a.min_steps);
     PagedItem it;
     it.any = false;
-    uint32_t left = index, before = 0;   // items of the sequences before
-    for (uint32_t at = 0; at < a.b.n_seqs; at += 64u) {
+    uint32_t left = index, before = 0;   // slots of the sequences before
+    // Single tokens among whole tiles are cut where one of them is twice as long as the tiles; in a launch of more than the card takes at once they come
+    // first, in a way through the sequences of their own, else last, so that each tile has a CU first.  Two chunks of 2048 rows and a token over 100 000
+    // positions, us: not cut 1092, cut and in the sequences' order 215, tokens first 140; a chunk of 2048 and 16 tokens over 8000: 144, 152, 119; a
+    // chunk of 509 rows among 24 tokens over up to 2000: 39, 39, 42.
+    bool tokens = true;
+    if (only_few) {
+        longest_whole = wave_max(longest_whole);
+        longest_cut = wave_max(longest_cut);
+        only_few = cut = cut && longest_cut > 2.0f * longest_whole;
+        tokens = !only_few || wave_sum(wholes) + pairs > (float)a.target;
+    }
+    bool second = !only_few;
+    for (uint32_t at = 0;;) {
         if (a.b.n_seqs > 64u) mine = read(at);
         const uint32_t tiles = tiles_of(mine);
         // (tiles: as many as fit; an integer share gave a chunk of 512 rows behind 3000 384 items instead of 512)
-        uint32_t splits = !cut ? 1u : FEW ? (steps_of(mine) + unit - 1u) / unit : (uint32_t)fmaf((float)steps_of(mine), of_steps, 0x1p-10f);
+        uint32_t splits = !cut || whole(mine) ? 1u : FEW || only_few ? (steps_of(mine) + unit - 1u) / unit : (uint32_t)fmaf((float)steps_of(mine), of_steps, 0x1p-10f);
         splits = splits < 1u ? 1u : splits > kMostSplits ? kMostSplits : splits;
         const uint32_t items = tiles * splits * n_kv;
         auto with_those_before = [&](uint32_t upto) {
@@ -156,17 +181,24 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
             }
             return upto;
         };
-        const uint32_t upto = with_those_before(items), count = TILES ? tiles * n_kv : items, counted = TILES ? with_those_before(count) : upto;
+        const uint32_t count = TILES ? tiles * n_kv : only_few && whole(mine) == tokens ? 0u : items;
+        const uint32_t counted = with_those_before(count), upto = TILES ? with_those_before(items) : counted;
         const unsigned long long past = __builtin_amdgcn_ballot_w64(counted > left);
         if (!past) {
             left -= (uint32_t)__builtin_amdgcn_readlane((int)counted, 63);
-            before += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+            before += tokens ? (uint32_t)__builtin_amdgcn_readlane((int)upto, 63) : 0u;
+            at += 64u;
+            if (at < a.b.n_seqs) continue;
+            if (second) break;
+            second = true;
+            tokens = !tokens;
+            at = 0;
             continue;
         }
         const int who = (int)__builtin_ctzll(past);
         auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, who); };
         left -= of(counted) - of(count);
-        before += of(upto) - of(items);
+        before += of(upto) - of(TILES ? items : count);
         it.seq = at + (uint32_t)who;
         it.s = PagedSeq{of(mine.row0), of(mine.rows), of(mine.len), of(mine.bad)};
         it.n_splits = of(splits);
@@ -176,6 +208,7 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
         left = TILES ? left : left / it.n_splits;
         it.tile = of(tiles) - 1u - left;   // the longest first
         it.base = before + left * it.n_splits * n_kv + it.kvh;
+        it.slot = it.base + it.split * n_kv;
         it.any = true;
         break;
     }
@@ -208,7 +241,7 @@ __device__ __forceinline__ void paged_hand_on(const SdpaPagedArgs& a, const Page
     constexpr uint32_t OS = D + 4, VP = D / 8;
     const uint32_t G = a.group;
     if (!whole) {
-        const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials + (size_t)blockIdx.x * (kTileCols * (D + 2u)), 0, (int)(kTileCols * (D + 2u) * 4u), 0x27000);
+        const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials + (size_t)it.slot * (kTileCols * (D + 2u)), 0, (int)(kTileCols * (D + 2u) * 4u), 0x27000);
         for (uint32_t idx = lane; idx < live * (uint32_t)(D / 4); idx += 64u) {
             const uint32_t col = idx / (uint32_t)(D / 4), pc = idx % (uint32_t)(D / 4);
             const pf_u32x4_t v = *reinterpret_cast<const pf_u32x4_t*>(ob + col * OS + pc * 4u);
@@ -638,7 +671,7 @@ constexpr uint32_t few_lds_bytes(uint32_t d) {
     return (stages > meet ? stages : meet) + 16u;   // and two words for the block
 }
 
-template <int D, bool CAP, bool WIDE, uint32_t SLOT_COLS>
+template <int D, bool CAP, bool WIDE>
 __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedItem& it, uint32_t lane) {
     constexpr uint32_t ROW = D * 2u, P = D / 8u, KT = kFewStep * ROW, STAGE = 2u * KT, RPI = 1024u / ROW;   // pieces of a row; rows of a request
     constexpr int REQ = (int)(KT / 1024u), KS = D / 32, DT = D / 16, PARTS = WIDE ? 2 : 1;
@@ -856,8 +889,7 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
     }
     __syncthreads();
     const bool whole = n_active == 1u;
-    constexpr uint32_t SLOT = SLOT_COLS * (D + 2u) * 4u;
-    const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials, 0, (int)(a.slots * SLOT), 0x27000);
+    const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials, 0, (int)(a.slots * a.slot_bytes), 0x27000);
     auto store = [&](uint32_t c, uint32_t d, const float4& o, float l) {
         const float f = l > 0.f || l != l ? 1.0f / l : 0.f;   // (a row that sees nothing: zeros)
         const float t = (__builtin_fabsf(o.x) + __builtin_fabsf(o.y)) + (__builtin_fabsf(o.z) + __builtin_fabsf(o.w));
@@ -884,7 +916,7 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
         if (whole) {
             store(c, d, o, l);
         } else {
-            const uint32_t at = blockIdx.x * SLOT;
+            const uint32_t at = it.slot * a.slot_bytes;
             const pf_u32x4_t v = {__float_as_uint(o.x), __float_as_uint(o.y), __float_as_uint(o.z), __float_as_uint(o.w)};
             __builtin_amdgcn_raw_buffer_store_b128(v, mem, (int)(at + (c * D + d) * 4u), 0, kPastCaches);
             if (d == 0) {
@@ -902,8 +934,8 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
         if (!word[0]) return;
         if (tid == 0) __hip_atomic_store(&a.counters[base], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         auto none = [](uint32_t) {};
-        if (n_active <= 8u) paged_merge_columns<D, kPastCaches, 8, 4>(mem, base, stride, SLOT, kFewCols * D * 4u, wave, columns, 4u, n_active, lane, store, none);
-        else paged_merge_columns<D, kPastCaches, 32, 1>(mem, base, stride, SLOT, kFewCols * D * 4u, wave, columns, 4u, n_active, lane, store, none);
+        if (n_active <= 8u) paged_merge_columns<D, kPastCaches, 8, 4>(mem, base, stride, a.slot_bytes, kFewCols * D * 4u, wave, columns, 4u, n_active, lane, store, none);
+        else paged_merge_columns<D, kPastCaches, 32, 1>(mem, base, stride, a.slot_bytes, kFewCols * D * 4u, wave, columns, 4u, n_active, lane, store, none);
     }
     __syncthreads();
     for (uint32_t again = word[1], c = 0; again; again >>= 1, ++c)
@@ -917,14 +949,14 @@ __global__ __launch_bounds__(256, 2) void sdpa_paged_kernel(const SdpaPagedArgs 
     const uint32_t lane = threadIdx.x & 63u;
     const PagedItem it = paged_item<false, kTileCols / SPLIT>(a, blockIdx.x, lane);
     if (!it.any) return;
-    if (it.s.rows * a.group <= kFewMost) paged_few<D, CAP, true, kTileCols>(a, it, lane);
+    if (it.s.rows * a.group <= kFewMost) paged_few<D, CAP, true>(a, it, lane);
     else paged_tile<D, CAP, SPLIT>(a, it, lane);
 }
 template <int D, bool CAP, bool WIDE>
 __global__ __launch_bounds__(256, 2) void sdpa_paged_few_kernel(const SdpaPagedArgs a) {
     const uint32_t lane = threadIdx.x & 63u;
     const PagedItem it = paged_item<true, kFewCols>(a, blockIdx.x, lane);
-    if (it.any) paged_few<D, CAP, WIDE, kFewCols>(a, it, lane);
+    if (it.any) paged_few<D, CAP, WIDE>(a, it, lane);
 }
 
 namespace {
@@ -932,10 +964,11 @@ namespace {
 // How a launch is cut: fewer tiles than `target` are cut along their positions, into items of `min_steps` steps at least.
 struct PagedPlan {
     bool few;          // single tokens: 16 columns a sequence and KV head at most
-    uint32_t target, min_steps, slots;
+    uint32_t target, min_steps, slots, few_slots;
     uint64_t tiles;    // of all sequences and KV heads, at most
     size_t slot_bytes, bytes;
 };
+constexpr uint32_t kFewLeast = 16;             // steps of 64 positions of a token among whole chunks
 constexpr size_t kPagedCounterBytes = 16384;   // a word for a slot
 PagedPlan paged_plan(bool few, uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t n_seqs, uint32_t rows) {
     PagedPlan p;
@@ -950,7 +983,9 @@ PagedPlan paged_plan(bool few, uint32_t n_heads, uint32_t n_kv, uint32_t head_di
     const uint32_t most = few ? 2048 : 896;   // slots: 64 MB at the most
     p.slots = p.tiles <= most / 2 ? std::min((uint32_t)p.tiles + p.target, most) : 0;   // (rounding leaves an item more for every tile)
     p.target = p.slots ? p.slots - (uint32_t)p.tiles : p.target;
-    p.bytes = kPagedCounterBytes + p.slots * p.slot_bytes;
+    // tiles of 128 that are too many to cut: the single tokens among them, which need not be short
+    p.few_slots = !few && !p.slots && n_seqs <= (2048u - 512u) / (2u * n_kv) ? 512u + 2u * n_kv * n_seqs : 0u;
+    p.bytes = kPagedCounterBytes + (p.few_slots ? p.few_slots * (size_t)kFewCols * (head_dim + 2) * 4 : p.slots * p.slot_bytes);
     return p;
 }
 
@@ -1024,10 +1059,18 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     const uint64_t filled = ((uint64_t)batch->rows * a.group + kTileCols / 2 - 1) / (kTileCols / 2), halves = (std::max<uint64_t>(filled, 2) + 2 * (uint64_t)(batch->n_seqs - 1)) * n_kv;
     const bool split = !p.few && halves <= (uint64_t)dev->cus && most > 4u && most <= 12u + halves / 12u;
     const bool cut = !split && p.slots && (p.few ? splits > 1u : most > 8u);
+    a.slot_bytes = (uint32_t)p.slot_bytes;
+    a.only_few = !cut && !split && p.few_slots && most > 2u * kFewLeast;
     if (!cut) a.slots = 0;
+    if (a.only_few) {
+        a.slots = p.few_slots;
+        a.slot_bytes = kFewCols * (D + 2u) * 4u;
+        a.target = 512;
+        a.min_steps = kFewLeast;
+    }
     l->func = p.few ? few[D == 128][softcap > 0.f][batch->max_rows * (n_heads / n_kv) > 8u] : tile[D == 128][softcap > 0.f][split];
     // (no more blocks than there can be items: one that finds none costs what it takes to look)
-    l->grid = dim3((uint32_t)(cut ? std::min<uint64_t>(p.slots, p.tiles * splits) : split ? halves : p.tiles), 1, 1);
+    l->grid = dim3((uint32_t)(cut ? std::min<uint64_t>(p.slots, p.tiles * splits) : split ? halves : p.tiles + (a.only_few ? a.target : 0u)), 1, 1);
     l->block = dim3(256, 1, 1);
     l->shmem = p.few ? few_lds_bytes(D) : std::max(tile_lds_bytes(D, split ? 2u : 1u), few_lds_bytes(D));
     if ((int)l->shmem > dev->max_dyn_lds) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: LDS tile does not fit");

@@ -398,3 +398,12 @@ def test_few_tiles_bad_page(fk):
     assert bool((np.abs(wide(got[other]) - ref[other]) <= 2.0 ** -8 * np.abs(ref[other]) + (2.0 ** -8 + 2.0 ** -11) * size[other]).all())
     with pytest.raises(fk.InvalidArgument, match="page id"):
         fk.paged_check(fault)
+
+
+@pytest.mark.parametrize("rows,lens", [([300, 1, 2], [300, 2500, 1500]), ([1, 140, 1, 0], [4000, 200, 70, 90]), ([1, 1, 150], [2049, 5000, 151])])
+@pytest.mark.parametrize("n_heads,dim,window,softcap", [(64, 64, 0, 0.0), (64, 128, 2100, 0.0), (128, 64, 0, 20.0)])
+def test_long_tokens_among_more_tiles_than_are_cut(fk, rows, lens, n_heads, dim, window, softcap):
+    p = Paged(rows, lens, 64, dim, 32, seed=50 + len(rows))
+    ws = fk.zeros(fk.sdpa_paged_workspace_bytes(n_heads, 64, dim, len(rows), sum(rows), max(lens)))
+    for _ in range(2):                                       # a workspace is left ready
+        check_attention(fk, p, n_heads, softcap=softcap, window=window, workspace=ws)
