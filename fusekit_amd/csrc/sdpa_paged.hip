@@ -31,7 +31,8 @@ struct SdpaPagedArgs {
     uint32_t* counters;    // [slots], zero before the first launch, left zero
     uint32_t slots, slot_bytes;
     uint32_t target, min_steps;   // items that a launch is cut into where its tiles are fewer; the least steps of an item
-    uint32_t only_few;            // of chunks among single tokens: whole chunks, cut tokens
+    uint32_t compact;             // tiles may be more than slots: only those that are cut have some
+    uint32_t only_few;            // of chunks among single tokens: whole chunks, cut tokens (compact)
 };
 
 // ---- one row of one head by a wave: positions in the order they lie, what the row does not see is not touched ----
@@ -145,7 +146,9 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
     }
     work = wave_sum(work);
     pairs = wave_sum(pairs);
-    bool cut = pairs + (float)a.target <= (float)a.slots;
+    // (compact: a tile that is cut has more than one share, and fewer than twice as many items as shares: 2 target of them have slots)
+    const bool compact = only_few || (!TILES && a.compact != 0 && !(pairs + (float)a.target <= (float)a.slots));
+    bool cut = compact || pairs + (float)a.target <= (float)a.slots;
     // (of at least work / target steps: all items together are at most target + pairs)
     const float share = work / (float)a.target;
     uint32_t unit = share < 0x1p30f ? (uint32_t)ceilf(share) : 1u << 30;
@@ -162,7 +165,7 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
     if (only_few) {
         longest_whole = wave_max(longest_whole);
         longest_cut = wave_max(longest_cut);
-        only_few = cut = cut && longest_cut > 2.0f * longest_whole;
+        only_few = cut = longest_cut > 2.0f * longest_whole;
         tokens = !only_few || wave_sum(wholes) + pairs > (float)a.target;
     }
     bool second = !only_few;
@@ -182,11 +185,12 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
             return upto;
         };
         const uint32_t count = TILES ? tiles * n_kv : only_few && whole(mine) == tokens ? 0u : items;
-        const uint32_t counted = with_those_before(count), upto = TILES ? with_those_before(items) : counted;
+        const uint32_t slots = compact && splits == 1u ? 0u : TILES ? items : count;
+        const uint32_t counted = with_those_before(count), upto = TILES || compact ? with_those_before(slots) : counted;
         const unsigned long long past = __builtin_amdgcn_ballot_w64(counted > left);
         if (!past) {
             left -= (uint32_t)__builtin_amdgcn_readlane((int)counted, 63);
-            before += tokens ? (uint32_t)__builtin_amdgcn_readlane((int)upto, 63) : 0u;
+            before += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
             at += 64u;
             if (at < a.b.n_seqs) continue;
             if (second) break;
@@ -198,7 +202,7 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
         const int who = (int)__builtin_ctzll(past);
         auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, who); };
         left -= of(counted) - of(count);
-        before += of(upto) - of(TILES ? items : count);
+        before += of(upto) - of(slots);
         it.seq = at + (uint32_t)who;
         it.s = PagedSeq{of(mine.row0), of(mine.rows), of(mine.len), of(mine.bad)};
         it.n_splits = of(splits);
@@ -964,6 +968,7 @@ namespace {
 // How a launch is cut: fewer tiles than `target` are cut along their positions, into items of `min_steps` steps at least.
 struct PagedPlan {
     bool few;          // single tokens: 16 columns a sequence and KV head at most
+    bool compact;      // more tiles than slots
     uint32_t target, min_steps, slots, few_slots;
     uint64_t tiles;    // of all sequences and KV heads, at most
     size_t slot_bytes, bytes;
@@ -981,10 +986,10 @@ PagedPlan paged_plan(bool few, uint32_t n_heads, uint32_t n_kv, uint32_t head_di
     p.tiles = few ? (columns / kFewCols + n_seqs) * n_kv : (columns / kTileCols + (uint64_t)n_seqs * (kFewMost / kFewCols)) * n_kv;
     p.slot_bytes = (size_t)cols * (head_dim + 2) * 4;
     const uint32_t most = few ? 2048 : 896;   // slots: 64 MB at the most
-    p.slots = p.tiles <= most / 2 ? std::min((uint32_t)p.tiles + p.target, most) : 0;   // (rounding leaves an item more for every tile)
-    p.target = p.slots ? p.slots - (uint32_t)p.tiles : p.target;
-    // tiles of 128 that are too many to cut: the single tokens among them, which need not be short
-    p.few_slots = !few && !p.slots && n_seqs <= (2048u - 512u) / (2u * n_kv) ? 512u + 2u * n_kv * n_seqs : 0u;
+    p.compact = p.tiles > most / 2;
+    p.slots = !p.compact ? std::min((uint32_t)p.tiles + p.target, most) : few ? 2 * p.target + 64 : 0;   // (rounding leaves an item more for every tile)
+    p.target = p.compact ? p.target : p.slots - (uint32_t)p.tiles;
+    p.few_slots = !few && p.compact ? 2 * p.target + 64 : 0;   // tiles of 128 that are too many to cut: the single tokens among them, which need not be short
     p.bytes = kPagedCounterBytes + (p.few_slots ? p.few_slots * (size_t)kFewCols * (head_dim + 2) * 4 : p.slots * p.slot_bytes);
     return p;
 }
@@ -1058,19 +1063,21 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     // (at most so many tiles: a sequence of few columns has two, of more one beyond what all together fill)
     const uint64_t filled = ((uint64_t)batch->rows * a.group + kTileCols / 2 - 1) / (kTileCols / 2), halves = (std::max<uint64_t>(filled, 2) + 2 * (uint64_t)(batch->n_seqs - 1)) * n_kv;
     const bool split = !p.few && halves <= (uint64_t)dev->cus && most > 4u && most <= 12u + halves / 12u;
-    const bool cut = !split && p.slots && (p.few ? splits > 1u : most > 8u);
+    // (more single tokens than have slots: a block for each that may be cut off takes what it takes to find none, 256 over 500 positions 110 us for 100; over
+    // more than 8 rounds nothing that shows, and of 255 over 500 and one over 60 000 156 us for 688)
+    const bool cut = !split && p.slots && (p.few && !p.compact ? splits > 1u : most > 8u);
     a.slot_bytes = (uint32_t)p.slot_bytes;
+    a.compact = p.few && p.compact;
     a.only_few = !cut && !split && p.few_slots && most > 2u * kFewLeast;
     if (!cut) a.slots = 0;
     if (a.only_few) {
         a.slots = p.few_slots;
         a.slot_bytes = kFewCols * (D + 2u) * 4u;
-        a.target = 512;
         a.min_steps = kFewLeast;
     }
     l->func = p.few ? few[D == 128][softcap > 0.f][batch->max_rows * (n_heads / n_kv) > 8u] : tile[D == 128][softcap > 0.f][split];
     // (no more blocks than there can be items: one that finds none costs what it takes to look)
-    l->grid = dim3((uint32_t)(cut ? std::min<uint64_t>(p.slots, p.tiles * splits) : split ? halves : p.tiles + (a.only_few ? a.target : 0u)), 1, 1);
+    l->grid = dim3((uint32_t)(cut && !a.compact ? std::min<uint64_t>(p.slots, p.tiles * splits) : split ? halves : p.tiles + (cut || a.only_few ? a.target : 0u)), 1, 1);
     l->block = dim3(256, 1, 1);
     l->shmem = p.few ? few_lds_bytes(D) : std::max(tile_lds_bytes(D, split ? 2u : 1u), few_lds_bytes(D));
     if ((int)l->shmem > dev->max_dyn_lds) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: LDS tile does not fit");

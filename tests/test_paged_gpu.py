@@ -407,3 +407,18 @@ def test_long_tokens_among_more_tiles_than_are_cut(fk, rows, lens, n_heads, dim,
     ws = fk.zeros(fk.sdpa_paged_workspace_bytes(n_heads, 64, dim, len(rows), sum(rows), max(lens)))
     for _ in range(2):                                       # a workspace is left ready
         check_attention(fk, p, n_heads, softcap=softcap, window=window, workspace=ws)
+
+
+@pytest.mark.parametrize("n_seqs,long_at,chunk_at", [(300, (7, 290), None), (130, (0,), None), (70, (3, 69), 65), (150, (149,), 0), (200, (), None)])
+@pytest.mark.parametrize("dim,window,softcap", [(64, 0, 0.0), (128, 3000, 20.0)])
+def test_more_sequences_than_have_slots(fk, n_seqs, long_at, chunk_at, dim, window, softcap):
+    lens = [int(n) for n in rng(n_seqs).integers(1, 40, n_seqs)]
+    rows = [1] * n_seqs
+    for i in long_at:
+        lens[i] = 3500 + i
+    if chunk_at is not None:
+        rows[chunk_at], lens[chunk_at] = 90, 130
+    p = Paged(rows, lens, 8, dim, 32, seed=60, spare_table=0)
+    ws = fk.zeros(fk.sdpa_paged_workspace_bytes(16, 8, dim, n_seqs, sum(rows), max(lens)))
+    for _ in range(2):
+        check_attention(fk, p, 16, softcap=softcap, window=window, workspace=ws)
