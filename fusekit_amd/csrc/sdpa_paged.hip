@@ -127,8 +127,22 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
     bool only_few = !FEW && !TILES && a.only_few != 0;   // (whole tiles have no slots)
     auto whole = [&](const PagedSeq& s) { return only_few && s.rows * a.group > kFewMost; };
     float work = 0.f, pairs = 0.f, wholes = 0.f, longest_whole = 0.f, longest_cut = 0.f;   // pairs: of tiles that may be cut
-    PagedSeq mine = read(0);
-    for (uint32_t at = 0;;) {
+    // (64 sequences at a time, three requests ahead: 1000 of them were 32 trips to memory one after another, 443 us of their tokens over 300 positions each for
+    // 220; 256 over 500 103 for 49)
+    const bool many = a.b.n_seqs > 64u;
+    PagedSeq mine, ahead[3];
+    auto from_the_first = [&] {
+        mine = read(0);
+        if (many)
+#pragma unroll
+            for (uint32_t u = 0; u < 3; ++u) ahead[u] = read(64u * (u + 1u));
+    };
+    auto next = [&](uint32_t at) {   // (past the last sequence: ones without rows)
+        mine = ahead[0], ahead[0] = ahead[1], ahead[1] = ahead[2];
+        ahead[2] = read(at + 192u);
+    };
+    from_the_first();
+    for (uint32_t at = 0; a.slots != 0 || index == 0;) {   // (nothing to cut: for the faults alone)
         const float t = (float)tiles_of(mine) * (float)n_kv;
         work = fmaf(t, (float)steps_of(mine), work);   // (the merge forms the same value)
         pairs += whole(mine) ? 0.f : t;
@@ -142,7 +156,7 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
             }
         }
         if ((at += 64u) >= a.b.n_seqs) break;
-        mine = read(at);
+        next(at);
     }
     work = wave_sum(work);
     pairs = wave_sum(pairs);
@@ -169,8 +183,8 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
         tokens = !only_few || wave_sum(wholes) + pairs > (float)a.target;
     }
     bool second = !only_few;
+    if (many) from_the_first();
     for (uint32_t at = 0;;) {
-        if (a.b.n_seqs > 64u) mine = read(at);
         const uint32_t tiles = tiles_of(mine);
         // (tiles: as many as fit; an integer share gave a chunk of 512 rows behind 3000 384 items instead of 512)
         uint32_t splits = !cut || whole(mine) ? 1u : FEW || only_few ? (steps_of(mine) + unit - 1u) / unit : (uint32_t)fmaf((float)steps_of(mine), of_steps, 0x1p-10f);
@@ -192,11 +206,15 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
             left -= (uint32_t)__builtin_amdgcn_readlane((int)counted, 63);
             before += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
             at += 64u;
-            if (at < a.b.n_seqs) continue;
+            if (at < a.b.n_seqs) {
+                next(at);
+                continue;
+            }
             if (second) break;
             second = true;
             tokens = !tokens;
             at = 0;
+            if (many) from_the_first();
             continue;
         }
         const int who = (int)__builtin_ctzll(past);
@@ -1063,8 +1081,8 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     // (at most so many tiles: a sequence of few columns has two, of more one beyond what all together fill)
     const uint64_t filled = ((uint64_t)batch->rows * a.group + kTileCols / 2 - 1) / (kTileCols / 2), halves = (std::max<uint64_t>(filled, 2) + 2 * (uint64_t)(batch->n_seqs - 1)) * n_kv;
     const bool split = !p.few && halves <= (uint64_t)dev->cus && most > 4u && most <= 12u + halves / 12u;
-    // (more single tokens than have slots: a block for each that may be cut off takes what it takes to find none, 256 over 500 positions 110 us for 100; over
-    // more than 8 rounds nothing that shows, and of 255 over 500 and one over 60 000 156 us for 688)
+    // (more single tokens than have slots: a block for each that may be cut off takes what it takes to find none, up to a tenth of 256 tokens over 500
+    // positions; over more than 8 rounds nothing that shows, and of 255 over 500 and one over 60 000 156 us for 688)
     const bool cut = !split && p.slots && (p.few && !p.compact ? splits > 1u : most > 8u);
     a.slot_bytes = (uint32_t)p.slot_bytes;
     a.compact = p.few && p.compact;
