@@ -127,8 +127,7 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
     bool only_few = !FEW && !TILES && a.only_few != 0;   // (whole tiles have no slots)
     auto whole = [&](const PagedSeq& s) { return only_few && s.rows * a.group > kFewMost; };
     float work = 0.f, pairs = 0.f, wholes = 0.f, longest_whole = 0.f, longest_cut = 0.f;   // pairs: of tiles that may be cut
-    // (64 sequences at a time, three requests ahead: 1000 of them were 32 trips to memory one after another, 443 us of their tokens over 300 positions each for
-    // 220; 256 over 500 103 for 49)
+    // (64 sequences at a time, three requests ahead, and once where nothing is cut: 1000 of them were 32 trips to memory one after another)
     const bool many = a.b.n_seqs > 64u;
     PagedSeq mine, ahead[3];
     auto from_the_first = [&] {
@@ -142,7 +141,8 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
         ahead[2] = read(at + 192u);
     };
     from_the_first();
-    for (uint32_t at = 0; a.slots != 0 || index == 0;) {   // (nothing to cut: for the faults alone)
+    const bool once = a.slots == 0 && index != 0;   // (nothing to cut: the sums are for the faults alone)
+    for (uint32_t at = 0; !once;) {
         const float t = (float)tiles_of(mine) * (float)n_kv;
         work = fmaf(t, (float)steps_of(mine), work);   // (the merge forms the same value)
         pairs += whole(mine) ? 0.f : t;
@@ -183,7 +183,7 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
         tokens = !only_few || wave_sum(wholes) + pairs > (float)a.target;
     }
     bool second = !only_few;
-    if (many) from_the_first();
+    if (many && !once) from_the_first();
     for (uint32_t at = 0;;) {
         const uint32_t tiles = tiles_of(mine);
         // (tiles: as many as fit; an integer share gave a chunk of 512 rows behind 3000 384 items instead of 512)
@@ -1085,7 +1085,7 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     // positions; over more than 8 rounds nothing that shows, and of 255 over 500 and one over 60 000 156 us for 688)
     const bool cut = !split && p.slots && (p.few && !p.compact ? splits > 1u : most > 8u);
     a.slot_bytes = (uint32_t)p.slot_bytes;
-    a.compact = p.few && p.compact;
+    a.compact = cut && p.few && p.compact;
     a.only_few = !cut && !split && p.few_slots && most > 2u * kFewLeast;
     if (!cut) a.slots = 0;
     if (a.only_few) {

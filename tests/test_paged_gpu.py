@@ -422,3 +422,10 @@ def test_more_sequences_than_have_slots(fk, n_seqs, long_at, chunk_at, dim, wind
     ws = fk.zeros(fk.sdpa_paged_workspace_bytes(16, 8, dim, n_seqs, sum(rows), max(lens)))
     for _ in range(2):
         check_attention(fk, p, 16, softcap=softcap, window=window, workspace=ws)
+
+
+@pytest.mark.parametrize("n_seqs,longest", [(130, 260), (256, 500), (140, 1024), (140, 1025), (300, 129)])
+def test_more_sequences_than_have_slots_of_some_rounds(fk, n_seqs, longest):
+    lens = [int(n) for n in rng(longest).integers(100, longest + 1, n_seqs)]
+    lens[5] = longest
+    check_attention(fk, Paged([1] * n_seqs, lens, 8, 64, 64, seed=61, spare_table=0), 8)
