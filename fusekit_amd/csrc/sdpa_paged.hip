@@ -983,6 +983,8 @@ __global__ __launch_bounds__(256, 2) void sdpa_paged_few_kernel(const SdpaPagedA
 
 namespace {
 
+static_assert(16384u + 896u * kTileCols * (128u + 2u) * 4u <= FK_SDPA_PAGED_WORKSPACE_MOST && 16384u + 2048u * kFewCols * (128u + 2u) * 4u <= FK_SDPA_PAGED_WORKSPACE_MOST);
+
 // How a launch is cut: fewer tiles than `target` are cut along their positions, into items of `min_steps` steps at least.
 struct PagedPlan {
     bool few;          // single tokens: 16 columns a sequence and KV head at most
@@ -1003,7 +1005,7 @@ PagedPlan paged_plan(bool few, uint32_t n_heads, uint32_t n_kv, uint32_t head_di
     const uint64_t columns = (uint64_t)rows * (n_heads / n_kv);
     p.tiles = few ? (columns / kFewCols + n_seqs) * n_kv : (columns / kTileCols + (uint64_t)n_seqs * (kFewMost / kFewCols)) * n_kv;
     p.slot_bytes = (size_t)cols * (head_dim + 2) * 4;
-    const uint32_t most = few ? 2048 : 896;   // slots: 64 MB at the most
+    const uint32_t most = few ? 2048 : 896;   // slots: FK_SDPA_PAGED_WORKSPACE_MOST at the most
     p.compact = p.tiles > most / 2;
     p.slots = !p.compact ? std::min((uint32_t)p.tiles + p.target, most) : few ? 2 * p.target + 64 : 0;   // (rounding leaves an item more for every tile)
     p.target = p.compact ? p.target : p.slots - (uint32_t)p.tiles;

@@ -675,6 +675,9 @@ def rope_paged_store(q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride,
                                   _addr(q_norm), _addr(k_norm), eps, rope_dims, interleaved, _addr(freq), batch, pool, _addr(stream)))
 
 
+SDPA_PAGED_WORKSPACE_MOST = 64 << 20   # serves every shape
+
+
 def sdpa_paged_workspace_bytes(n_heads, n_kv, head_dim, n_seqs, rows, max_len) -> int:
     out = C.c_size_t()
     check(lib.fk_sdpa_paged_workspace_bytes(n_heads, n_kv, head_dim, n_seqs, rows, max_len, C.byref(out)))

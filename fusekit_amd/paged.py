@@ -178,10 +178,7 @@ class PagedDecoder:
         seqs = {S, *(v for v in (384, 256, 128, 64, 32) if v < S)}
         ws = max(2 * ws, max(native.qgemm_workspace_bytes(m, c.vocab, c.hidden, 0 if self.head.bits == 16 else self.head.group) for m in seqs))
         self.ws = DeviceBuffer(ws)
-        # (for any number of sequences and rows up to these: the most that a batch of them asks for)
-        sdpa = max(native.sdpa_paged_workspace_bytes(c.n_heads, c.n_kv, c.head_dim, s, max(s, r), page_rows * n_pages)
-                   for s in range(1, S + 1) for r in {R, *(v for v in range(128, R, 128))})
-        self.sdpa_ws = native.zeros(sdpa)
+        self.sdpa_ws = native.zeros(native.SDPA_PAGED_WORKSPACE_MOST)
 
     def forward(self, batch: Sequence[Tuple[PagedSequence, Sequence[int]]]) -> DeviceBuffer:
         """Each sequence takes its new tokens (one at least); returns the logits [len(batch), vocab], overwritten by the next call."""

@@ -634,8 +634,10 @@ fk_status fk_rope_paged_store(const uint16_t *q, uint32_t q_stride, const uint16
  *     strides multiples of 8, pointers 16-byte aligned; out must not overlap q.  One call serves chunks of prompts and
  *     single tokens together; a row's result does not depend on the other sequences but for the order in which its
  *     positions are added up (how finely a long context is cut goes by the whole batch).
- *     workspace: fk_sdpa_paged_workspace_bytes() bytes (below 64 MB), zeroed before the first launch and left ready by each;
- *     launches that share it must not overlap, those of graphs included. */
+ *     workspace: fk_sdpa_paged_workspace_bytes() bytes, or the bytes that serve every shape (the former grow and shrink with the
+ *     rows), zeroed before the first launch and left ready by each; launches that share it must not overlap, those of graphs
+ *     included. */
+#define FK_SDPA_PAGED_WORKSPACE_MOST (64u << 20)
 fk_status fk_sdpa_paged_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t n_seqs, uint32_t rows,
                                         uint32_t max_len, size_t *bytes);
 fk_status fk_sdpa_paged(const uint16_t *q, uint32_t q_stride, uint16_t *out, uint32_t out_stride, uint32_t n_heads,

@@ -228,3 +228,12 @@ def test_sound_calls_ask_for_the_device():
         with pytest.raises(fk.FusekitError) as e:
             call()
         assert e.value.status == fk.FK_ERR_HIP
+
+
+def test_one_workspace_serves_every_shape():
+    draw = np.random.default_rng(0)
+    for _ in range(3000):
+        n_kv, group = int(draw.integers(1, 129)), int(draw.integers(1, 33))
+        n_seqs, rows = (int(np.exp(draw.uniform(0, np.log(20000)))) for _ in range(2))
+        need = fk.sdpa_paged_workspace_bytes(n_kv * group, n_kv, int(draw.choice([64, 128])), n_seqs, rows, int(draw.integers(1, 10 ** 6)))
+        assert need <= fk.SDPA_PAGED_WORKSPACE_MOST
