@@ -993,23 +993,26 @@ struct PagedPlan {
     uint64_t tiles;    // of all sequences and KV heads, at most
     size_t slot_bytes, bytes;
 };
-constexpr uint32_t kFewLeast = 16;             // steps of 64 positions of a token among whole chunks
+constexpr uint32_t kFewLeast = 16, kFewTarget = 512;   // steps of 64 positions of a token's item among whole chunks; items
 constexpr size_t kPagedCounterBytes = 16384;   // a word for a slot
 PagedPlan paged_plan(bool few, uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t n_seqs, uint32_t rows) {
     PagedPlan p;
     const uint32_t cols = few ? kFewCols : kTileCols;
     p.few = few;
-    p.target = few ? 768 : 512;
+    // (tiles: as many as stand on the card at once, two of 128 dims a CU, three of 64.  Of 64 dims, 32 / 4 heads, 1170 rows behind some 9000 positions 156 us with 768,
+    // 205 with 512, 171 with 1024.)
+    p.target = few || head_dim == 64 ? 768 : 512;
     p.min_steps = few ? 1 : 4;
     // (a sequence of up to kFewMost columns has tiles of 16 also among chunks)
     const uint64_t columns = (uint64_t)rows * (n_heads / n_kv);
     p.tiles = few ? (columns / kFewCols + n_seqs) * n_kv : (columns / kTileCols + (uint64_t)n_seqs * (kFewMost / kFewCols)) * n_kv;
     p.slot_bytes = (size_t)cols * (head_dim + 2) * 4;
-    const uint32_t most = few ? 2048 : 896;   // slots: FK_SDPA_PAGED_WORKSPACE_MOST at the most
-    p.compact = p.tiles > most / 2;
+    // (more tiles are not cut: of 64 dims 600 of 2400 rows behind few positions 90 us, cut 99)
+    const uint32_t most_tiles = few ? 1024 : 448, most = few ? 2048 : head_dim == 64 ? 1216 : 896;   // slots: FK_SDPA_PAGED_WORKSPACE_MOST at the most
+    p.compact = p.tiles > most_tiles;
     p.slots = !p.compact ? std::min((uint32_t)p.tiles + p.target, most) : few ? 2 * p.target + 64 : 0;   // (rounding leaves an item more for every tile)
     p.target = p.compact ? p.target : p.slots - (uint32_t)p.tiles;
-    p.few_slots = !few && p.compact ? 2 * p.target + 64 : 0;   // tiles of 128 that are too many to cut: the single tokens among them, which need not be short
+    p.few_slots = !few && p.compact ? 2 * kFewTarget + 64 : 0;   // tiles of 128 that are too many to cut: the single tokens among them, which need not be short
     p.bytes = kPagedCounterBytes + (p.few_slots ? p.few_slots * (size_t)kFewCols * (head_dim + 2) * 4 : p.slots * p.slot_bytes);
     return p;
 }
@@ -1093,6 +1096,7 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     if (a.only_few) {
         a.slots = p.few_slots;
         a.slot_bytes = kFewCols * (D + 2u) * 4u;
+        a.target = kFewTarget;
         a.min_steps = kFewLeast;
     }
     l->func = p.few ? few[D == 128][softcap > 0.f][batch->max_rows * (n_heads / n_kv) > 8u] : tile[D == 128][softcap > 0.f][split];
