@@ -1,7 +1,8 @@
 // Beam search: the k best continuations of each group's beams, and state rows that follow the beams chosen.
 //
-//     total[b, t] = score[b] + logit[b, t] - lse[b],   lse[b] = m + log sum_t exp(logit[b, t] - m)
+//     total[b, t] = score[b] - log sum_t exp(logit[b, t] - m) + (logit[b, t] - m),   m the largest logit of row b
 //
+// (the differences first: logits of any size, a mask of the type's lowest value among them, lose nothing by it).
 // The k best of a group in order, ties to the lower b * vocab + t.  Inside a row the order is that of the logits, so a row
 // contributes only its k largest logits; rows are then compared in 64 bits.
 #include <math.h>
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
     __shared__ double values[kBeamList], part[4], base[kBeamMax];
     __shared__ uint64_t flats[kBeamList];
     __shared__ uint32_t counts[4], flag, ended[kBeamMax];
-    __shared__ float near[kBeamMax];
+    __shared__ float near[kBeamMax], peak[kBeamMax];
     constexpr uint32_t AHEAD = 6;
     __shared__ uint32_t keys[AHEAD * 256u];
     __shared__ float top[4];
@@ -145,17 +146,17 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
             for (int i = 1; i < VEC * 4; ++i) m2 = __builtin_elementwise_max(m2, beam_order(w[i]));
             most = m2[0] > m2[1] ? m2[0] : m2[1];
             mw = wave_max(beam_value(most));
-            // exp(x - m) as 2^(x L - r), one rounding in the exponent, r the rounded m L: what r and L are off by is put right below
-            const float ref = mw == -INFINITY ? 0.f : mw, r = ref * kBeamLog2E;
+            // exp(x - m) as 2^((x - m) L): the difference first, which is exact or far from 0 whatever the logits' size (x L - m L leaves
+            // fp32 from 2.4e38 on, and is off by 2^-24 of m L before)
+            const float ref = mw == -INFINITY ? 0.f : mw;
             sum = 0.0;
 #pragma unroll
             for (int i = 0; i < VEC * 2; ++i) {
-                const float e0 = __builtin_amdgcn_exp2f(fmaf(bf16_lo(w[2 * i]), kBeamLog2E, -r)), e1 = __builtin_amdgcn_exp2f(fmaf(bf16_hi(w[2 * i]), kBeamLog2E, -r));
-                const float e2 = __builtin_amdgcn_exp2f(fmaf(bf16_lo(w[2 * i + 1]), kBeamLog2E, -r)), e3 = __builtin_amdgcn_exp2f(fmaf(bf16_hi(w[2 * i + 1]), kBeamLog2E, -r));
+                const float e0 = __builtin_amdgcn_exp2f((bf16_lo(w[2 * i]) - ref) * kBeamLog2E), e1 = __builtin_amdgcn_exp2f((bf16_hi(w[2 * i]) - ref) * kBeamLog2E);
+                const float e2 = __builtin_amdgcn_exp2f((bf16_lo(w[2 * i + 1]) - ref) * kBeamLog2E), e3 = __builtin_amdgcn_exp2f((bf16_hi(w[2 * i + 1]) - ref) * kBeamLog2E);
                 sum += (double)((e0 + e1) + (e2 + e3));
             }
             sum = wave_sum_wide(sum);
-            sum *= 1.0 - 0.69314718055994531 * ((double)ref * (double)kBeamLog2E - (double)r);
             if (__builtin_expect(pass != 0 || sum == sum, 1)) break;
             // a NaN among them: it counts as -inf (and an infinity's sum stays what it is)
 #pragma unroll
@@ -316,8 +317,8 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
             }
             s = wave_sum_wide(s);
             if (lane == 0) {
-                values[b] = (double)m;
-                values[kBeamMax + b] = s;
+                peak[b] = m;
+                values[b] = s;
             }
             m4[0] = m4[1], m4[1] = m4[2], m4[2] = m4[3];
             s4[0] = s4[1], s4[1] = s4[2], s4[2] = s4[3];
@@ -326,15 +327,15 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
     __syncthreads();
     if (tid < a.beams) {
         ended[tid] = is_over;
-        base[tid] = is_over ? (double)score : (double)score - (values[tid] + log(values[kBeamMax + tid]));
+        base[tid] = is_over ? (double)score : (double)score - log(values[tid]);   // and a continuation's total: base + (logit - peak)
         near[tid] = (float)base[tid];
     }
     __syncthreads();
     // Entry j of list l (a piece's, in order): its fp32 score, off by less than `margin`, or -inf; and in 64 bits, with its place as beam << 32 |
     // token, which is in the order of beam * vocab + token.  A finished row's one candidate is the first entry of its first piece.
     auto rough = [&](uint32_t b, uint32_t p, uint32_t j, uint32_t key, float& margin) {
-        const float c = near[b], x = ended[b] ? 0.f : beam_value((int)(key >> 16) - 0x8000), v = c + x;
-        margin = fminf(fmaxf(__builtin_fabsf(c), __builtin_fabsf(x)) * 0x1p-22f, 1e30f);
+        const float c = near[b], x = ended[b] ? 0.f : beam_value((int)(key >> 16) - 0x8000) - peak[b], v = c + x;
+        margin = fminf(fmaxf(__builtin_fabsf(c), __builtin_fabsf(x)) * 0x1p-21f, 1e30f);
         return (ended[b] ? (p | j) == 0u : key != 0u) && v > -INFINITY ? v : -INFINITY;
     };
     auto exactly = [&](uint32_t b, uint32_t p, uint32_t j, uint32_t key, uint64_t& flat) {
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
             return (p | j) == 0u ? base[b] : (double)-INFINITY;
         }
         flat = (uint64_t)b << 32 | (p * PIECE + (0xffffu - (key & 0xffffu)));
-        const double v = base[b] + (double)beam_value((int)(key >> 16) - 0x8000);
+        const double v = base[b] + ((double)beam_value((int)(key >> 16) - 0x8000) - (double)peak[b]);
         return key && v > -INFINITY ? v : (double)-INFINITY;
     };
     // The bound: of up to 256 lists from the first 256 / lists entries of each, of more from their first.  k fp32 scores less their margins reach it,
