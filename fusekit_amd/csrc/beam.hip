@@ -5,6 +5,7 @@
 // (the differences first: logits of any size, a mask of the type's lowest value among them, lose nothing by it).
 // The k best of a group in order, ties to the lower b * vocab + t.  Inside a row the order is that of the logits, so a row
 // contributes only its k largest logits; rows are then compared in 64 bits.
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -331,19 +332,21 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
         near[tid] = (float)base[tid];
     }
     __syncthreads();
-    // Entry j of list l (a piece's, in order): its fp32 score, off by less than `margin`, or -inf; and in 64 bits, with its place as beam << 32 |
-    // token, which is in the order of beam * vocab + token.  A finished row's one candidate is the first entry of its first piece.
-    auto rough = [&](uint32_t b, uint32_t p, uint32_t j, uint32_t key, float& margin) {
-        const float c = near[b], x = ended[b] ? 0.f : beam_value((int)(key >> 16) - 0x8000) - peak[b], v = c + x;
-        margin = fminf(fmaxf(__builtin_fabsf(c), __builtin_fabsf(x)) * 0x1p-21f, 1e30f);
-        return (ended[b] ? (p | j) == 0u : key != 0u) && v > -INFINITY ? v : -INFINITY;
+    // Entry j of list l (a piece's, in order): bounds of its score's order in fp32, or nothing; and the score in 64 bits, with its place as
+    // beam, how far the logit's order is below the highest, token: ties go to the lower beam, inside it by the logits and then to the lower
+    // token, also where a score is so large that 64 bits do not tell logits apart.  A finished row's one candidate is the first entry of its first piece.
+    auto rough = [&](uint32_t b, uint32_t p, uint32_t j, uint32_t key, uint32_t& least, uint32_t& most) {
+        // (a sum that leaves fp32 although neither part does is still a candidate: its least order is that of -inf)
+        const float c = near[b], x = ended[b] ? 0.f : fmaxf(beam_value((int)(key >> 16) - 0x8000) - peak[b], -FLT_MAX), v = c + x;
+        const float margin = fminf(fmaxf(__builtin_fabsf(c), __builtin_fabsf(x)) * 0x1p-21f, 0x1p108f);
+        least = order_key(v - margin);
+        most = order_key(fmaxf(v, -FLT_MAX) + margin);
+        return (ended[b] ? (p | j) == 0u : key != 0u) && c > -INFINITY;
     };
-    auto exactly = [&](uint32_t b, uint32_t p, uint32_t j, uint32_t key, uint64_t& flat) {
-        if (ended[b]) {
-            flat = (uint64_t)b << 32 | a.pad;
-            return (p | j) == 0u ? base[b] : (double)-INFINITY;
-        }
-        flat = (uint64_t)b << 32 | (p * PIECE + (0xffffu - (key & 0xffffu)));
+    auto exactly = [&](uint32_t b, uint32_t p, uint32_t j, uint32_t key, uint64_t& at) {
+        at = (uint64_t)b << 48 | a.pad;
+        if (ended[b]) return (p | j) == 0u ? base[b] : (double)-INFINITY;
+        at = (uint64_t)b << 48 | (uint64_t)(0xffffu - (key >> 16)) << 32 | (p * PIECE + (0xffffu - (key & 0xffffu)));
         const double v = base[b] + ((double)beam_value((int)(key >> 16) - 0x8000) - (double)peak[b]);
         return key && v > -INFINITY ? v : (double)-INFINITY;
     };
@@ -355,10 +358,8 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
         const uint32_t j = lists < 256u ? l0 / lists : 0u, l = lists < 256u ? l0 - j * lists : l0;
         if (j >= k) break;
         const uint32_t b = l / a.pieces;
-        float margin;
-        const float v = rough(b, l - b * a.pieces, j, key_of(l, j), margin);
-        const uint32_t o = v > -INFINITY ? order_key(v - margin) : 0u;
-        mine = o > mine ? o : mine;
+        uint32_t least, most;
+        if (rough(b, l - b * a.pieces, j, key_of(l, j), least, most)) mine = least > mine ? least : mine;
     }
     const uint32_t bound = bound_of_best<32, 12>(mine, k, all);
     // Who reaches it: a thread goes down a list as far as fp32 scores with their margins do, and looks at those in 64 bits.
@@ -371,9 +372,8 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
 #pragma unroll 1
         for (uint32_t j = 0; j < k; ++j) {
             const uint32_t key = on ? key_of(l, j) : 0u;
-            float margin;
-            const float near_v = rough(b, p, j, key, margin);
-            on = on && near_v > -INFINITY && order_key(near_v + margin) >= bound;
+            uint32_t least, most;
+            on = rough(b, p, j, key, least, most) && on && most >= bound;
             if (__builtin_amdgcn_ballot_w64(on) == 0) break;
             uint64_t flat;
             const double v = exactly(b, p, j, key, flat);
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
     const bool fits = counts[0] <= kBeamPart && counts[1] <= kBeamPart && counts[2] <= kBeamPart && counts[3] <= kBeamPart;
     auto put = [&](uint32_t at, double v, uint64_t flat) {
         a.out_scores[(size_t)g * k + at] = (float)v;
-        a.out_beams[(size_t)g * k + at] = (uint32_t)(flat >> 32);
+        a.out_beams[(size_t)g * k + at] = (uint32_t)(flat >> 48);
         a.out_tokens[(size_t)g * k + at] = (uint32_t)flat;
     };
     if (__builtin_expect(fits, 1)) {
@@ -413,12 +413,12 @@ __global__ __launch_bounds__(256) void beam_select_kernel(const BeamArgs a) {
         if (__builtin_expect(n >= k || tid != 0, 1)) return;
         // fewer than k above -inf: the lowest places that are not among them
         uint64_t at = 0;
-        auto next = [&] { at = (uint32_t)at + 1u < a.vocab ? at + 1u : ((at >> 32) + 1u) << 32; };
+        auto next = [&] { at = (uint32_t)at + 1u < a.vocab ? at + 1u : ((at >> 48) + 1u) << 48; };
         for (uint32_t i = n; i < k; ++i, next()) {
             for (bool again = true; again;) {
                 again = false;
                 for (uint32_t c = 0; c < kBeamList; ++c)
-                    if (c % kBeamPart < counts[c / kBeamPart] && flats[c] == at) {
+                    if (c % kBeamPart < counts[c / kBeamPart] && (flats[c] >> 48 << 48 | (uint32_t)flats[c]) == at) {
                         next();
                         again = true;
                     }

@@ -654,7 +654,8 @@ fk_status fk_pages_copy(void *base, uint32_t n_planes, size_t plane_stride, uint
  * ties to the lower b * vocab + t.  logits bf16 rows row_stride apart; scores fp32 [groups * beams]; finished (or NULL):
  * u32 [groups * beams], a beam whose word is not 0 goes on only with pad_token and keeps its score.  A row's exponentials are
  * fp32, of the differences from its largest logit, their sum and all sums behind it 64-bit (four terms at a time fp32); finite logits of any
- * size count as what they are, masks of the type's lowest value among them; inside a beam the order is that of the logits.  A NaN
+ * size count as what they are, masks of the type's lowest value among them; inside a beam the order is that of the logits, also where
+ * its score is so large that the sums do not tell them apart (sums beyond fp32 are listed in their order, as -inf).  A NaN
  * logit counts as -inf, a score that is not a number likewise.  Where fewer than k continuations are above -inf, the
  * lowest b * vocab + t that are left follow with -inf.  out_* [groups, k]; beams and k up to 64, groups up to 4096, groups * beams
  * up to 65535.  workspace: fk_beam_select_workspace_bytes(), zeroed once; launches that share it must not overlap. */

@@ -1,5 +1,5 @@
-"""Beam search's selection (fk_beam_select) over the whole range of bf16 logits: masks of the type's lowest value, logits of its largest,
-against a statement in 64 bits that subtracts a row's largest logit first.
+"""Beam search's selection (fk_beam_select) over the whole range of bf16 logits and fp32 scores: masks of the type's lowest value, logits and scores of its
+largest, against a statement in 64 bits that subtracts a row's largest logit first.
 
 Beams and tokens are compared exactly: by the total, then the beam, inside it by the logits, then the token.  A score is a sum of the row's score, a logit
 and the logarithm of a sum of exponentials that are each off by at most 2^-21 of themselves, and is rounded to fp32 once: 2^-21 + 2^-24 |score|."""
@@ -98,3 +98,38 @@ def test_large_logits(fk, offset, sign):
         g = rng(int(np.log10(offset)))
         x = oracle.f32_to_bf16((sign * offset * (1 + 0.02 * g.standard_normal((groups * n_beams, vocab)))).astype(np.float32))
         check(fk, x, -g.random(groups * n_beams), groups, n_beams, 7)
+
+
+@pytest.mark.parametrize("score", [-1e10, -1e17, -1e30, -1e37, -3.3895314e38, -3.4028235e38])
+def test_scores_that_logits_are_lost_in(fk, score):
+    """A beam that took a masked token: its continuations are still in the order of its logits, and behind the other beams'."""
+    x, _ = make(9, 6, 3000)
+    lost = score * (1 - np.arange(6) / 16)                           # (far apart, so that beams do not meet)
+    check(fk, x, np.where([1, 0, 1, 0, 1, 1], lost, [0, -1, 0, -2, 0, 0]), 2, 3, 10)
+    check(fk, np.repeat(x[:1], 6, 0), np.full(6, score), 2, 3, 10)    # equal beams: the lower first
+    x[:, 4:] = LOWEST                                                # totals beyond fp32: listed as -inf, in their order
+    check(fk, x, np.where([1, 0, 1, 0, 1, 1], lost, [0, -1, 0, -2, 0, 0]), 2, 3, 20)
+    check(fk, x, np.where([1, 0, 1, 0, 0, 1], lost, -np.inf), 2, 3, 20)
+
+
+def test_masks_and_finished_beams(fk):
+    x, s = make(12, 8, 6000)
+    x[:, 3:] = LOWEST
+    f = np.array([0, 1, 0, 0, 1, 1, 0, 0])
+    check(fk, x, s, 2, 4, 16, finished=f, pad=5999)
+    s[1] = -3e38
+    check(fk, x, s, 2, 4, 16, finished=f, pad=2)
+
+
+def test_steps_under_a_mask(fk):
+    """The scores of one step are those of the next, as a search that may take one token a step has them."""
+    s = np.zeros(4, np.float32)
+    s[1:] = -np.inf
+    for step in range(5):
+        x, _ = make(40 + step, 4, 5000)
+        keep = x[:, 17 + step].copy()
+        x[:] = LOWEST
+        x[:, 17 + step] = keep
+        check(fk, x, s, 1, 4, 4)
+        s = select(fk, x, s, 1, 4, 4)[0][0]
+        assert s[0] == 0.0
