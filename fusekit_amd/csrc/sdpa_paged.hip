@@ -35,13 +35,21 @@ struct SdpaPagedArgs {
     uint32_t only_few;            // of chunks among single tokens: whole chunks, cut tokens (compact)
 };
 
+// Positions up to that of a sequence's new row `place`; 0: the row sees nothing.
+__device__ __forceinline__ uint32_t paged_limit(const PagedSeq& s, uint32_t place) { return s.len + place + 1u > s.rows ? s.len + place + 1u - s.rows : 0u; }
+
+// What sums of probabilities are multiplied with, l their total: 0 for a row that sees nothing, and not a number, which has the column done again by
+// paged_row, where l is not between bounds that it does not leave unless scores are beyond some 1e9: the reference, a rounded product, and the exponents,
+// each one rounding of product and reference, are then apart by more than fp32's exponents hold.
+__device__ __forceinline__ float paged_inverse(float l, uint32_t limit) { return l > 0x1p-60f && l < 0x1p60f ? 1.0f / l : limit ? __builtin_nanf("") : 0.f; }
+
 // ---- one row of one head by a wave: positions in the order they lie, what the row does not see is not touched ----
 // The statement of the operator as it stands; the tiles below come here for a column whose sums are not finite, since a zero
 // probability times an infinity that other rows of the tile see is no number.
 template <int D>
 __device__ __forceinline__ void paged_row(const SdpaPagedArgs& a, uint32_t seq, const PagedSeq& s, uint32_t place, uint32_t head, uint32_t lane) {
     const uint32_t kvh = head / a.group, row = s.row0 + place, page_rows = 1u << a.b.page_shift;
-    const uint32_t end = s.len + place + 1u > s.rows ? s.len + place + 1u - s.rows : 0u;   // positions up to the row's own
+    const uint32_t end = paged_limit(s, place);
     const uint32_t first = a.window && end > a.window ? end - a.window : 0u;
     const uint16_t* qr = a.q + (size_t)row * a.q_stride + (size_t)head * D;
     constexpr int DL = D / 64;
@@ -244,7 +252,7 @@ struct PagedRange {
 };
 template <uint32_t STEP>
 __device__ __forceinline__ PagedRange paged_range(const SdpaPagedArgs& a, const PagedItem& it, uint32_t e_tile, uint32_t e_last) {
-    auto limit_of = [&](uint32_t place) { return it.s.len + place + 1u > it.s.rows ? it.s.len + place + 1u - it.s.rows : 0u; };
+    auto limit_of = [&](uint32_t place) { return paged_limit(it.s, place); };
     PagedRange r;
     r.kv_end = __builtin_amdgcn_readfirstlane(limit_of(e_last / a.group));
     const uint32_t first = limit_of(e_tile / a.group);
@@ -325,7 +333,7 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kb = lane >> 5, nl = lane & 31u;
     const uint32_t G = a.group, columns = it.s.rows * G;   // (below 2^31: the host has checked)
     const uint32_t column_tile = SPLIT == 1 ? wave : wave & 1u, my_half = SPLIT == 1 ? 0u : wave >> 1;
-    auto limit_of = [&](uint32_t place) { return it.s.len + place + 1u > it.s.rows ? it.s.len + place + 1u - it.s.rows : 0u; };   // positions a row may see end here
+    auto limit_of = [&](uint32_t place) { return paged_limit(it.s, place); };                              // positions a row may see end here
     auto low_of = [&](uint32_t limit) { return a.window && limit > a.window ? limit - a.window : 0u; };                           // and begin here
     const uint32_t e_tile = it.tile * COLS, e_last = columns - e_tile < COLS ? columns - 1u : e_tile + COLS - 1u;
     const PagedRange range = paged_range<STEP>(a, it, e_tile, e_last);
@@ -537,7 +545,7 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
     float* const all = reinterpret_cast<float*>(lds_raw);
     float* const ob = all + wave * 32u * OS;
     const bool whole = n_active == 1u;
-    const float f = whole && SPLIT == 1 ? (l_run > 0.f || l_run != l_run ? 1.0f / l_run : 0.f) : 1.0f;   // (a row that sees nothing: zeros)
+    const float f = whole && SPLIT == 1 ? paged_inverse(l_run, q_limit) : 1.0f;
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -566,7 +574,7 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
             const uint32_t c = c0 + idx / (D / 4u), d = idx % (D / 4u) * 4u;
             join(c, w0, w1, m, l);
             if (whole) {
-                const float r = l > 0.f || l != l ? 1.0f / l : 0.f;
+                const float r = paged_inverse(l, limit_of((e0 + c) / G));
                 w0 *= r;
                 w1 *= r;
             }
@@ -663,9 +671,9 @@ __global__ __launch_bounds__(256) void sdpa_paged_merge_kernel(const SdpaPagedAr
     const uint32_t left = columns - e_tile, end = left < c0 + kMergeCols ? left : c0 + kMergeCols;
     bool odd = false;
     auto put = [&](uint32_t c, uint32_t d, const float4& o, float l) {
-        const float f = l > 0.f || l != l ? 1.0f / l : 0.f;   // (a row that sees nothing: zeros)
         const float t = (__builtin_fabsf(o.x) + __builtin_fabsf(o.y)) + (__builtin_fabsf(o.z) + __builtin_fabsf(o.w));
         const uint32_t e = e_tile + c, place = e / G;
+        const float f = paged_inverse(l, paged_limit(it.s, place));
         *reinterpret_cast<uint2*>(a.out + (size_t)(it.s.row0 + place) * a.out_stride + (size_t)(it.kvh * G + (e - place * G)) * D + d) =
             make_uint2(pack_bf16(o.x * f, o.y * f), pack_bf16(o.z * f, o.w * f));
         odd = !(t * f < INFINITY);
@@ -704,7 +712,7 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
 
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
     const uint32_t G = a.group, e0 = it.tile * kFewCols, left_cols = it.s.rows * G - e0, columns = left_cols < kFewCols ? left_cols : kFewCols;   // of this tile
-    auto limit_of = [&](uint32_t place) { return it.s.len + place + 1u > it.s.rows ? it.s.len + place + 1u - it.s.rows : 0u; };
+    auto limit_of = [&](uint32_t place) { return paged_limit(it.s, place); };
     auto low_of = [&](uint32_t limit) { return a.window && limit > a.window ? limit - a.window : 0u; };
     const PagedRange range = paged_range<kFewRound>(a, it, e0, e0 + columns - 1u);
     const uint32_t kv_end = range.kv_end, n_active = range.n_active, lim_lo = __builtin_amdgcn_readfirstlane(limit_of(e0 / G));
@@ -913,9 +921,9 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
     const bool whole = n_active == 1u;
     const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials, 0, (int)(a.slots * a.slot_bytes), 0x27000);
     auto store = [&](uint32_t c, uint32_t d, const float4& o, float l) {
-        const float f = l > 0.f || l != l ? 1.0f / l : 0.f;   // (a row that sees nothing: zeros)
         const float t = (__builtin_fabsf(o.x) + __builtin_fabsf(o.y)) + (__builtin_fabsf(o.z) + __builtin_fabsf(o.w));
         const uint32_t pl = (e0 + c) / G;
+        const float f = paged_inverse(l, limit_of(pl));
         *reinterpret_cast<uint2*>(a.out + (size_t)(it.s.row0 + pl) * a.out_stride + (size_t)(it.kvh * G + (e0 + c - pl * G)) * D + d) =
             make_uint2(pack_bf16(o.x * f, o.y * f), pack_bf16(o.z * f, o.w * f));
         if (!(t * f < INFINITY)) atomicOr(const_cast<uint32_t*>(&word[1]), 1u << c);
