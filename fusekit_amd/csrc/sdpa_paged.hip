@@ -13,9 +13,9 @@
 
 namespace fk {
 
-// Probabilities carry the factor 2^-32, which cancels: a sum of 2^16 times 2^8 of them times the type's largest values stays in
-// fp32's range (2^8: how far a step's maximum may lie above the softmax reference).
-constexpr float kSmallLog2 = 32.0f, kSmall = 0x1p-32f, kPagedLag = 8.0f;
+// Probabilities carry the factor 2^-8, which cancels, since a step's maximum may lie 2^8 above the softmax reference: values down to the type's smallest
+// keep their products in fp32's range, and sums of its largest that leave it are done again by paged_row, in 64 bits.
+constexpr float kPagedLag = 8.0f;
 constexpr float kLog2E = 1.44269504088896341f;
 
 struct SdpaPagedArgs {
@@ -54,9 +54,10 @@ __device__ __forceinline__ void paged_row(const SdpaPagedArgs& a, uint32_t seq, 
     const uint16_t* qr = a.q + (size_t)row * a.q_stride + (size_t)head * D;
     constexpr int DL = D / 64;
     uint32_t bad = 0;
-    float m = -INFINITY, l = 0.f, o[DL];
+    float m = -INFINITY;
+    double l = 0.0, o[DL];   // (values of the type's whole range, and 2^31 of the largest)
 #pragma unroll
-    for (int i = 0; i < DL; ++i) o[i] = 0.f;
+    for (int i = 0; i < DL; ++i) o[i] = 0.0;
     for (uint32_t at = first; at < end; at += 64u) {
         const uint32_t pos = at + lane < end ? at + lane : end - 1u;
         const uint32_t page = paged_page(a.b, seq, pos >> a.b.page_shift, bad);
@@ -73,8 +74,8 @@ __device__ __forceinline__ void paged_row(const SdpaPagedArgs& a, uint32_t seq, 
         x *= a.scale;
         if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
         if (at + lane >= end) x = -INFINITY;
-        const float m_new = fmaxf(m, wave_max(x)), ref = m_new == -INFINITY ? 0.f : m_new, alpha = expf(m - ref), p = expf(x - ref) * kSmall;
-        l = l * alpha + wave_sum(p);
+        const float m_new = fmaxf(m, wave_max(x)), ref = m_new == -INFINITY ? 0.f : m_new, alpha = expf(m - ref), p = expf(x - ref);
+        l = l * alpha + (double)wave_sum(p);
         m = m_new;
 #pragma unroll
         for (int i = 0; i < DL; ++i) o[i] *= alpha;
@@ -84,12 +85,12 @@ __device__ __forceinline__ void paged_row(const SdpaPagedArgs& a, uint32_t seq, 
             const float pj = __shfl(p, (int)j, 64);
             const size_t vb = __shfl((unsigned long long)base, (int)j, 64);
 #pragma unroll
-            for (int i = 0; i < DL; ++i) o[i] = fmaf(pj, bf16_bits_to_f32(a.v[vb + lane + 64u * i]), o[i]);
+            for (int i = 0; i < DL; ++i) o[i] = fma((double)pj, (double)bf16_bits_to_f32(a.v[vb + lane + 64u * i]), o[i]);
         }
     }
 #pragma unroll
     for (int i = 0; i < DL; ++i)
-        a.out[(size_t)row * a.out_stride + (size_t)head * D + lane + 64u * i] = (uint16_t)f32_to_bf16_bits(end > first ? o[i] / l : 0.f);
+        a.out[(size_t)row * a.out_stride + (size_t)head * D + lane + 64u * i] = (uint16_t)f32_to_bf16_bits(end > first ? (float)(o[i] / l) : 0.f);
 }
 
 // ---- which piece of the work a block does ----
@@ -493,7 +494,7 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
         for (int i = 1; i < 32; ++i) mt = fmaxf(mt, s[i / 16][i % 16]);
         mt = other_half_max(mt) * scale2;
         const bool grow = mt > m_run + kPagedLag;
-        const float m_new = grow ? mt : m_run, m_ref = m_new == -INFINITY ? 0.f : m_new, m_sub = m_ref + kSmallLog2;
+        const float m_new = grow ? mt : m_run, m_ref = m_new == -INFINITY ? 0.f : m_new, m_sub = m_ref + kPagedLag;
         const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_ref) : 1.0f;
         m_run = m_new;
         l_run *= alpha;
@@ -846,7 +847,7 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
 #pragma unroll
                 for (int i = 0; i < DT; ++i) acc[p][i] *= alpha;
         }
-        const float m_sub = (m_run == -INFINITY ? 0.f : m_run) + kSmallLog2;
+        const float m_sub = (m_run == -INFINITY ? 0.f : m_run) + kPagedLag;
         pf_u32x4_t pb[PARTS];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

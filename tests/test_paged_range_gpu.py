@@ -1,6 +1,6 @@
-"""Attention over a paged cache (fk_sdpa_paged) with scores of any size, against the statement in 64 bits.
+"""Attention over a paged cache (fk_sdpa_paged) with scores and values of any size, against the statement in 64 bits.
 
-A query and a key differ from 0 in their first dim only, so that a score is the product of two bf16 values, exact in fp32: what is left of the tolerance is the
+In the tests of scores a query and a key differ from 0 in their first dim only, so that a score is the product of two bf16 values, exact in fp32: what is left of the tolerance is the
 probabilities' rounding to bf16, 2^-8 of A = sum p |v| / sum p, that of the output, 2^-8 of it, and 2^-11 A for exponentials and sums in fp32."""
 import numpy as np
 import pytest
@@ -56,3 +56,30 @@ def test_a_row_that_sees_nothing_beside_large_scores(fk):
         assert bool((np.abs(wide(got) - ref) <= 2.0 ** -8 * np.abs(ref) + (2.0 ** -8 + 2.0 ** -11) * a).all())
         with pytest.raises(fk.InvalidArgument, match="length"):
             fk.paged_check(fault)
+
+
+@pytest.mark.parametrize("rows,lens,n_heads,n_kv,dim", SHAPES)
+@pytest.mark.parametrize("size", [1e-34, 1e-28, 1e30, 2e37])
+def test_values_of_any_size(fk, rows, lens, n_heads, n_kv, dim, size):
+    """Values near both ends of bf16's range, weighted by ordinary scores.  An fp32 score of `dim` products of values below 5 and 10, times dim^-1/2, is off
+    by less than 128 * 2^-24 * 128 * 50 * 0.09 / 30 = 1.5e-4 with the sums that normal values have: 2^-11 A with the sums' own rounding."""
+    p = Paged(rows, lens, n_kv, dim, 32, seed=10)
+    for i, n in enumerate(lens):
+        page, slot = p.where(i, np.arange(n))
+        p.v[page, :, slot] = oracle.f32_to_bf16((size * rng(11 + i).standard_normal((n, n_kv, dim))).astype(np.float32))
+    q, got, _ = attend(fk, p, n_heads)
+    ref, a = attention(p, q, n_heads, dim ** -0.5)
+    off = np.abs(wide(got) - ref) - (2.0 ** -8 * np.abs(ref) + (2.0 ** -8 + 2.0 ** -11) * a + 2.0 ** -126)   # (below the smallest normal number: to 0)
+    assert off.max() <= 0, off.max()
+
+
+@pytest.mark.parametrize("rows,lens,n_heads,n_kv,dim", SHAPES)
+def test_the_largest_values(fk, rows, lens, n_heads, n_kv, dim):
+    """Sums of probabilities times the type's largest values leave fp32, their average does not."""
+    p = Paged(rows, lens, n_kv, dim, 32, seed=12)
+    for i, n in enumerate(lens):
+        page, slot = p.where(i, np.arange(n))
+        p.v[page, :, slot] = np.where(np.arange(dim) % 3 == 0, 0xFF7F, 0x7F60)
+    q, got, _ = attend(fk, p, n_heads)
+    ref = np.broadcast_to(wide(np.where(np.arange(dim) % 3 == 0, 0xFF7F, 0x7F60).astype(np.uint16)), got.shape)
+    assert bool((np.abs(wide(got) / ref - 1) <= 2.0 ** -7 + 2.0 ** -11).all())   # the probabilities' rounding and the output's
