@@ -171,7 +171,9 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
     pairs = wave_sum(pairs);
     // (compact: a tile that is cut has more than one share, and fewer than twice as many items as shares: 2 target of them have slots)
     const bool compact = only_few || (!TILES && a.compact != 0 && !(pairs + (float)a.target <= (float)a.slots));
-    bool cut = compact || pairs + (float)a.target <= (float)a.slots;
+    // (a batch whose row_start falls can have more tiles than the host has counted: cut, the last items of a tile would be behind the launch's end,
+    // and its counter would never be left ready)
+    bool cut = pairs + (float)a.target <= (compact ? (float)gridDim.x : (float)a.slots);
     // (of at least work / target steps: all items together are at most target + pairs)
     const float share = work / (float)a.target;
     uint32_t unit = share < 0x1p30f ? (uint32_t)ceilf(share) : 1u << 30;
@@ -188,8 +190,9 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
     if (only_few) {
         longest_whole = wave_max(longest_whole);
         longest_cut = wave_max(longest_cut);
-        only_few = cut = longest_cut > 2.0f * longest_whole;
-        tokens = !only_few || wave_sum(wholes) + pairs > (float)a.target;
+        const float tiles = wave_sum(wholes) + pairs;
+        only_few = cut = longest_cut > 2.0f * longest_whole && tiles + (float)a.target <= (float)gridDim.x;
+        tokens = !only_few || tiles > (float)a.target;
     }
     bool second = !only_few;
     if (many && !once) from_the_first();

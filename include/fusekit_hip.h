@@ -595,7 +595,7 @@ enum {
     FK_PAGED_BAD_PAGE = 4               /* a page id that the pool does not have */
 };
 /* Synchronises the stream; FK_ERR_INVALID with a message where *fault is set, which is then zeroed.  What the launches
- * since the last check wrote for the sequence at fault is undefined (inside its own rows and pages). */
+ * since the last check wrote for the sequence at fault is undefined (inside its own rows and pages); workspaces are left ready. */
 fk_status fk_paged_check(uint32_t *fault, fk_stream s);
 
 /* Rotary frequencies of one model as fk_rope_paged_store takes them, in 64 bits: d_freq[i], i < dims / 2, is how many
