@@ -242,7 +242,6 @@ constexpr uint32_t kPagePairs = 480;
 struct PagesCopyArgs {
     unsigned char* base;
     size_t plane_stride, page_bytes;
-    uint32_t n_pairs;
     uint32_t pairs[2 * kPagePairs];
 };
 __global__ __launch_bounds__(256) void pages_copy_kernel(const PagesCopyArgs a) {
@@ -287,11 +286,11 @@ fk_status run_pages_copy(void* base, uint32_t n_planes, size_t plane_stride, uin
     a.plane_stride = plane_stride;
     a.page_bytes = page_bytes;
     for (uint32_t at = 0; at < n_pairs; at += kPagePairs) {
-        a.n_pairs = std::min(kPagePairs, n_pairs - at);
-        memcpy(a.pairs, pairs + 2 * (size_t)at, (size_t)a.n_pairs * 8);
+        const uint32_t n = std::min(kPagePairs, n_pairs - at);
+        memcpy(a.pairs, pairs + 2 * (size_t)at, (size_t)n * 8);
         const uint32_t parts = (uint32_t)std::min<size_t>((page_bytes / 16 + 255) / 256, 64);
         void* params[1] = {&a};
-        FK_HIP(hipLaunchKernel(reinterpret_cast<const void*>(&pages_copy_kernel), dim3(a.n_pairs, n_planes, parts), dim3(256), params, 0, s));
+        FK_HIP(hipLaunchKernel(reinterpret_cast<const void*>(&pages_copy_kernel), dim3(n, n_planes, parts), dim3(256), params, 0, s));
     }
     return FK_OK;
 }

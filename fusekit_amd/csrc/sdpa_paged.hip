@@ -24,7 +24,7 @@ struct SdpaPagedArgs {
     const uint16_t* k;
     const uint16_t* v;
     uint16_t* out;
-    uint32_t q_stride, out_stride, n_heads, group;
+    uint32_t q_stride, out_stride, group;
     uint32_t window;
     float scale, softcap;
     float* partials;       // [slots][columns of a tile][D], then (m, l) [slots][columns of a tile]
@@ -267,26 +267,27 @@ __device__ __forceinline__ PagedRange paged_range(const SdpaPagedArgs& a, const 
     return r;
 }
 
-// What a wave hands on of 32 columns, `live` of them, et the first: outputs, or where the tile is cut the sums as they are, the reference and the sum of the
-// probabilities into this item's slot (`c0`: the first column's place there).  ob: [32][D + 4] in LDS, outputs or sums.
+// What a wave hands on of up to 32 columns, `live` of them, et the first, from ob, [32][D + 4] in LDS.  Where the tile is cut: the sums as they are, the reference and
+// the sum of the probabilities into this item's slot (`c0`: the first column's place there).
 template <int D>
-__device__ __forceinline__ void paged_hand_on(const SdpaPagedArgs& a, const PagedItem& it, const float* ob, uint32_t et, uint32_t c0, uint32_t live, bool whole, float m,
-                                              float l, uint32_t lane) {
+__device__ __forceinline__ void paged_store_part(const SdpaPagedArgs& a, const PagedItem& it, const float* ob, uint32_t c0, uint32_t live, float m, float l, uint32_t lane) {
+    constexpr uint32_t OS = D + 4;
+    const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials + (size_t)it.slot * (kTileCols * (D + 2u)), 0, (int)(kTileCols * (D + 2u) * 4u), 0x27000);
+    for (uint32_t idx = lane; idx < live * (uint32_t)(D / 4); idx += 64u) {
+        const uint32_t col = idx / (uint32_t)(D / 4), pc = idx % (uint32_t)(D / 4);
+        const pf_u32x4_t v = *reinterpret_cast<const pf_u32x4_t*>(ob + col * OS + pc * 4u);
+        __builtin_amdgcn_raw_buffer_store_b128(v, mem, (int)(((c0 + col) * D + pc * 4u) * 4u), 0, 0);
+    }
+    if (lane < live) {   // (the lanes below 32 hold all of a column's l)
+        const pf_u32x2_t ml = {__float_as_uint(m), __float_as_uint(l)};
+        __builtin_amdgcn_raw_buffer_store_b64(ml, mem, (int)((kTileCols * D + (c0 + lane) * 2u) * 4u), 0, 0);
+    }
+}
+// Where it is whole: outputs.
+template <int D>
+__device__ __forceinline__ void paged_store_columns(const SdpaPagedArgs& a, const PagedItem& it, const float* ob, uint32_t et, uint32_t live, uint32_t lane) {
     constexpr uint32_t OS = D + 4, VP = D / 8;
     const uint32_t G = a.group;
-    if (!whole) {
-        const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials + (size_t)it.slot * (kTileCols * (D + 2u)), 0, (int)(kTileCols * (D + 2u) * 4u), 0x27000);
-        for (uint32_t idx = lane; idx < live * (uint32_t)(D / 4); idx += 64u) {
-            const uint32_t col = idx / (uint32_t)(D / 4), pc = idx % (uint32_t)(D / 4);
-            const pf_u32x4_t v = *reinterpret_cast<const pf_u32x4_t*>(ob + col * OS + pc * 4u);
-            __builtin_amdgcn_raw_buffer_store_b128(v, mem, (int)(((c0 + col) * D + pc * 4u) * 4u), 0, 0);
-        }
-        if (lane < live) {   // (the lanes below 32 hold all of a column's l)
-            const pf_u32x2_t ml = {__float_as_uint(m), __float_as_uint(l)};
-            __builtin_amdgcn_raw_buffer_store_b64(ml, mem, (int)((kTileCols * D + (c0 + lane) * 2u) * 4u), 0, 0);
-        }
-        return;
-    }
     uint32_t again = 0;   // columns whose sums are not finite, done again one by one
     for (uint32_t base = 0; base < live * VP; base += 64u) {
         const uint32_t idx = base + lane, col = idx / VP, pc = idx % VP;
@@ -548,7 +549,7 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
     constexpr uint32_t OS = D + 4;
     float* const all = reinterpret_cast<float*>(lds_raw);
     float* const ob = all + wave * 32u * OS;
-    const bool whole = n_active == 1u;
+    const bool whole = n_active == 1u;   // (tiles of 64 columns are never cut)
     const float f = whole && SPLIT == 1 ? paged_inverse(l_run, q_limit) : 1.0f;
 #pragma unroll
     for (int i = 0; i < DT; ++i)
@@ -558,36 +559,27 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
                 make_float4(oacc[i][4 * g + 0] * f, oacc[i][4 * g + 1] * f, oacc[i][4 * g + 2] * f, oacc[i][4 * g + 3] * f);
     if constexpr (SPLIT == 1) {
         wave_lds_order();
-        paged_hand_on<D>(a, it, ob, e0, wave * 32u, live, whole, m_run, l_run, lane);
+        if (whole) paged_store_columns<D>(a, it, ob, e0, live, lane);
+        else paged_store_part<D>(a, it, ob, wave * 32u, live, m_run, l_run, lane);
     } else {   // the two waves of a column tile join their halves, 16 columns each
         float* const ml = all + 4u * 32u * OS;   // [wave][column] reference, sum
         if (kb == 0) *reinterpret_cast<float2*>(ml + (wave * 32u + nl) * 2u) = make_float2(m_run, l_run);
         __syncthreads();
         const uint32_t c0 = my_half * 16u, mine = live > c0 ? (live - c0 < 16u ? live - c0 : 16u) : 0u;
         const float* const other = all + (wave ^ 2u) * 32u * OS;
-        auto join = [&](uint32_t c, float& w0, float& w1, float& m, float& l) {
-            const float2 x = *reinterpret_cast<const float2*>(ml + (wave * 32u + c) * 2u), y = *reinterpret_cast<const float2*>(ml + ((wave ^ 2u) * 32u + c) * 2u);
-            m = fmaxf(x.x, y.x);
-            const float ref = m == -INFINITY ? 0.f : m;
-            w0 = __builtin_amdgcn_exp2f(x.x - ref);
-            w1 = __builtin_amdgcn_exp2f(y.x - ref);
-            l = fmaf(x.y, w0, y.y * w1);
-        };
-        float w0, w1, m, l;
         for (uint32_t idx = lane; idx < 16u * (D / 4u); idx += 64u) {
             const uint32_t c = c0 + idx / (D / 4u), d = idx % (D / 4u) * 4u;
-            join(c, w0, w1, m, l);
-            if (whole) {
-                const float r = paged_inverse(l, limit_of((e0 + c) / G));
-                w0 *= r;
-                w1 *= r;
-            }
-            const float4 x = *reinterpret_cast<const float4*>(ob + c * OS + d), y = *reinterpret_cast<const float4*>(other + c * OS + d);
-            *reinterpret_cast<float4*>(ob + c * OS + d) = make_float4(fmaf(x.x, w0, y.x * w1), fmaf(x.y, w0, y.y * w1), fmaf(x.z, w0, y.z * w1), fmaf(x.w, w0, y.w * w1));
+            const float2 x = *reinterpret_cast<const float2*>(ml + (wave * 32u + c) * 2u), y = *reinterpret_cast<const float2*>(ml + ((wave ^ 2u) * 32u + c) * 2u);
+            const float m = fmaxf(x.x, y.x), ref = m == -INFINITY ? 0.f : m;
+            float w0 = __builtin_amdgcn_exp2f(x.x - ref), w1 = __builtin_amdgcn_exp2f(y.x - ref);
+            const float r = paged_inverse(fmaf(x.y, w0, y.y * w1), limit_of((e0 + c) / G));
+            w0 *= r;
+            w1 *= r;
+            const float4 u = *reinterpret_cast<const float4*>(ob + c * OS + d), v = *reinterpret_cast<const float4*>(other + c * OS + d);
+            *reinterpret_cast<float4*>(ob + c * OS + d) = make_float4(fmaf(u.x, w0, v.x * w1), fmaf(u.y, w0, v.y * w1), fmaf(u.z, w0, v.z * w1), fmaf(u.w, w0, v.w * w1));
         }
-        join(c0 + (lane & 15u), w0, w1, m, l);
         wave_lds_order();
-        paged_hand_on<D>(a, it, ob + c0 * OS, e0 + c0, column_tile * 32u + c0, mine, whole, m, l, lane);
+        paged_store_columns<D>(a, it, ob + c0 * OS, e0 + c0, mine, lane);
     }
 }
 
@@ -1071,7 +1063,7 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     const DeviceFacts* dev;
     FK_TRY(device_facts(&dev));
     a.q = q; a.k = pool->k; a.v = pool->v; a.out = out;
-    a.q_stride = q_stride; a.out_stride = out_stride; a.n_heads = n_heads; a.group = n_heads / n_kv;
+    a.q_stride = q_stride; a.out_stride = out_stride; a.group = n_heads / n_kv;
     a.window = window; a.scale = scale; a.softcap = softcap;
     a.counters = static_cast<uint32_t*>(workspace);
     a.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kPagedCounterBytes);
