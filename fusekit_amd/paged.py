@@ -137,6 +137,12 @@ class PageAllocator:
         return t
 
 
+def largest_rows(most: int) -> List[int]:
+    """Row counts whose qgemm workspaces serve all counts up to `most`: the split of k differs between the forms of up to 32, up to 64 and more rows and
+    with the number of 128-row tiles, so that more rows can need less."""
+    return sorted({most, *(m for m in (32, 64) if m < most), *range(128, most, 128)})
+
+
 class PagedDecoder:
     """A dense decoder over pages.  forward() takes any mix of sequences, each with its new tokens, and leaves the logits behind the last token
     of each."""
@@ -173,10 +179,8 @@ class PagedDecoder:
         self.logits = DeviceBuffer(S * c.vocab * 2)
         g = 0 if c.bits == 16 else c.group
         shapes = ((c.n_q + 2 * c.n_kvd, c.hidden), (c.hidden, c.n_q), (c.inter, c.hidden), (c.hidden, c.inter))
-        rows = {R, *(v for v in (*range(512, 4096, 128), 384, 256, 128, 64, 32) if v < R)}
-        ws = max(native.qgemm_workspace_bytes(m, n, k, g) for m in rows for n, k in shapes)
-        seqs = {S, *(v for v in (384, 256, 128, 64, 32) if v < S)}
-        ws = max(2 * ws, max(native.qgemm_workspace_bytes(m, c.vocab, c.hidden, 0 if self.head.bits == 16 else self.head.group) for m in seqs))
+        ws = max(native.qgemm_workspace_bytes(m, n, k, g) for m in largest_rows(R) for n, k in shapes)
+        ws = max(2 * ws, max(native.qgemm_workspace_bytes(m, c.vocab, c.hidden, 0 if self.head.bits == 16 else self.head.group) for m in largest_rows(S)))
         self.ws = DeviceBuffer(ws)
         self.sdpa_ws = native.zeros(native.SDPA_PAGED_WORKSPACE_MOST)
 
