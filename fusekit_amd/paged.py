@@ -153,6 +153,16 @@ class PagedDecoder:
         """rope: scaling and its numbers as native.rope_frequencies takes them; window, softcap: of every layer."""
         if cfg.kv_bits:
             raise ValueError("pages hold a bf16 cache")
+        if cfg.head_dim not in (64, 128) or cfg.n_kv < 1 or cfg.n_heads % cfg.n_kv:
+            raise ValueError("paged attention takes heads of 64 or 128 dims, and as many query heads for each KV head")
+        if not 16 <= page_rows <= 1024 or page_rows & (page_rows - 1):
+            raise ValueError("page_rows: a power of two from 16 to 1024")
+        if min(n_pages, max_rows, max_seqs) < 1:
+            raise ValueError("a decoder has pages, rows and sequences")
+        if rope_dims is not None and (rope_dims % 16 or not 0 <= rope_dims <= cfg.head_dim):
+            raise ValueError("rope_dims: a multiple of 16 up to head_dim, or 0")
+        if not 0 <= window < 1 << 31 or not 0.0 <= softcap <= 1024.0:
+            raise ValueError("window and softcap are not negative, softcap up to 1024 (0: none)")
         self.cfg, self.w, self.stream = cfg, weights, stream
         self.pages = PageAllocator(n_pages, page_rows)
         self.max_rows, self.max_seqs, self.window, self.softcap = max_rows, max_seqs, window, softcap

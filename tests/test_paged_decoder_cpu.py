@@ -12,3 +12,15 @@ def test_workspaces_are_sized_for_every_count_of_rows(most):
     for m in range(1, most + 1):
         edge = 32 if m <= 32 else 64 if m <= 64 else -(-m // 128) * 128
         assert min(edge, most) in counts
+
+
+@pytest.mark.parametrize("cfg,change", [(dict(kv_bits=8), {}), (dict(head_dim=96), {}), (dict(head_dim=256), {}), (dict(n_heads=6), {}), ({}, dict(page_rows=8)),
+                                        ({}, dict(page_rows=48)), ({}, dict(page_rows=2048)), ({}, dict(page_rows=0)), ({}, dict(n_pages=0)), ({}, dict(max_rows=0)),
+                                        ({}, dict(max_seqs=-1)), ({}, dict(rope_dims=8)), ({}, dict(rope_dims=80)), ({}, dict(rope_dims=-16)), ({}, dict(window=-1)),
+                                        ({}, dict(softcap=-1.0)), ({}, dict(softcap=2000.0)), ({}, dict(softcap=float("nan")))], ids=str)
+def test_what_the_operators_do_not_take_is_refused_at_once(cfg, change):
+    from fusekit_amd.decoder import DecoderConfig
+    from fusekit_amd.paged import PagedDecoder
+    c = DecoderConfig(**{**dict(n_layers=1, hidden=256, n_heads=4, n_kv=4, head_dim=64, inter=256, vocab=100), **cfg})
+    with pytest.raises(ValueError):
+        PagedDecoder(c, None, **{**dict(n_pages=4, page_rows=16), **change})
