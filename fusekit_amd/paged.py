@@ -98,6 +98,18 @@ class PageAllocator:
             seq.length += r
         return copies
 
+    def restore(self, seqs: Sequence[PagedSequence], held: Sequence[Tuple[List[int], int]]) -> None:
+        """Takes an extend() of `seqs` back: held[i] is (list(seqs[i].pages), seqs[i].length) from before it, and nothing else has happened since."""
+        for seq, (pages, length) in reversed(list(zip(seqs, held))):
+            for i in reversed(range(len(seq.pages))):
+                if i < len(pages) and pages[i] == seq.pages[i]:
+                    continue
+                self.users[seq.pages[i]] = 0
+                self._free.append(seq.pages[i])
+                if i < len(pages):                             # the tail that others see too
+                    self.users[pages[i]] += 1
+            seq.pages, seq.length = list(pages), length
+
     def _take(self) -> int:
         page = self._free.pop()
         self.users[page] = 1
@@ -195,8 +207,9 @@ class PagedDecoder:
         self.sdpa_ws = native.zeros(native.SDPA_PAGED_WORKSPACE_MOST)
 
     def forward(self, batch: Sequence[Tuple[PagedSequence, Sequence[int]]]) -> DeviceBuffer:
-        """Each sequence takes its new tokens (one at least); returns the logits [len(batch), vocab], overwritten by the next call."""
-        c, w, st = self.cfg, self.w, self.stream
+        """Each sequence takes its new tokens (one at least); returns the logits [len(batch), vocab], overwritten by the next call.  A call that raises
+        leaves the sequences as they were."""
+        c = self.cfg
         seqs, tokens = [s for s, _ in batch], [list(t) for _, t in batch]
         n, rows = len(seqs), [len(t) for t in tokens]
         R = sum(rows)
@@ -205,8 +218,19 @@ class PagedDecoder:
         flat = [t for ts in tokens for t in ts]
         if min(flat) < 0 or max(flat) >= c.vocab:
             raise ValueError("a token outside of the vocabulary")
+        held = [(list(s.pages), s.length) for s in seqs]
         copies = self.pages.extend(seqs, rows)
-        self.copy_pages(copies)
+        try:
+            self.copy_pages(copies)
+            return self._launch(seqs, rows, flat)
+        except BaseException:
+            self.pages.restore(seqs, held)
+            raise
+
+    def _launch(self, seqs: List[PagedSequence], rows: List[int], flat: List[int]) -> DeviceBuffer:
+        """The launches of forward(), for sequences that have room for their rows."""
+        c, w, st = self.cfg, self.w, self.stream
+        n, R = len(seqs), len(flat)
         starts = np.concatenate([[0], np.cumsum(rows)])
         stride = max(len(s.pages) for s in seqs)
         words = np.concatenate([starts, [s.length for s in seqs], flat, self.pages.table(seqs, stride).ravel()]).astype(np.uint32)
@@ -253,12 +277,18 @@ class PagedDecoder:
         return len(copies)
 
     def prefill(self, seq: PagedSequence, prompt: Sequence[int]) -> DeviceBuffer:
-        """A prompt in chunks of max_rows tokens; the logits behind its last token are the first row."""
-        prompt = list(prompt)
+        """A prompt in chunks of max_rows tokens; the logits behind its last token are the first row.  A call that raises leaves the sequence at the
+        positions that it had."""
+        prompt, before = list(prompt), seq.length
         if not prompt:
             raise ValueError("empty prompt")
-        for i in range(0, len(prompt), self.max_rows):
-            logits = self.forward([(seq, prompt[i:i + self.max_rows])])
+        try:
+            for i in range(0, len(prompt), self.max_rows):
+                logits = self.forward([(seq, prompt[i:i + self.max_rows])])
+        except BaseException:
+            if seq.live and seq.length > before:
+                self.pages.truncate(seq, before)
+            raise
         return logits
 
     def beam_search(self, prompt: Sequence[int], beams: int, max_tokens: int, eos: Optional[int] = None) -> List[Tuple[List[int], float]]:

@@ -1,4 +1,5 @@
 """PagedDecoder on the host: what it sizes and what it refuses before a device is asked for anything."""
+import numpy as np
 import pytest
 
 from fusekit_amd.paged import largest_rows
@@ -24,3 +25,24 @@ def test_what_the_operators_do_not_take_is_refused_at_once(cfg, change):
     c = DecoderConfig(**{**dict(n_layers=1, hidden=256, n_heads=4, n_kv=4, head_dim=64, inter=256, vocab=100), **cfg})
     with pytest.raises(ValueError):
         PagedDecoder(c, None, **{**dict(n_pages=4, page_rows=16), **change})
+
+
+def test_an_extension_taken_back_leaves_the_pool_as_it_was():
+    from fusekit_amd.paged import PageAllocator
+    a, rng = PageAllocator(120, 4), np.random.Generator(np.random.PCG64(2))
+    live = [a.new() for _ in range(3)]
+    for step in range(300):
+        live = live[:6] + [a.fork(live[int(rng.integers(0, len(live)))])]
+        before = a.users.copy(), list(a._free), [(list(s.pages), s.length) for s in live]
+        some = [live[i] for i in rng.permutation(len(live))[:int(rng.integers(1, len(live) + 1))]]
+        rows = rng.integers(0, 7, len(some))
+        held = [(list(s.pages), s.length) for s in some]
+        a.extend(some, rows)
+        a.restore(some, held)
+        assert (a.users == before[0]).all() and a._free == before[1] and [(s.pages, s.length) for s in live] == before[2]
+        a.extend(some, rows)
+        for s in live[6:]:
+            a.release(s)
+        live = live[:6]
+        for s in live:
+            a.truncate(s, min(s.length, int(rng.integers(0, 50))))

@@ -1,0 +1,62 @@
+"""PagedDecoder when a call fails: sequences and pages are as they were, and the next call is sound."""
+import numpy as np
+import pytest
+
+from helpers import rng
+from test_paged_decoder_gpu import models, paged  # noqa: F401 (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def state(d, *seqs):
+    return d.pages.users.tolist(), d.pages.free_pages, [(list(s.pages), s.length) for s in seqs]
+
+
+def rows(d, cfg, n):
+    return d.logits.to_numpy(np.uint16)[:n * cfg.vocab].reshape(n, cfg.vocab)
+
+
+@pytest.mark.parametrize("name,nth", [("rope_paged_store", 0), ("sdpa_paged", 1), ("qgemm", 3), ("pages_copy", 0), ("rmsnorm_rows", 4)])
+def test_a_launch_that_is_refused(fk, models, monkeypatch, name, nth):  # noqa: F811
+    cfg, d = paged(models, "norms")
+    text = rng(3).integers(0, cfg.vocab, 60).tolist()
+    a = d.pages.new()
+    d.forward([(a, text[:21])])
+    b = d.pages.fork(a)                                       # both are about to write into the page that they share
+    batch = [(a, text[21:40]), (b, text[40:43])]
+    before, calls, real = state(d, a, b), [0], getattr(fk, name)
+
+    def fails(*args, **more):
+        calls[0] += 1
+        if calls[0] > nth:
+            raise fk.InvalidArgument(fk.FK_ERR_INVALID, "refused")
+        return real(*args, **more)
+
+    with monkeypatch.context() as m:
+        m.setattr(fk, name, fails)
+        with pytest.raises(fk.InvalidArgument, match="refused"):
+            d.forward(batch)
+    assert state(d, a, b) == before
+    d.forward(batch)
+    fk.paged_check(d.fault)
+    got = rows(d, cfg, 2)
+    e = paged(models, "norms")[1]
+    x, y = e.pages.new(), e.pages.new()
+    e.forward([(x, text[:21])])
+    e.forward([(y, text[:21])])
+    e.forward([(x, text[21:40]), (y, text[40:43])])
+    fk.sync()
+    assert np.array_equal(got, rows(e, cfg, 2))
+
+
+def test_a_prompt_that_does_not_fit(fk, models):  # noqa: F811
+    from fusekit_amd.paged import OutOfPages
+    cfg, d = paged(models, "norms", n_pages=6, max_rows=40)
+    s = d.pages.new()
+    d.forward([(s, [1, 2, 3])])
+    before = state(d, s)
+    with pytest.raises(OutOfPages):
+        d.prefill(s, [5] * 100)                               # two chunks of 40 fit, the third does not
+    assert state(d, s) == before
+    d.prefill(s, [5] * 60)
+    assert s.length == 63
