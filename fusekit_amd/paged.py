@@ -296,6 +296,8 @@ class PagedDecoder:
         takes `eos` (its last token then) goes on unchanged.  Pages are shared as far as the beams' pasts are the same."""
         if not 1 <= beams <= min(64, self.max_seqs) or max_tokens < 1 or beams > self.cfg.vocab:
             raise ValueError("beams: 1 to 64, max_seqs and the vocabulary at most, and a token at least")
+        if beams > self.max_rows and max_tokens > 1:
+            raise ValueError("a step takes a row for every beam: max_rows at most")
         c, st = self.cfg, self.stream
         u32 = lambda a: np.asarray(a, dtype=np.uint32)
         ws = native.zeros(max(native.beam_select_workspace_bytes(1, b, c.vocab, beams) for b in (1, beams)))
@@ -347,9 +349,12 @@ class PagedDecoder:
     def generate(self, prompts: Sequence[Sequence[int]], max_tokens: int) -> List[List[int]]:
         """Greedy continuations of several prompts, decoded together."""
         c, st = self.cfg, self.stream
+        prompts = [list(p) for p in prompts]
         n = len(prompts)
-        if not 0 < n <= self.max_seqs or max_tokens < 1:
-            raise ValueError("one prompt at least, max_seqs at most, and a token at least")
+        if not 0 < n <= self.max_seqs or max_tokens < 1 or not all(prompts):
+            raise ValueError("one prompt at least, max_seqs at most, none empty, and a token at least")
+        if n > self.max_rows and max_tokens > 1:
+            raise ValueError("a step takes a row for every prompt: max_rows at most")
         ws = native.zeros(max(native.beam_select_workspace_bytes(g, 1, c.vocab, 1) for g in range(1, n + 1)))
         zero, chosen = native.zeros(4 * n), DeviceBuffer(12 * n)
         out = [chosen.ptr + 4 * n * i for i in range(3)]

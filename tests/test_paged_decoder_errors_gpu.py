@@ -60,3 +60,14 @@ def test_a_prompt_that_does_not_fit(fk, models):  # noqa: F811
     assert state(d, s) == before
     d.prefill(s, [5] * 60)
     assert s.length == 63
+
+
+def test_more_beams_or_prompts_than_rows_of_a_pass_are_refused_before_any_work(fk, models, monkeypatch):  # noqa: F811
+    cfg, d = paged(models, "norms", max_rows=4, max_seqs=8)
+    monkeypatch.setattr(d, "forward", lambda batch: pytest.fail("a pass was run"))
+    for bad in (lambda: d.beam_search([1, 2], 5, 3), lambda: d.generate([[1]] * 5, 2), lambda: d.generate([[1], []], 2)):
+        with pytest.raises(ValueError):
+            bad()
+    monkeypatch.undo()
+    assert len(d.beam_search([1, 2], 5, 1)) == 5 and len(d.generate([[1]] * 5, 1)) == 5      # (a first token takes no step)
+    assert len(d.beam_search([1, 2], 4, 2)) == 4 and len(d.generate([[1]] * 4, 2)) == 4 and d.pages.free_pages == 64
