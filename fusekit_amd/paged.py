@@ -208,7 +208,8 @@ class PagedDecoder:
 
     def forward(self, batch: Sequence[Tuple[PagedSequence, Sequence[int]]]) -> DeviceBuffer:
         """Each sequence takes its new tokens (one at least); returns the logits [len(batch), vocab], overwritten by the next call.  A call that raises
-        leaves the sequences as they were."""
+        leaves the sequences as they were.  Does not wait for the device: what a launch finds wrong in a batch is in `fault`, for native.paged_check
+        (beam_search and generate look at every step)."""
         c = self.cfg
         seqs, tokens = [s for s, _ in batch], [list(t) for _, t in batch]
         n, rows = len(seqs), [len(t) for t in tokens]
@@ -316,7 +317,7 @@ class PagedDecoder:
                 if step:
                     native.beam_reorder(history, history, 4 * max_tokens, out[1], 1, beams, beams, st)
                 native.beam_reorder(out[2], history.ptr + 4 * step, 4, same, 1, beams, beams, st, dst_stride=4 * max_tokens)
-                native.sync(st)
+                native.paged_check(self.fault, st)                 # (waits for the stream)
                 total, parent, token = chosen.to_numpy(np.uint32, (3, beams))
                 grown = [not over[p] for p in parent]
                 over = [over[p] or (eos is not None and int(t) == eos) for p, t in zip(parent, token)]
@@ -361,7 +362,7 @@ class PagedDecoder:
 
         def best(logits: DeviceBuffer, rows: int) -> List[int]:
             native.beam_select(logits, c.vocab, zero, None, 0, rows, 1, c.vocab, 1, *out, ws, ws.nbytes, st)
-            native.sync(st)
+            native.paged_check(self.fault, st)                     # (waits for the stream)
             return [int(t) for t in chosen.to_numpy(np.uint32, (3, n))[2, :rows]]
 
         seqs = [self.pages.new() for _ in prompts]

@@ -71,3 +71,13 @@ def test_more_beams_or_prompts_than_rows_of_a_pass_are_refused_before_any_work(f
     monkeypatch.undo()
     assert len(d.beam_search([1, 2], 5, 1)) == 5 and len(d.generate([[1]] * 5, 1)) == 5      # (a first token takes no step)
     assert len(d.beam_search([1, 2], 4, 2)) == 4 and len(d.generate([[1]] * 4, 2)) == 4 and d.pages.free_pages == 64
+
+
+@pytest.mark.parametrize("call", [lambda d: d.beam_search([1, 2], 2, 3), lambda d: d.generate([[1], [2, 3]], 3)])
+def test_what_a_launch_reports_is_raised(fk, models, call):  # noqa: F811
+    cfg, d = paged(models, "norms")
+    want = call(d)
+    d.fault.upload(np.array([2], np.uint32))                  # as a launch that meets a bad length sets it
+    with pytest.raises(fk.InvalidArgument, match="length"):
+        call(d)
+    assert d.pages.free_pages == 64 and call(d) == want
