@@ -60,6 +60,11 @@ def main() -> int:
 
     if args.cmd == "bench":
         return bench_cli.run(args)
+    if args.cmd == "generate":
+        if not 0 <= args.beams <= 64:
+            ap.error("--beams: 1 to 64")
+        if args.eos is not None and not args.beams:
+            ap.error("--eos ends the continuations of a beam search: it goes with --beams")
     from . import native as fk
     if args.cmd == "info":
         t = fk.target_describe()

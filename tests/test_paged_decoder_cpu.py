@@ -1,4 +1,7 @@
 """PagedDecoder on the host: what it sizes and what it refuses before a device is asked for anything."""
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -46,3 +49,9 @@ def test_an_extension_taken_back_leaves_the_pool_as_it_was():
         live = live[:6]
         for s in live:
             a.truncate(s, min(s.length, int(rng.integers(0, 50))))
+
+
+@pytest.mark.parametrize("options,word", [(["--beams", "-1"], "1 to 64"), (["--beams", "65"], "1 to 64"), (["--eos", "3"], "--beams")])
+def test_commands_that_beam_search_does_not_take(options, word):
+    r = subprocess.run([sys.executable, "-m", "fusekit_amd", "generate", "--model", "nowhere", "--ids", "1", *options], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 2 and word in r.stderr
