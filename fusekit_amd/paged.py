@@ -272,9 +272,17 @@ class PagedDecoder:
             native.pages_copy(self.pool, 2 * self.cfg.n_layers, self.plane_bytes, self.pages.n_pages, self.page_bytes, copies, self.stream)
 
     def compact(self) -> int:
-        """Moves the pages in use to the front of the pool; returns how many were moved."""
-        copies = self.pages.compact()
-        self.copy_pages(copies)
+        """Moves the pages in use to the front of the pool; returns how many were moved.  A call that raises leaves the sequences as they were."""
+        a = self.pages
+        held = a.users.copy(), list(a._free), [(s, s.pages) for s in a._sequences.values()]
+        copies = a.compact()
+        try:
+            self.copy_pages(copies)
+        except BaseException:
+            a.users, a._free = held[0], held[1]
+            for seq, pages in held[2]:
+                seq.pages = pages
+            raise
         return len(copies)
 
     def prefill(self, seq: PagedSequence, prompt: Sequence[int]) -> DeviceBuffer:

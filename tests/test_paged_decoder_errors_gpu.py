@@ -81,3 +81,25 @@ def test_what_a_launch_reports_is_raised(fk, models, call):  # noqa: F811
     with pytest.raises(fk.InvalidArgument, match="length"):
         call(d)
     assert d.pages.free_pages == 64 and call(d) == want
+
+
+def test_a_compaction_that_is_refused(fk, models, monkeypatch):  # noqa: F811
+    cfg, d = paged(models, "norms")
+    text = rng(4).integers(0, cfg.vocab, 50).tolist()
+    a, b = d.pages.new(), d.pages.new()
+    d.forward([(a, text[:40]), (b, text)])
+    c = d.pages.fork(b)
+    d.pages.release(a)
+    before, free = state(d, b, c), list(d.pages._free)
+
+    def fails(*args, **more):
+        raise fk.InvalidArgument(fk.FK_ERR_INVALID, "refused")
+    with monkeypatch.context() as m:
+        m.setattr(fk, "pages_copy", fails)
+        with pytest.raises(fk.InvalidArgument, match="refused"):
+            d.compact()
+    assert state(d, b, c) == before and d.pages._free == free
+    first = d.forward([(c, [7])]).to_numpy(np.uint16)[:cfg.vocab]
+    assert d.compact() > 0
+    fk.sync()
+    assert np.array_equal(d.forward([(b, [7])]).to_numpy(np.uint16)[:cfg.vocab], first)
