@@ -657,7 +657,8 @@ fk_status fk_pages_copy(void *base, uint32_t n_planes, size_t plane_stride, uint
  * size count as what they are, masks of the type's lowest value among them; inside a beam the order is that of the logits, also where
  * its score is so large that the sums do not tell them apart (sums beyond fp32 are listed in their order, as -inf).  A NaN
  * logit counts as -inf, a score that is not a number likewise.  Where fewer than k continuations are above -inf, the
- * lowest b * vocab + t that are left follow with -inf.  out_* [groups, k]; beams and k up to 64, groups up to 4096, groups * beams
+ * lowest b * vocab + t that are left follow with -inf.  out_* [groups, k], apart from the inputs, but that out_scores may be scores
+ * where k is beams; beams and k up to 64, groups up to 4096, groups * beams
  * up to 65535.  workspace: fk_beam_select_workspace_bytes(), zeroed once; launches that share it must not overlap. */
 fk_status fk_beam_select_workspace_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k, size_t *bytes);
 fk_status fk_beam_select(const uint16_t *logits, size_t row_stride, const float *scores, const uint32_t *finished,

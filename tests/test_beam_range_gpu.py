@@ -133,3 +133,21 @@ def test_steps_under_a_mask(fk):
         check(fk, x, s, 1, 4, 4)
         s = select(fk, x, s, 1, 4, 4)[0][0]
         assert s[0] == 0.0
+
+
+def test_scores_in_place(fk):
+    """What a search without host steps does: the new scores where the old ones were."""
+    groups, n_beams, vocab = 9, 5, 5003
+    x, s = make(50, groups * n_beams, vocab)
+    s = s.astype(np.float32)
+    d, scores = fk.DeviceBuffer.from_numpy(x), fk.DeviceBuffer.from_numpy(s)
+    outs = [fk.zeros(4 * groups * n_beams) for _ in range(2)]
+    ws = fk.zeros(fk.beam_select_workspace_bytes(groups, n_beams, vocab, n_beams))
+    for _ in range(3):
+        ref = plain(x, s, None, 0, groups, n_beams, n_beams)
+        fk.beam_select(d, vocab, scores, None, 0, groups, n_beams, vocab, n_beams, scores, *outs, ws, ws.nbytes)
+        fk.sync()
+        got = [b.to_numpy(t, (groups, n_beams)) for b, t in zip((scores, *outs), (np.float32, np.uint32, np.uint32))]
+        assert bool((got[1] == ref[1]).all() and (got[2] == ref[2]).all())
+        assert bool((np.abs(got[0] - ref[0]) <= 2.0 ** -21 + 2.0 ** -24 * np.abs(ref[0])).all())
+        s = got[0].ravel()

@@ -7,6 +7,7 @@ import oracle
 from helpers import normal_bf16, rng
 from paged_reference import Paged, attention, wide
 from test_paged_gpu import attend, check_attention
+from test_paged_graph_gpu import Graph, stream  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -191,3 +192,67 @@ def test_probabilities_of_few_columns_have_16_bits(fk, rows, lens, n_heads, n_kv
                 r = start[i] + j
                 lost += (np.abs(coarse - ref[r, h]) > 2.0 ** -8 * np.abs(ref[r, h]) + (2.0 ** -16 + 2.0 ** -20) * a[r, h]).sum()
     assert lost > 0 or min(lens[i] for i in few) > 1000
+
+
+# ---------------------------------------------------------------- captured, and on several streams
+
+class Planned:
+    """A call planned for up to `longest` positions, whose lengths are device values."""
+
+    def __init__(self, fk, rows, longest, n_heads, n_kv, dim, seed, page_rows=32):
+        self.fk, up = fk, fk.DeviceBuffer.from_numpy
+        n, self.rows, self.width = len(rows), sum(rows), n_heads * dim
+        per = -(-longest // page_rows)
+        table = rng(seed).permutation(n * per).astype(np.uint32)
+        self.lens = fk.zeros(4 * n)
+        self.d = [up(np.concatenate([[0], np.cumsum(rows)]).astype(np.uint32)), up(table)]
+        self.pages = [up(normal_bf16(seed + i, (n * per, n_kv, page_rows, dim))) for i in (1, 2)]
+        self.q, self.out = up(normal_bf16(seed + 3, (self.rows, self.width), std=2.0)), fk.zeros(2 * self.rows * self.width)
+        self.batch = fk.PagedBatch(self.d[0], self.lens, self.d[1], per, n, self.rows, max(rows), longest)
+        self.pool = fk.PagePool(*self.pages, n * per, page_rows, n_kv, dim)
+        self.ws, self.shape = fk.zeros(fk.sdpa_paged_workspace_bytes(n_heads, n_kv, dim, n, self.rows, longest)), (n_heads, dim)
+
+    def run(self, stream=None, out=None, workspace=None):
+        n_heads, dim = self.shape
+        ws = workspace or self.ws
+        self.fk.sdpa_paged(self.q, self.width, out or self.out, self.width, n_heads, dim ** -0.5, 0.0, 0, self.batch, self.pool, ws, ws.nbytes, stream)
+
+
+@pytest.mark.parametrize("rows", [[70, 1], [1, 100, 2], [40]])
+@pytest.mark.parametrize("n_heads,n_kv,dim", [(8, 2, 128), (14, 2, 64)])
+def test_cut_chunks_in_a_graph_whose_lengths_change(fk, stream, rows, n_heads, n_kv, dim):  # noqa: F811
+    st = stream()
+    a = Planned(fk, rows, 6000, n_heads, n_kv, dim, seed=20 + len(rows))
+    plain, ws = fk.zeros(a.out.nbytes), fk.zeros(a.ws.nbytes)
+    a.lens.upload(np.array([5000] * len(rows), np.uint32))
+    a.run(st)
+    fk.sync(st)
+    g = Graph(fk, st, lambda: a.run(st))
+    for i, length in enumerate((6000, 700, 3001, 5999, 150, 6000)):
+        a.lens.upload(np.array([max(r, length - 37 * j) for j, r in enumerate(rows)], np.uint32))
+        g.replay()
+        fk.sync(st)
+        a.run(st, plain, ws)
+        fk.sync(st)
+        assert np.array_equal(a.out.to_numpy(np.uint16), plain.to_numpy(np.uint16)), i
+        assert not a.ws.to_numpy(np.uint8)[:16384].any()
+    g.free()
+
+
+def test_cut_chunks_on_two_streams_at_once(fk, stream):  # noqa: F811
+    one, two = stream(), stream()
+    a, b = (Planned(fk, r, 5000, 8, 2, 128, seed=s) for r, s in (([90, 1], 31), ([1, 60, 1], 41)))
+    for p in (a, b):
+        p.lens.upload(np.array([5000 - 400 * i for i in range(p.batch.n_seqs)], np.uint32))
+    want = []
+    for p in (a, b):
+        p.run()
+        fk.sync()
+        want.append(p.out.to_numpy(np.uint16))
+        p.out.upload(np.zeros(p.rows * p.width, np.uint16))
+    for _ in range(8):
+        a.run(one)
+        b.run(two)
+    for st, p, w in ((one, a, want[0]), (two, b, want[1])):
+        fk.sync(st)
+        assert np.array_equal(p.out.to_numpy(np.uint16), w)
