@@ -22,12 +22,13 @@ constexpr uint32_t kBeamCounterStep = 32;
 constexpr size_t kBeamCounterBytes = (size_t)4 * kBeamCounterStep * kBeamGroups;
 
 // One launch.  A block takes a piece of a row: it leaves the piece's largest logit, its sum of exponentials and its k largest logits in order; the
-// block of a group that comes last forms lse and the k best of what all pieces left.  The pieces are cut by token, never by address: rows that
+// block of a group that comes last forms the rows' sums and the k best of what all pieces left.  The pieces are cut by token, never by address: rows that
 // hold the same values have the same sums wherever they lie, so that ties between beams stay ties.
 //
 // The k largest of a piece without sorting it: the k-th largest of the maxima of 64 (beyond k = 24: 256) parts of it is a bound that at least k
 // values reach and few more; found by bisection over its 16 bits with ballots.  What reaches it is collected in LDS and ranked by counting.
-// Only a piece full of ties has more than fit there: its k largest are then taken one by one.  Logits are compared two at a time as 16-bit
+// Only a piece full of ties has more than fit there: its k largest are then taken one by one (all but one token in a thousand at bf16's lowest value: 16 x 8
+// rows of 151851 102 us for 21, 4 of 32000 13 for 9; masked with -inf, which is not collected, as without a mask).  Logits are compared two at a time as 16-bit
 // integers: with a negative one's magnitude negated, bf16 values are in order (and -0 is 0).
 //
 // 16 x 8 rows of 151851 in 21 us, 1.85 TB/s.  A block waits for its piece (3 us while all ask at once), then for the bound, the list and the counter after

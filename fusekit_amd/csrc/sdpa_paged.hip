@@ -318,6 +318,8 @@ __device__ __forceinline__ void paged_store_columns(const SdpaPagedArgs& a, cons
 // on the same card).  The matrix unit works in half of the cycles, the vector unit as long.  What holds the rate is the card's power as much as that:
 // tiles of 256 columns with the softmax of one step between the products of another took a fifth fewer cycles at a clock a fifth lower (1.94 -> 1.54 GHz),
 // 428 us for 439, and lost a third where tiles are few.
+// A probability enters the second product as bf16, off by 2^-8 of itself at most, the sum it is divided by as fp32: outputs are off by 2.1e-3 of their norm where
+// their own rounding is 1.7e-3.  A second half, as single tokens have, would be half as many matrix instructions again.
 // SPLIT 2: tiles of 64 columns and 128 positions a step, for launches that leave CUs to themselves; two waves share 32 columns, 64 positions a step each,
 // and join at the end (the planner has the rule and its figures).
 constexpr uint32_t tile_lds_bytes(uint32_t d, uint32_t split) {
