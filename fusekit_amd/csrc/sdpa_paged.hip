@@ -32,6 +32,7 @@ struct SdpaPagedArgs {
     uint32_t slots, slot_bytes;
     uint32_t target, min_steps;   // items that a launch is cut into where its tiles are fewer; the least steps of an item
     uint32_t compact;             // tiles may be more than slots: only those that are cut have some
+    uint32_t blocks;              // of the launch
     uint32_t only_few;            // of chunks among single tokens: whole chunks, cut tokens (compact)
 };
 
@@ -41,7 +42,10 @@ __device__ __forceinline__ uint32_t paged_limit(const PagedSeq& s, uint32_t plac
 // What sums of probabilities are multiplied with, l their total: 0 for a row that sees nothing, and not a number, which has the column done again by
 // paged_row, where l is not between bounds that it does not leave unless scores are beyond some 1e9: the reference, a rounded product, and the exponents,
 // each one rounding of product and reference, are then apart by more than fp32's exponents hold.
-__device__ __forceinline__ float paged_inverse(float l, uint32_t limit) { return l > 0x1p-60f && l < 0x1p60f ? 1.0f / l : limit ? __builtin_nanf("") : 0.f; }
+__device__ __forceinline__ float paged_inverse(float l, uint32_t limit) {
+    const float f = 1.0f / l;
+    return __builtin_expect(f > 0x1p-60f && f < 0x1p60f, 1) ? f : limit ? __builtin_nanf("") : 0.f;
+}
 
 // ---- one row of one head by a wave: positions in the order they lie, what the row does not see is not touched ----
 // The statement of the operator as it stands; the tiles below come here for a column whose sums are not finite, since a zero
@@ -173,7 +177,7 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
     const bool compact = only_few || (!TILES && a.compact != 0 && !(pairs + (float)a.target <= (float)a.slots));
     // (a batch whose row_start falls can have more tiles than the host has counted: cut, the last items of a tile would be behind the launch's end,
     // and its counter would never be left ready)
-    bool cut = pairs + (float)a.target <= (compact ? (float)gridDim.x : (float)a.slots);
+    bool cut = pairs + (float)a.target <= (float)(compact ? a.blocks : a.slots);
     // (of at least work / target steps: all items together are at most target + pairs)
     const float share = work / (float)a.target;
     uint32_t unit = share < 0x1p30f ? (uint32_t)ceilf(share) : 1u << 30;
@@ -191,7 +195,7 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
         longest_whole = wave_max(longest_whole);
         longest_cut = wave_max(longest_cut);
         const float tiles = wave_sum(wholes) + pairs;
-        only_few = cut = longest_cut > 2.0f * longest_whole && tiles + (float)a.target <= (float)gridDim.x;
+        only_few = cut = longest_cut > 2.0f * longest_whole && tiles + (float)a.target <= (float)a.blocks;
         tokens = !only_few || tiles > (float)a.target;
     }
     bool second = !only_few;
@@ -1107,7 +1111,8 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     }
     l->func = p.few ? few[D == 128][softcap > 0.f][batch->max_rows * (n_heads / n_kv) > 8u] : tile[D == 128][softcap > 0.f][split];
     // (no more blocks than there can be items: one that finds none costs what it takes to look)
-    l->grid = dim3((uint32_t)(cut && !a.compact ? std::min<uint64_t>(p.slots, p.tiles * splits) : split ? halves : p.tiles + (cut || a.only_few ? a.target : 0u)), 1, 1);
+    a.blocks = (uint32_t)(cut && !a.compact ? std::min<uint64_t>(p.slots, p.tiles * splits) : split ? halves : p.tiles + (cut || a.only_few ? a.target : 0u));
+    l->grid = dim3(a.blocks, 1, 1);
     l->block = dim3(256, 1, 1);
     l->shmem = p.few ? few_lds_bytes(D) : std::max(tile_lds_bytes(D, split ? 2u : 1u), few_lds_bytes(D));
     if ((int)l->shmem > dev->max_dyn_lds) return set_error(FK_ERR_UNSUPPORTED, "sdpa_paged: LDS tile does not fit");
