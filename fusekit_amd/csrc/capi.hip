@@ -1002,8 +1002,14 @@ fk_status fk_sdpa_paged_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_
 fk_status fk_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, uint32_t out_stride, uint32_t n_heads, float scale, float softcap,
                         uint32_t window, const fk_paged_batch* batch, const fk_page_pool* pool, void* workspace, size_t workspace_bytes,
                         fk_stream s) {
+    return fk_sdpa_paged_sinks(q, q_stride, out, out_stride, n_heads, scale, softcap, window, 0, batch, pool, workspace, workspace_bytes, s);
+}
+
+fk_status fk_sdpa_paged_sinks(const uint16_t* q, uint32_t q_stride, uint16_t* out, uint32_t out_stride, uint32_t n_heads, float scale, float softcap,
+                              uint32_t window, uint32_t sinks, const fk_paged_batch* batch, const fk_page_pool* pool, void* workspace,
+                              size_t workspace_bytes, fk_stream s) {
     Launch l;
-    FK_TRY(plan_sdpa_paged(q, q_stride, out, out_stride, n_heads, scale, softcap, window, batch, pool, workspace, workspace_bytes, &l));
+    FK_TRY(plan_sdpa_paged(q, q_stride, out, out_stride, n_heads, scale, softcap, window, sinks, batch, pool, workspace, workspace_bytes, &l));
     return run_launch(l, (hipStream_t)s);
 }
 
@@ -1019,12 +1025,31 @@ fk_status fk_paged_check(uint32_t* fault, fk_stream s) {
     if (bits & FK_PAGED_BAD_ROWS) m += " row_start falls or exceeds the launch's rows;";
     if (bits & FK_PAGED_BAD_LENGTH) m += " a length above max_len or below the sequence's new rows;";
     if (bits & FK_PAGED_BAD_PAGE) m += " a page id that the pool does not have;";
+    if (bits & FK_PAGED_BAD_SLOT) m += " a slot beyond the tables or named twice;";
+    if (bits & FK_PAGED_NO_PAGE) m += " fewer free pages than the batch needs;";
     return set_error(FK_ERR_INVALID, m);
 }
 
 fk_status fk_pages_copy(void* base, uint32_t n_planes, size_t plane_stride, uint32_t n_pages, size_t page_bytes, const uint32_t* pairs,
                         uint32_t n_pairs, fk_stream s) {
     return run_pages_copy(base, n_planes, plane_stride, n_pages, page_bytes, pairs, n_pairs, (hipStream_t)s);
+}
+
+fk_status fk_paged_extend(const fk_paged_requests* requests, const fk_paged_batch* batch, uint32_t n_pages, uint32_t page_rows, uint32_t* row_slots,
+                          fk_stream s) {
+    Launch l;
+    FK_TRY(plan_paged_extend(requests, batch, n_pages, page_rows, row_slots, &l));
+    return run_launch(l, (hipStream_t)s);
+}
+
+fk_status fk_sample_workspace_bytes(uint32_t rows, uint32_t vocab, size_t* bytes) { return sample_workspace_bytes(rows, vocab, bytes); }
+
+fk_status fk_sample(const uint16_t* logits, size_t row_stride, uint32_t rows, uint32_t vocab, const float* temperature, const uint32_t* top_k,
+                    const float* top_p, const float* min_p, const float* u, uint32_t* tokens, float* logprobs, void* workspace,
+                    size_t workspace_bytes, fk_stream s) {
+    Launch l;
+    FK_TRY(plan_sample(logits, row_stride, rows, vocab, temperature, top_k, top_p, min_p, u, tokens, logprobs, workspace, workspace_bytes, &l));
+    return run_launch(l, (hipStream_t)s);
 }
 
 fk_status fk_beam_select_workspace_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k, size_t* bytes) {

@@ -405,8 +405,14 @@ fk_status plan_rope_paged_store(const uint16_t* q, uint32_t q_stride, const uint
 fk_status sdpa_paged_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t n_seqs, uint32_t rows, uint32_t max_len,
                                      size_t* bytes);
 fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, uint32_t out_stride, uint32_t n_heads, float scale,
-                          float softcap, uint32_t window, const fk_paged_batch* batch, const fk_page_pool* pool, void* workspace,
+                          float softcap, uint32_t window, uint32_t sinks, const fk_paged_batch* batch, const fk_page_pool* pool, void* workspace,
                           size_t workspace_bytes, Launch* launch);
+fk_status plan_paged_extend(const fk_paged_requests* requests, const fk_paged_batch* batch, uint32_t n_pages, uint32_t page_rows, uint32_t* row_slots,
+                            Launch* out);
+fk_status sample_workspace_bytes(uint32_t rows, uint32_t vocab, size_t* bytes);
+fk_status plan_sample(const uint16_t* logits, size_t row_stride, uint32_t rows, uint32_t vocab, const float* temperature, const uint32_t* top_k,
+                      const float* top_p, const float* min_p, const float* u, uint32_t* tokens, float* logprobs, void* workspace, size_t workspace_bytes,
+                      Launch* out);
 fk_status run_pages_copy(void* base, uint32_t n_planes, size_t plane_stride, uint32_t n_pages, size_t page_bytes, const uint32_t* pairs,
                          uint32_t n_pairs, hipStream_t s);
 fk_status beam_select_workspace_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k, size_t* bytes);

@@ -2,7 +2,7 @@
 //
 //     out[r, h] = sum_j p_j V[j] / sum_j p_j,   p_j = exp(x_j - max x),   x_j = c(q[r, h] . K[j] * scale),   max(0, p - window + 1) <= j <= p
 //
-// with p the row's position and c(x) = x, or softcap * tanh(x / softcap).
+// with p the row's position and c(x) = x, or softcap * tanh(x / softcap); with `sinks` also the positions j < sinks (j <= p) before the window.
 #include <math.h>
 
 #include <algorithm>
@@ -25,7 +25,7 @@ struct SdpaPagedArgs {
     const uint16_t* v;
     uint16_t* out;
     uint32_t q_stride, out_stride, group;
-    uint32_t window;
+    uint32_t window, sinks;
     float scale, softcap;
     float* partials;       // [slots][columns of a tile][D], then (m, l) [slots][columns of a tile]
     uint32_t* counters;    // [slots], zero before the first launch, left zero
@@ -55,6 +55,7 @@ __device__ __forceinline__ void paged_row(const SdpaPagedArgs& a, uint32_t seq, 
     const uint32_t kvh = head / a.group, row = s.row0 + place, page_rows = 1u << a.b.page_shift;
     const uint32_t end = paged_limit(s, place);
     const uint32_t first = a.window && end > a.window ? end - a.window : 0u;
+    const uint32_t sinks = a.sinks < first ? a.sinks : first, gap = first - sinks, seen = end - gap;   // the positions seen: sinks, then from `first` on
     const uint16_t* qr = a.q + (size_t)row * a.q_stride + (size_t)head * D;
     constexpr int DL = D / 64;
     uint32_t bad = 0;
@@ -62,8 +63,8 @@ __device__ __forceinline__ void paged_row(const SdpaPagedArgs& a, uint32_t seq, 
     double l = 0.0, o[DL];   // (values of the type's whole range, and 2^31 of the largest)
 #pragma unroll
     for (int i = 0; i < DL; ++i) o[i] = 0.0;
-    for (uint32_t at = first; at < end; at += 64u) {
-        const uint32_t pos = at + lane < end ? at + lane : end - 1u;
+    for (uint32_t at = 0; at < seen; at += 64u) {
+        const uint32_t place_seen = at + lane < seen ? at + lane : seen - 1u, pos = place_seen < sinks ? place_seen : place_seen + gap;
         const uint32_t page = paged_page(a.b, seq, pos >> a.b.page_shift, bad);
         const size_t base = (((size_t)page * a.b.n_kv + kvh) * page_rows + (pos & (page_rows - 1u))) * D;
         const uint4* kr = reinterpret_cast<const uint4*>(a.k + base);
@@ -77,13 +78,13 @@ __device__ __forceinline__ void paged_row(const SdpaPagedArgs& a, uint32_t seq, 
         }
         x *= a.scale;
         if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
-        if (at + lane >= end) x = -INFINITY;
+        if (at + lane >= seen) x = -INFINITY;
         const float m_new = fmaxf(m, wave_max(x)), ref = m_new == -INFINITY ? 0.f : m_new, alpha = expf(m - ref), p = expf(x - ref);
         l = l * alpha + (double)wave_sum(p);
         m = m_new;
 #pragma unroll
         for (int i = 0; i < DL; ++i) o[i] *= alpha;
-        const uint32_t n = end - at < 64u ? end - at : 64u;
+        const uint32_t n = seen - at < 64u ? seen - at : 64u;
 #pragma unroll 1
         for (uint32_t j = 0; j < n; ++j) {
             const float pj = __shfl(p, (int)j, 64);
@@ -94,7 +95,7 @@ __device__ __forceinline__ void paged_row(const SdpaPagedArgs& a, uint32_t seq, 
     }
 #pragma unroll
     for (int i = 0; i < DL; ++i)
-        a.out[(size_t)row * a.out_stride + (size_t)head * D + lane + 64u * i] = (uint16_t)f32_to_bf16_bits(end > first ? (float)(o[i] / l) : 0.f);
+        a.out[(size_t)row * a.out_stride + (size_t)head * D + lane + 64u * i] = (uint16_t)f32_to_bf16_bits(seen ? (float)(o[i] / l) : 0.f);
 }
 
 // ---- which piece of the work a block does ----
@@ -125,7 +126,7 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
         uint32_t seen = s.len;
         if (a.window) {
             const uint32_t span = COLS / a.group + 2u;   // rows of a tile, at most
-            const uint64_t w = (uint64_t)a.window + (s.rows < span ? s.rows : span) + STEP - 1u;
+            const uint64_t w = (uint64_t)a.window + a.sinks + (s.rows < span ? s.rows : span) + (a.sinks ? 2u * STEP : STEP) - 1u;
             seen = w < seen ? (uint32_t)w : seen;
         }
         return (seen + STEP - 1u) / STEP;
@@ -254,9 +255,12 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
 }
 constexpr int kPastCaches = 16;   // (sc1: what another block wrote, or is to read)
 
-// What a tile's columns e_tile .. e_last see, in steps of STEP positions, and how its items share them: item i takes `per` steps from step0 + i * per.
+// What a tile's columns e_tile .. e_last see, in steps of STEP positions, and how its items share them: item i takes `per` of the `steps` from i * per on.
+// The steps are counted without those that lie between the sinks and the window: step number n is n, from `near` on n + gap.
 struct PagedRange {
-    uint32_t kv_end, step0, steps, per, n_active;   // n_active: items that have steps, one at least
+    uint32_t kv_end, steps, per, n_active;   // n_active: items that have steps, one at least
+    uint32_t near, gap;
+    __device__ __forceinline__ uint32_t step(uint32_t n) const { return n < near ? n : n + gap; }
 };
 template <uint32_t STEP>
 __device__ __forceinline__ PagedRange paged_range(const SdpaPagedArgs& a, const PagedItem& it, uint32_t e_tile, uint32_t e_last) {
@@ -264,8 +268,11 @@ __device__ __forceinline__ PagedRange paged_range(const SdpaPagedArgs& a, const 
     PagedRange r;
     r.kv_end = __builtin_amdgcn_readfirstlane(limit_of(e_last / a.group));
     const uint32_t first = limit_of(e_tile / a.group);
-    r.step0 = __builtin_amdgcn_readfirstlane((a.window && first > a.window ? first - a.window : 0u) / STEP);
-    r.steps = (r.kv_end + STEP - 1u) / STEP - (r.kv_end ? r.step0 : 0u);
+    const uint32_t step0 = __builtin_amdgcn_readfirstlane((a.window && first > a.window ? first - a.window : 0u) / STEP);
+    const uint32_t sink_steps = a.sinks / STEP + (a.sinks % STEP ? 1u : 0u);
+    r.near = sink_steps < step0 ? sink_steps : step0;
+    r.gap = step0 - r.near;
+    r.steps = (r.kv_end + STEP - 1u) / STEP - (r.kv_end ? r.gap : 0u);
     r.per = (r.steps + it.n_splits - 1u) / it.n_splits;
     r.n_active = r.per ? (r.steps + r.per - 1u) / r.per : 1u;
     return r;
@@ -350,8 +357,8 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
     const PagedRange range = paged_range<STEP>(a, it, e_tile, e_last);
     const uint32_t kv_end = range.kv_end, n_active = range.n_active;
     if (it.split >= n_active) return;
-    const uint32_t begin = __builtin_amdgcn_readfirstlane(range.step0 + it.split * range.per);
-    const uint32_t stop = __builtin_amdgcn_readfirstlane(it.split + 1u == n_active ? range.step0 + range.steps : begin + range.per);
+    const uint32_t begin = __builtin_amdgcn_readfirstlane(it.split * range.per);
+    const uint32_t stop = __builtin_amdgcn_readfirstlane(it.split + 1u == n_active ? range.steps : begin + range.per);
 
     // this lane's column; a wave's columns past the last repeat it, and a wave without columns does the last one's loads and nothing else
     const uint32_t e0 = e_tile + column_tile * 32u;
@@ -379,7 +386,7 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
     struct Pages {
         uint32_t id[SPLIT];
     };
-    auto span_of = [&](uint32_t step, uint32_t g) { return step * STEP + (wave * SPLIT + g) * 16u; };   // the first of 16 rows of a step that this wave requests
+    auto span_of = [&](uint32_t step, uint32_t g) { return range.step(step) * STEP + (wave * SPLIT + g) * 16u; };   // the first of 16 rows of a step that this wave requests
     auto pages_of = [&](uint32_t step) {                                                                 // (past the range: the last position's)
         Pages p;
 #pragma unroll
@@ -444,8 +451,8 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
             issue(step + 1u, next, stage ^ 1u);
             if (step + 2u < stop) next = pages_of(step + 2u);
         }
-        const uint32_t kv0 = step * STEP + my_half * kTileStep;            // this wave's 64 positions
-        if (kv0 >= last_limit || kv0 + kTileStep <= first_low) continue;   // nothing that a row of this wave sees
+        const uint32_t kv0 = range.step(step) * STEP + my_half * kTileStep;                   // this wave's 64 positions
+        if (kv0 >= last_limit || (kv0 + kTileStep <= first_low && kv0 >= a.sinks)) continue;   // nothing that a row of this wave sees
         const unsigned char *ks = lds + stage * STAGE + my_half * kTileStep * ROW, *vs = ks + TILE;
         // (two of the eight pairs of fragments ahead of their matrix instructions; all of them first took 1 % longer of two chunks of 2048 rows, 2 % with a window)
         pf_u32x4_t kf[3][2];
@@ -495,7 +502,7 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const uint32_t kv = kv0 + (uint32_t)(t * 32 + r % 4 + 8 * (r / 4)) + 4u * kb;
-                    if (kv >= q_limit || kv < q_low) s[t][r] = -INFINITY;
+                    if (kv >= q_limit || (kv < q_low && kv >= a.sinks)) s[t][r] = -INFINITY;
                 }
         }
         // the softmax reference moves only when a step's maximum outgrows it by 2^8
@@ -720,10 +727,18 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
     const uint32_t kv_end = range.kv_end, n_active = range.n_active, lim_lo = __builtin_amdgcn_readfirstlane(limit_of(e0 / G));
     const uint32_t low_hi = __builtin_amdgcn_readfirstlane(low_of(kv_end));
     if (it.split >= n_active) return;
-    const uint32_t first = (range.step0 + it.split * range.per) * kFewRound + wave * kFewStep;
-    uint32_t end = (range.step0 + (it.split + 1u) * range.per) * kFewRound;
-    end = __builtin_amdgcn_readfirstlane(end < kv_end ? end : kv_end);
-    const uint32_t n_steps = __builtin_amdgcn_readfirstlane(end > first ? (end - first + kFewRound - 1u) / kFewRound : 0u);
+    const uint32_t round0 = it.split * range.per;
+    uint32_t rounds = range.steps < round0 + range.per ? range.steps - round0 : range.per;   // of this item
+    // (of the sinks' last round a wave whose positions lie behind them sees nothing, and leaves it out)
+    const uint32_t near_wave = a.sinks > wave * kFewStep ? (a.sinks - wave * kFewStep + kFewRound - 1u) / kFewRound : 0u;
+    const bool leaves = near_wave < range.near && near_wave >= round0 && near_wave - round0 < rounds;
+    rounds -= leaves ? 1u : 0u;
+    auto at_round = [&](uint32_t j) {
+        const uint32_t n = round0 + j;
+        return range.step(n + (leaves && n >= near_wave ? 1u : 0u)) * kFewRound + wave * kFewStep;
+    };
+    // (a wave's place in the last round may lie behind the context)
+    const uint32_t n_steps = __builtin_amdgcn_readfirstlane(rounds ? rounds - (at_round(rounds - 1u) >= kv_end ? 1u : 0u) : 0u);
 
     const uint32_t mine = n % QT < columns ? n % QT : columns - 1u;   // (columns past the last repeat it and store nothing)
     const uint32_t place = (e0 + mine) / G, q_limit = limit_of(place), q_low = low_of(q_limit);
@@ -778,18 +793,19 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
 
     uint32_t page[2] = {0, 0};
     if (n_steps) {
+        const uint32_t first = at_round(0), second = at_round(1);
         page[0] = page_of(first);
         page[1] = page_of(first + 16u);
         issue_k(first, page);
         issue_v(first, page);
         if (n_steps > 1u) {
-            page[0] = page_of(first + kFewRound);
-            page[1] = page_of(first + kFewRound + 16u);
+            page[0] = page_of(second);
+            page[1] = page_of(second + 16u);
         }
     }
 #pragma unroll 1
     for (uint32_t j = 0; j < n_steps; ++j) {
-        const uint32_t kv0 = first + j * kFewRound;
+        const uint32_t kv0 = at_round(j), kv1 = at_round(j + 1u);
         unsigned char* const ks = lds + my_stage;
         unsigned char* const vs = ks + KT;
         const bool more = j + 1u < n_steps;
@@ -821,7 +837,7 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
             for (int i = 0; i < 4; ++i) x[t * 4 + i] = s4[i];
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (more) issue_k(kv0 + kFewRound, page);   // the keys are in registers: their place takes the next step's
+        if (more) issue_k(kv1, page);   // the keys are in registers: their place takes the next step's
         if constexpr (CAP) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[i] * turn2)), cap2);
@@ -830,7 +846,7 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const uint32_t kv = kv0 + (uint32_t)(i / 4) * 16u + 4u * g + (uint32_t)(i % 4);
-                if (kv >= q_limit || kv < q_low) x[i] = -INFINITY;
+                if (kv >= q_limit || (kv < q_low && kv >= a.sinks)) x[i] = -INFINITY;
             }
         }
         float mx = x[0];
@@ -883,10 +899,11 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
             for (int i = 0; i < DT; ++i) acc[p][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[i], __builtin_bit_cast(pf_bf16x8_t, pb[p]), acc[p][i], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
         if (more) {
-            issue_v(kv0 + kFewRound, page);
+            issue_v(kv1, page);
             if (j + 2u < n_steps) {
-                page[0] = page_of(kv0 + 2u * kFewRound);
-                page[1] = page_of(kv0 + 2u * kFewRound + 16u);
+                const uint32_t kv2 = at_round(j + 2u);
+                page[0] = page_of(kv2);
+                page[1] = page_of(kv2 + 16u);
             }
         }
     }
@@ -1041,7 +1058,8 @@ fk_status sdpa_paged_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t h
 }
 
 fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, uint32_t out_stride, uint32_t n_heads, float scale, float softcap,
-                          uint32_t window, const fk_paged_batch* batch, const fk_page_pool* pool, void* workspace, size_t workspace_bytes, Launch* l) {
+                          uint32_t window, uint32_t sinks, const fk_paged_batch* batch, const fk_page_pool* pool, void* workspace, size_t workspace_bytes,
+                          Launch* l) {
     SdpaPagedArgs a;
     memset(&a, 0, sizeof(a));
     FK_TRY(paged_args("sdpa_paged", batch, pool, &a.b));
@@ -1070,6 +1088,8 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     FK_TRY(device_facts(&dev));
     a.q = q; a.k = pool->k; a.v = pool->v; a.out = out;
     a.q_stride = q_stride; a.out_stride = out_stride; a.group = n_heads / n_kv;
+    // (without a window everything is seen, and sinks beyond the longest sequence are as many)
+    a.sinks = window ? std::min(sinks, batch->max_len) : 0;
     a.window = window; a.scale = scale; a.softcap = softcap;
     a.counters = static_cast<uint32_t*>(workspace);
     a.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kPagedCounterBytes);
@@ -1087,7 +1107,7 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     // Positions that a tile can see, in steps.  Chunks of up to 8 steps are not cut: the merge costs what it saves (a prompt of 512 rows, 32 / 8 heads x
     // 128: 18 us whole, 24 in halves).
     const uint32_t step = p.few ? kFewRound : kTileStep, span = (p.few ? kFewCols : kTileCols) / a.group + 2u;
-    const uint64_t seen = window ? std::min<uint64_t>(batch->max_len, (uint64_t)window + std::min(batch->max_rows, span) + step) : batch->max_len;
+    const uint64_t seen = window ? std::min<uint64_t>(batch->max_len, (uint64_t)window + a.sinks + std::min(batch->max_rows, span) + (a.sinks ? 2u : 1u) * step) : batch->max_len;
     const uint32_t most = (uint32_t)((seen + step - 1u) / step), splits = (most + p.min_steps - 1u) / p.min_steps;
     // Tiles of 64 columns and twice the positions a step where each has a CU to itself: a lone block's step takes 1.3 to 1.5 us, most of it waits that do not
     // depend on what it holds, and half as many are left.  32 / 8 heads x 128, us in whole or cut tiles of 128 and in these: a fresh prompt of 512 rows 17.2,

@@ -660,6 +660,18 @@ class PagedBatch(C.Structure):
         super().__init__(_addr(row_start), _addr(kv_len), _addr(page_table), table_stride, n_seqs, rows, max_rows, max_len, _addr(fault))
 
 
+class PagedRequests(C.Structure):
+    """fk_paged_requests: uint32 arrays in device memory.  slot [n_seqs] (None: sequence i is in slot i), new_rows [n_seqs] (None: one each), lengths and
+    lengths_out [n_slots], tables [n_slots, table_stride], free_pages [n_pages], words n_free, n_free_out, counter (zeroed once)."""
+    _fields_ = [("slot", C.c_void_p), ("new_rows", C.c_void_p), ("n_slots", C.c_uint32), ("lengths", C.c_void_p), ("lengths_out", C.c_void_p),
+                ("tables", C.c_void_p), ("table_stride", C.c_uint32), ("free_pages", C.c_void_p), ("n_free", C.c_void_p), ("n_free_out", C.c_void_p),
+                ("counter", C.c_void_p)]
+
+    def __init__(self, slot, new_rows, n_slots, lengths, lengths_out, tables, table_stride, free_pages, n_free, n_free_out, counter):
+        super().__init__(_addr(slot), _addr(new_rows), n_slots, _addr(lengths), _addr(lengths_out), _addr(tables), table_stride, _addr(free_pages),
+                         _addr(n_free), _addr(n_free_out), _addr(counter))
+
+
 ROPE_SCALINGS = {"plain": 0, "linear": 1, "parts": 2, "ramp": 3}
 
 
@@ -689,6 +701,18 @@ def sdpa_paged(q, q_stride, out, out_stride, n_heads, scale, softcap, window, ba
     """Attention of a batch's new rows, chunks and single tokens, over its pages (fk_sdpa_paged)."""
     check(lib.fk_sdpa_paged(_addr(q), q_stride, _addr(out), out_stride, n_heads, scale, softcap, window, batch, pool, _addr(workspace),
                             workspace_bytes, _addr(stream)))
+
+
+def sdpa_paged_sinks(q, q_stride, out, out_stride, n_heads, scale, softcap, window, sinks, batch: PagedBatch, pool: PagePool, workspace,
+                     workspace_bytes, stream=None):
+    """sdpa_paged with the first `sinks` positions visible besides the window (fk_sdpa_paged_sinks)."""
+    check(lib.fk_sdpa_paged_sinks(_addr(q), q_stride, _addr(out), out_stride, n_heads, scale, softcap, window, sinks, batch, pool, _addr(workspace),
+                                  workspace_bytes, _addr(stream)))
+
+
+def paged_extend(requests: PagedRequests, batch: PagedBatch, n_pages, page_rows, row_slots=None, stream=None):
+    """A batch's row starts, lengths and page tables from the requests' lengths, with the pages that are missing (fk_paged_extend)."""
+    check(lib.fk_paged_extend(requests, batch, n_pages, page_rows, _addr(row_slots), _addr(stream)))
 
 
 def paged_check(fault, stream=None) -> None:
@@ -724,6 +748,18 @@ def beam_select(logits, row_stride, scores, finished, pad_token, groups, beams, 
     """The k best continuations of each group's beams (fk_beam_select)."""
     check(lib.fk_beam_select(_addr(logits), row_stride, _addr(scores), _addr(finished), pad_token, groups, beams, vocab, k,
                              _addr(out_scores), _addr(out_beams), _addr(out_tokens), _addr(workspace), workspace_bytes, _addr(stream)))
+
+
+def sample_workspace_bytes(rows, vocab) -> int:
+    out = C.c_size_t()
+    check(lib.fk_sample_workspace_bytes(rows, vocab, C.byref(out)))
+    return out.value
+
+
+def sample(logits, row_stride, rows, vocab, temperature, top_k, top_p, min_p, u, tokens, logprobs, workspace, workspace_bytes, stream=None):
+    """A token drawn from each row of logits with its temperature, top-k, top-p and min-p (device arrays or None) and its random number (fk_sample)."""
+    check(lib.fk_sample(_addr(logits), row_stride, rows, vocab, _addr(temperature), _addr(top_k), _addr(top_p), _addr(min_p), _addr(u), _addr(tokens),
+                        _addr(logprobs), _addr(workspace), workspace_bytes, _addr(stream)))
 
 
 def beam_reorder(src, dst, row_bytes, parents, groups, beams, n_out, stream=None, src_stride=None, dst_stride=None):
@@ -809,7 +845,7 @@ class Event:
 
 # Argument types of the operators, declared once: ctypes converts plain numbers and addresses in C, and a call does not build an
 # object for each (rmsnorm + q / k / v, thirteen arguments: 6.4 us a call with the objects, 5.4 without; a launch
-# alone takes 4.0).  p an address, W an fk_weight, Q a quantised cache, B / P a paged batch / pool, u / i / f a 32-bit number, d a
+# alone takes 4.0).  p an address, W an fk_weight, Q a quantised cache, B / P / R a paged batch / pool / requests, u / i / f a 32-bit number, d a
 # 64-bit one, z a size.
 _SIGNATURES = {
     "fk_qgemv": "Wpppp", "fk_linear_residual": "Wppppp", "fk_rmsnorm_qkv": "ppfWWWppppppp",
@@ -830,12 +866,13 @@ _SIGNATURES = {
     "fk_step_init": "pppp", "fk_step_init_rope": "ppppufp", "fk_rope_store_sdpa_decode": "pppppppppuuuuuuffufpppp",
     "fk_xcd_kslice_meta": "puupp", "fk_xcd_check": "pp", "fk_route_order": "puupp", "fk_set_gemv_policy": "uu",
     "fk_rope_frequencies": "udidddupp", "fk_rope_paged_store": "pupupupuuppfuipBPp", "fk_sdpa_paged_workspace_bytes": "uuuuuup",
-    "fk_sdpa_paged": "pupuuffuBPpzp", "fk_paged_check": "pp", "fk_pages_copy": "puzuzpup", "fk_beam_select_workspace_bytes": "uuuup",
+    "fk_sdpa_paged": "pupuuffuBPpzp", "fk_sdpa_paged_sinks": "pupuuffuuBPpzp", "fk_paged_check": "pp", "fk_pages_copy": "puzuzpup", "fk_beam_select_workspace_bytes": "uuuup",
     "fk_beam_select": "pzppuuuuuppppzp", "fk_beam_reorder": "pzpzzpuuup",
+    "fk_paged_extend": "RBuupp", "fk_sample_workspace_bytes": "uup", "fk_sample": "pzuuppppppppzp",
     "fk_set_qgemm_wide": "i", "fk_set_gemv_flat_only": "i", "fk_stream_sync": "p",
 }
 
 _TYPES = {"p": C.c_void_p, "W": C.POINTER(Weight), "Q": C.POINTER(_KvQuantCache), "u": C.c_uint32, "i": C.c_int, "f": C.c_float,
-          "B": C.POINTER(PagedBatch), "P": C.POINTER(PagePool), "d": C.c_double, "z": C.c_size_t}
+          "B": C.POINTER(PagedBatch), "R": C.POINTER(PagedRequests), "P": C.POINTER(PagePool), "d": C.c_double, "z": C.c_size_t}
 for _name, _signature in _SIGNATURES.items():
     getattr(lib, _name).argtypes = [_TYPES[_t] for _t in _signature]

@@ -592,7 +592,9 @@ typedef struct fk_paged_batch {
 enum {
     FK_PAGED_BAD_ROWS = 1,              /* row_start falls, or a sequence has more rows than max_rows or the buffers hold */
     FK_PAGED_BAD_LENGTH = 2,            /* kv_len above max_len, or below the sequence's new rows */
-    FK_PAGED_BAD_PAGE = 4               /* a page id that the pool does not have */
+    FK_PAGED_BAD_PAGE = 4,              /* a page id that the pool does not have, or more free pages than the pool has */
+    FK_PAGED_BAD_SLOT = 8,              /* fk_paged_extend: a slot beyond the tables, or named twice */
+    FK_PAGED_NO_PAGE = 16               /* fk_paged_extend: fewer free pages than the batch needs */
 };
 /* Synchronises the stream; FK_ERR_INVALID with a message where *fault is set, which is then zeroed.  What the launches
  * since the last check wrote for the sequence at fault is undefined (inside its own rows and pages); workspaces are left ready. */
@@ -643,6 +645,36 @@ fk_status fk_sdpa_paged_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_
 fk_status fk_sdpa_paged(const uint16_t *q, uint32_t q_stride, uint16_t *out, uint32_t out_stride, uint32_t n_heads,
                         float scale, float softcap, uint32_t window, const fk_paged_batch *batch,
                         const fk_page_pool *pool, void *workspace, size_t workspace_bytes, fk_stream s);
+/* The same with the first `sinks` positions of a sequence visible besides the window: a row at position p attends to the positions j <= p with
+ *     j < sinks or j > p - window.  (window 0: to all of them.)  Pages that lie between the two are not read but for the ends of 128 positions that
+ *     are walked at a time; what they hold reaches no row. */
+fk_status fk_sdpa_paged_sinks(const uint16_t *q, uint32_t q_stride, uint16_t *out, uint32_t out_stride, uint32_t n_heads,
+                              float scale, float softcap, uint32_t window, uint32_t sinks, const fk_paged_batch *batch,
+                              const fk_page_pool *pool, void *workspace, size_t workspace_bytes, fk_stream s);
+/* A batch built on the device: what launches over `batch` read -- row_start, kv_len, page_table -- and the pool row of every new row are written from
+ * the lengths that the requests have, so that a decode loop, or a captured graph of one step, goes on without the host.  Requests keep their length and
+ * their pages in slots (a row of `tables` each); the batch names the slots that run and how many new rows each has.  Sequence i gets the pages that
+ * its new rows need, from the top of the stack free_pages[0 .. *n_free - 1] on in the sequences' order, at the end of its row of `tables`, and a copy of that
+ * row in batch->page_table (as many entries as it has pages; what is behind stays as it is).  row_slots (may be NULL): new row r lies in row row_slots[r] of the pool, its page
+ * times page_rows + its row there (rows behind the last stay as they are).  lengths_out and n_free_out are what is then held and free; they may be lengths
+ * and n_free.  A slot's last page, where it is partly filled, must be its own (fork: fk_pages_copy).
+ * All or nothing: where a slot, a count of rows, a length or the free pages do not fit, no sequence has a new row, kv_len is 0, tables, lengths and free
+ * pages stay as they were, and bits of *batch->fault say why.  What is written overlaps nothing else. */
+typedef struct fk_paged_requests {
+    const uint32_t *slot;               /* device [n_seqs], each below n_slots and named once; NULL: sequence i is in slot i */
+    const uint32_t *new_rows;           /* device [n_seqs], 0 up to max_rows; NULL: one each */
+    uint32_t n_slots;                   /* up to 2^18 */
+    const uint32_t *lengths;            /* device [n_slots]: positions before the new rows */
+    uint32_t *lengths_out;              /* device [n_slots] */
+    uint32_t *tables;                   /* device [n_slots, table_stride] */
+    uint32_t table_stride;
+    const uint32_t *free_pages;         /* device [n_pages] */
+    const uint32_t *n_free;             /* device word */
+    uint32_t *n_free_out;               /* device word */
+    uint32_t *counter;                  /* device word, zeroed once; calls that share it must not overlap */
+} fk_paged_requests;
+fk_status fk_paged_extend(const fk_paged_requests *requests, const fk_paged_batch *batch, uint32_t n_pages, uint32_t page_rows,
+                          uint32_t *row_slots, fk_stream s);
 /* Pages copied inside a pool: page pairs[2 i] to page pairs[2 i + 1] in each of n_planes planes that lie plane_stride
  * bytes apart (the layers' K and V; n_pages pages of page_bytes, a multiple of 16).  pairs is HOST memory and is read
  * before the call returns (a captured launch keeps the pairs it was captured with).  What a fork of a sequence leaves to
@@ -665,6 +697,20 @@ fk_status fk_beam_select(const uint16_t *logits, size_t row_stride, const float 
                          uint32_t pad_token, uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k,
                          float *out_scores, uint32_t *out_beams, uint32_t *out_tokens, void *workspace,
                          size_t workspace_bytes, fk_stream s);
+/* A token drawn from each row of logits (bf16, row_stride apart).  With w_i = exp((x_i - max x) / T), the tokens in the order of their logits, the
+ * largest first, ties to the lower token: the first top_k are taken; of what they weigh together, W_k, the shortest run from the first on that weighs
+ * top_p * W_k at least; of that, those with w_i >= min_p.  tokens[r] is the first whose running sum is above u * W, W the sum of what is left.  The settings
+ * are device arrays of one value a row; NULL: T 1, top_k 0, top_p 1, min_p 0, which leave all.  The largest always stays.  T not above 0: the
+ * largest, the lowest token of several; top_k 0 or beyond the vocabulary: all; top_p not below 1: all; min_p not above 0: all, above 1: as 1; u outside of
+ * [0, 1): as the nearest inside, NaN as 0.  logprobs (may be NULL): log softmax(x) of the token, at T = 1, nothing cut.
+ * Weights are formed in 64 bits and held as integers in units of 2^-(62 - ceil(log2 vocab)) of the largest (2^-44 for 151936 tokens): sums do not depend
+ * on their order, a row's token not on the other rows.  -inf and NaN logits are never drawn; where a row has nothing else its token is 0 and its
+ * logprob -inf.  +inf logits share all of the weight.  Outputs overlap nothing else.  vocab up to 2^24, rows up to 65535.  workspace:
+ * fk_sample_workspace_bytes(), zeroed once and left ready by each launch; launches that share it must not overlap. */
+fk_status fk_sample_workspace_bytes(uint32_t rows, uint32_t vocab, size_t *bytes);
+fk_status fk_sample(const uint16_t *logits, size_t row_stride, uint32_t rows, uint32_t vocab, const float *temperature,
+                    const uint32_t *top_k, const float *top_p, const float *min_p, const float *u, uint32_t *tokens,
+                    float *logprobs, void *workspace, size_t workspace_bytes, fk_stream s);
 /* Rows of per-beam state follow the beams that were chosen: dst row g * n_out + i becomes src row g * beams + parents[g * n_out + i], rows of
  * row_bytes (any number) that lie src_stride / dst_stride bytes apart (a column of a history, part of a wider state).  dst
  * may be src where n_out == beams and the strides are the same (rows are then exchanged in place); otherwise what the two span
