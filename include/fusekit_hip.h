@@ -702,9 +702,9 @@ fk_status fk_beam_select(const uint16_t *logits, size_t row_stride, const float 
  * top_p * W_k at least; of that, those with w_i >= min_p.  tokens[r] is the first whose running sum is above u * W, W the sum of what is left.  The settings
  * are device arrays of one value a row; NULL: T 1, top_k 0, top_p 1, min_p 0, which leave all.  The largest always stays.  T not above 0: the
  * largest, the lowest token of several; top_k 0 or beyond the vocabulary: all; top_p not below 1: all; min_p not above 0: all, above 1: as 1; u outside of
- * [0, 1): as the nearest inside, NaN as 0.  logprobs (may be NULL): log softmax(x) of the token, at T = 1, nothing cut.
- * Weights are formed in 64 bits and held as integers in units of 2^-(62 - ceil(log2 vocab)) of the largest (2^-44 for 151936 tokens): sums do not depend
- * on their order, a row's token not on the other rows.  -inf and NaN logits are never drawn; where a row has nothing else its token is 0 and its
+ * [0, 1): 0 or 1 - 2^-24, NaN as 0.  logprobs (may be NULL): log softmax(x) of the token, at T = 1, nothing cut.
+ * Weights and sums are 64-bit; tokens of one logit are counted and weighed together, so that a row's token does not depend on the other rows or on
+ * how rows are cut. -inf and NaN logits are never drawn; where a row has nothing else its token is 0 and its
  * logprob -inf.  +inf logits share all of the weight.  Outputs overlap nothing else.  vocab up to 2^24, rows up to 65535.  workspace:
  * fk_sample_workspace_bytes(), zeroed once and left ready by each launch; launches that share it must not overlap. */
 fk_status fk_sample_workspace_bytes(uint32_t rows, uint32_t vocab, size_t *bytes);

@@ -28,8 +28,8 @@ def sample(logits, t, k, p, m, u):
     least = min(np.float64(m), 1.0) if m > 0 else 0.0
     order, w = order[w >= least], w[w >= least]
     upto = np.cumsum(w)
-    u = np.float64(u) if u > 0 else 0.0                                  # (NaN as 0)
-    at = min(int(np.searchsorted(upto, u * upto[-1], side="right")), int(np.flatnonzero(w)[-1]))
+    u = min(np.float64(u), 1 - 2.0 ** -24) if u > 0 else 0.0             # (the nearest fp32 value in [0, 1); NaN as 0)
+    at = int(np.searchsorted(upto, u * upto[-1], side="right"))
     return int(order[at]), float(lp[order[at]])
 
 

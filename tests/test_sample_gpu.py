@@ -1,8 +1,7 @@
 """Tokens drawn from logits (fk_sample) against a plain statement in 64 bits.
 
-Tolerances.  A token is a whole number and has to be the plain statement's: its weights are off by half a unit of 2^-44 or less of the largest, so that a
-random number has to lie within some 1e-9 of a border for the two to differ.  A log probability is rounded once, 2^-24 of it; its sum is off by vocab *
-2^-(63 - ceil(log2 vocab)) of the largest weight at most, 2^-27 for 151851 tokens."""
+Tolerances.  A token is a whole number and has to be the plain statement's: both form weights and sums in 64 bits, so that a random number has to lie within
+some 1e-13 of a border for the two to differ.  A log probability is rounded once, 2^-24 of it; in 64 bits it is off by far less than 2^-26."""
 import numpy as np
 import pytest
 
@@ -232,3 +231,44 @@ def test_captured_and_on_two_streams(fk, stream):  # noqa: F811
         two.check()
     g.free()
     h.free()
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 262145), (3, 300001), (1, 1 << 21)])
+def test_vocabularies_of_more_groups_than_a_row_has(fk, rows, vocab):
+    Draw(fk, normal(61, rows, vocab), pad=1, seed=vocab, **mixed(61, rows)).run().check()
+    flat = normal(62, rows, vocab, std=0.01)
+    Draw(fk, flat, seed=vocab, u=[0.1, 0.5, 0.97][:rows]).run().check()
+
+
+def test_many_rows_of_a_large_vocabulary(fk):
+    """More rows than the device has CUs, of more than 2^20 tokens."""
+    rows, vocab = 257, (1 << 20) + 5
+    one = normal(63, 1, vocab)
+    d = Draw(fk, np.repeat(one[:, :64], rows, 0), **mixed(63, rows))
+    d.vocab, d.stride = vocab, 0                  # (the whole rows: made on the device, one after the other)
+    d.logits = fk.DeviceBuffer(2 * rows * (vocab + 3))
+    row = fk.DeviceBuffer.from_numpy(np.concatenate([one[0], [0x7F7F] * 3]).astype(np.uint16))
+    same = fk.zeros(4 * rows)
+    for at in range(0, rows, 64):
+        n = min(64, rows - at)
+        fk.beam_reorder(row, d.logits.ptr + 2 * at * (vocab + 3), 2 * (vocab + 3), same, 1, 1, n)
+    d.stride, d.ws = vocab + 3, fk.zeros(fk.sample_workspace_bytes(rows, vocab))
+    d.run()
+    fk.sync()
+    tokens, logprobs = d.got()
+    x = oracle.bf16_to_f32(one[0]).astype(np.float64)
+    for i in list(range(0, rows, 37)) + [rows - 1]:
+        t, lp = sample(x, *(d.v[n][i] for n in NAMES))
+        assert tokens[i] == t and abs(logprobs[i] - lp) <= 2.0 ** -24 * abs(lp) + 2.0 ** -26, i
+
+
+def test_few_tokens_that_min_p_cuts(fk):
+    """A handful of logits far apart: the cut falls where no logit is, and the next one lies many bins on."""
+    bits = np.full((300, 500), 0xFF7F, np.uint16)
+    r = rng(64)
+    for i in range(300):
+        at = r.choice(500, r.integers(1, 9), replace=False)
+        bits[i, at] = oracle.f32_to_bf16((r.uniform(-1, 1, len(at)) * 10.0 ** r.uniform(-8, 2, len(at))).astype(np.float32))
+    for rows in (300, 20):
+        Draw(fk, bits[:rows], min_p=r.uniform(0, 1, rows), temperature=10.0 ** r.uniform(-3, 2, rows), top_k=r.integers(0, 6, rows)).run().check()
+        Draw(fk, bits[:rows], top_p=r.uniform(0, 1, rows), temperature=10.0 ** r.uniform(-3, 2, rows)).run().check()
