@@ -47,15 +47,22 @@ __device__ __forceinline__ float paged_inverse(float l, uint32_t limit) {
     return __builtin_expect(f > 0x1p-60f && f < 0x1p60f, 1) ? f : limit ? __builtin_nanf("") : 0.f;
 }
 
+// Sinks are a matter of the kernel's type: kept at run time, none of them cost a chunk of 512 rows behind 2500 positions with a window of 2000 41.8 us for
+// 38.5 (the registers that hold addresses go to them).
+template <bool SINKS>
+__device__ __forceinline__ uint32_t paged_sinks(const SdpaPagedArgs& a) {
+    return SINKS ? a.sinks : 0u;
+}
+
 // ---- one row of one head by a wave: positions in the order they lie, what the row does not see is not touched ----
 // The statement of the operator as it stands; the tiles below come here for a column whose sums are not finite, since a zero
 // probability times an infinity that other rows of the tile see is no number.
-template <int D>
+template <int D, bool SINKS>
 __device__ __forceinline__ void paged_row(const SdpaPagedArgs& a, uint32_t seq, const PagedSeq& s, uint32_t place, uint32_t head, uint32_t lane) {
     const uint32_t kvh = head / a.group, row = s.row0 + place, page_rows = 1u << a.b.page_shift;
     const uint32_t end = paged_limit(s, place);
     const uint32_t first = a.window && end > a.window ? end - a.window : 0u;
-    const uint32_t sinks = a.sinks < first ? a.sinks : first, gap = first - sinks, seen = end - gap;   // the positions seen: sinks, then from `first` on
+    const uint32_t sinks = paged_sinks<SINKS>(a) < first ? paged_sinks<SINKS>(a) : first, gap = first - sinks, seen = end - gap;   // the positions seen: sinks, then from `first` on
     const uint16_t* qr = a.q + (size_t)row * a.q_stride + (size_t)head * D;
     constexpr int DL = D / 64;
     uint32_t bad = 0;
@@ -114,7 +121,7 @@ struct PagedItem {
     bool any;
 };
 // FEW: a launch of single tokens only.  TILES: `index` counts tiles, not items.
-template <bool FEW, uint32_t COLS, bool TILES = false>
+template <bool FEW, uint32_t COLS, bool SINKS, bool TILES = false>
 __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t index, uint32_t lane) {
     constexpr uint32_t STEP = FEW ? kFewRound : kTileStep;
     const uint32_t n_kv = a.b.n_kv;
@@ -126,7 +133,7 @@ __device__ __forceinline__ PagedItem paged_item(const SdpaPagedArgs& a, uint32_t
         uint32_t seen = s.len;
         if (a.window) {
             const uint32_t span = COLS / a.group + 2u;   // rows of a tile, at most
-            const uint64_t w = (uint64_t)a.window + a.sinks + (s.rows < span ? s.rows : span) + (a.sinks ? 2u * STEP : STEP) - 1u;
+            const uint64_t w = (uint64_t)a.window + paged_sinks<SINKS>(a) + (s.rows < span ? s.rows : span) + (SINKS ? 2u * STEP : STEP) - 1u;
             seen = w < seen ? (uint32_t)w : seen;
         }
         return (seen + STEP - 1u) / STEP;
@@ -262,14 +269,14 @@ struct PagedRange {
     uint32_t near, gap;
     __device__ __forceinline__ uint32_t step(uint32_t n) const { return n < near ? n : n + gap; }
 };
-template <uint32_t STEP>
+template <uint32_t STEP, bool SINKS>
 __device__ __forceinline__ PagedRange paged_range(const SdpaPagedArgs& a, const PagedItem& it, uint32_t e_tile, uint32_t e_last) {
     auto limit_of = [&](uint32_t place) { return paged_limit(it.s, place); };
     PagedRange r;
     r.kv_end = __builtin_amdgcn_readfirstlane(limit_of(e_last / a.group));
     const uint32_t first = limit_of(e_tile / a.group);
     const uint32_t step0 = __builtin_amdgcn_readfirstlane((a.window && first > a.window ? first - a.window : 0u) / STEP);
-    const uint32_t sink_steps = a.sinks / STEP + (a.sinks % STEP ? 1u : 0u);
+    const uint32_t sinks = paged_sinks<SINKS>(a), sink_steps = sinks / STEP + (sinks % STEP ? 1u : 0u);
     r.near = sink_steps < step0 ? sink_steps : step0;
     r.gap = step0 - r.near;
     r.steps = (r.kv_end + STEP - 1u) / STEP - (r.kv_end ? r.gap : 0u);
@@ -295,7 +302,7 @@ __device__ __forceinline__ void paged_store_part(const SdpaPagedArgs& a, const P
     }
 }
 // Where it is whole: outputs.
-template <int D>
+template <int D, bool SINKS>
 __device__ __forceinline__ void paged_store_columns(const SdpaPagedArgs& a, const PagedItem& it, const float* ob, uint32_t et, uint32_t live, uint32_t lane) {
     constexpr uint32_t OS = D + 4, VP = D / 8;
     const uint32_t G = a.group;
@@ -316,7 +323,7 @@ __device__ __forceinline__ void paged_store_columns(const SdpaPagedArgs& a, cons
     }
     for (; again; again &= again - 1u) {
         const uint32_t ec = et + (uint32_t)__builtin_ctz(again), pl = ec / G;
-        paged_row<D>(a, it.seq, it.s, pl, it.kvh * G + (ec - pl * G), lane);
+        paged_row<D, SINKS>(a, it.seq, it.s, pl, it.kvh * G + (ec - pl * G), lane);
     }
 }
 
@@ -338,7 +345,7 @@ constexpr uint32_t tile_lds_bytes(uint32_t d, uint32_t split) {
     return stage > outb ? stage : outb;
 }
 
-template <int D, bool CAP, uint32_t SPLIT>
+template <int D, bool CAP, uint32_t SPLIT, bool SINKS>
 __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedItem& it, uint32_t lane) {
     constexpr int KB = D / 16, DT = D / 32, VP = D / 8;
     constexpr uint32_t COLS = kTileCols / SPLIT, STEP = kTileStep * SPLIT;           // of a block: columns, positions a step
@@ -354,7 +361,8 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
     auto limit_of = [&](uint32_t place) { return paged_limit(it.s, place); };                              // positions a row may see end here
     auto low_of = [&](uint32_t limit) { return a.window && limit > a.window ? limit - a.window : 0u; };                           // and begin here
     const uint32_t e_tile = it.tile * COLS, e_last = columns - e_tile < COLS ? columns - 1u : e_tile + COLS - 1u;
-    const PagedRange range = paged_range<STEP>(a, it, e_tile, e_last);
+    const uint32_t sinks = paged_sinks<SINKS>(a);
+    const PagedRange range = paged_range<STEP, SINKS>(a, it, e_tile, e_last);
     const uint32_t kv_end = range.kv_end, n_active = range.n_active;
     if (it.split >= n_active) return;
     const uint32_t begin = __builtin_amdgcn_readfirstlane(it.split * range.per);
@@ -452,7 +460,7 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
             if (step + 2u < stop) next = pages_of(step + 2u);
         }
         const uint32_t kv0 = range.step(step) * STEP + my_half * kTileStep;                   // this wave's 64 positions
-        if (kv0 >= last_limit || (kv0 + kTileStep <= first_low && kv0 >= a.sinks)) continue;   // nothing that a row of this wave sees
+        if (kv0 >= last_limit || (kv0 + kTileStep <= first_low && kv0 >= sinks)) continue;   // nothing that a row of this wave sees
         const unsigned char *ks = lds + stage * STAGE + my_half * kTileStep * ROW, *vs = ks + TILE;
         // (two of the eight pairs of fragments ahead of their matrix instructions; all of them first took 1 % longer of two chunks of 2048 rows, 2 % with a window)
         pf_u32x4_t kf[3][2];
@@ -496,13 +504,13 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
                 for (int r = 0; r < 16; ++r)
                     s[t][r] = fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[t][r] * turn2)), cap2);
         }
-        if (kv0 + kTileStep > first_limit || kv0 < last_low) {
+        if (kv0 + kTileStep > first_limit || (kv0 < last_low && kv0 + kTileStep > sinks)) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const uint32_t kv = kv0 + (uint32_t)(t * 32 + r % 4 + 8 * (r / 4)) + 4u * kb;
-                    if (kv >= q_limit || (kv < q_low && kv >= a.sinks)) s[t][r] = -INFINITY;
+                    if (kv >= q_limit || (kv < q_low && kv >= sinks)) s[t][r] = -INFINITY;
                 }
         }
         // the softmax reference moves only when a step's maximum outgrows it by 2^8
@@ -572,7 +580,7 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
                 make_float4(oacc[i][4 * g + 0] * f, oacc[i][4 * g + 1] * f, oacc[i][4 * g + 2] * f, oacc[i][4 * g + 3] * f);
     if constexpr (SPLIT == 1) {
         wave_lds_order();
-        if (whole) paged_store_columns<D>(a, it, ob, e0, live, lane);
+        if (whole) paged_store_columns<D, SINKS>(a, it, ob, e0, live, lane);
         else paged_store_part<D>(a, it, ob, wave * 32u, live, m_run, l_run, lane);
     } else {   // the two waves of a column tile join their halves, 16 columns each
         float* const ml = all + 4u * 32u * OS;   // [wave][column] reference, sum
@@ -592,7 +600,7 @@ __device__ __forceinline__ void paged_tile(const SdpaPagedArgs& a, const PagedIt
             *reinterpret_cast<float4*>(ob + c * OS + d) = make_float4(fmaf(u.x, w0, v.x * w1), fmaf(u.y, w0, v.y * w1), fmaf(u.z, w0, v.z * w1), fmaf(u.w, w0, v.w * w1));
         }
         wave_lds_order();
-        paged_store_columns<D>(a, it, ob + c0 * OS, e0 + c0, mine, lane);
+        paged_store_columns<D, SINKS>(a, it, ob + c0 * OS, e0 + c0, mine, lane);
     }
 }
 
@@ -666,14 +674,14 @@ __device__ __forceinline__ void paged_merge_columns(const __amdgpu_buffer_rsrc_t
 // The parts of cut tiles of 128 columns joined, in a launch of its own: a block takes 16 columns of a tile, a wave one at a time.  (By the tile's last
 // item, as single tokens are, one CU reads all parts, 66 KB each: a chunk of 64 rows behind 8000 positions, 16 parts a tile, 45 us.)
 constexpr uint32_t kMergeCols = 16;
-template <int D>
+template <int D, bool SINKS>
 __global__ __launch_bounds__(256) void sdpa_paged_merge_kernel(const SdpaPagedArgs a) {
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const PagedItem it = paged_item<false, kTileCols, true>(a, blockIdx.x / (kTileCols / kMergeCols), lane);
+    const PagedItem it = paged_item<false, kTileCols, SINKS, true>(a, blockIdx.x / (kTileCols / kMergeCols), lane);
     if (!it.any) return;
     const uint32_t G = a.group, columns = it.s.rows * G, e_tile = it.tile * kTileCols, c0 = blockIdx.x % (kTileCols / kMergeCols) * kMergeCols;
     if (columns <= kFewMost || e_tile + c0 >= columns) return;
-    const PagedRange range = paged_range<kTileStep>(a, it, e_tile, columns - e_tile < kTileCols ? columns - 1u : e_tile + kTileCols - 1u);
+    const PagedRange range = paged_range<kTileStep, SINKS>(a, it, e_tile, columns - e_tile < kTileCols ? columns - 1u : e_tile + kTileCols - 1u);
     if (range.n_active == 1u) return;
     constexpr uint32_t SLOT = kTileCols * (D + 2u) * 4u;
     const __amdgpu_buffer_rsrc_t mem = __builtin_amdgcn_make_buffer_rsrc(a.partials, 0, (int)(a.slots * SLOT), 0x27000);
@@ -690,7 +698,7 @@ __global__ __launch_bounds__(256) void sdpa_paged_merge_kernel(const SdpaPagedAr
     auto done = [&](uint32_t c) {
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd) != 0, 0)) {
             const uint32_t e = e_tile + c, place = e / G;
-            paged_row<D>(a, it.seq, it.s, place, it.kvh * G + (e - place * G), lane);
+            paged_row<D, SINKS>(a, it.seq, it.s, place, it.kvh * G + (e - place * G), lane);
             odd = false;
         }
     };
@@ -710,7 +718,7 @@ constexpr uint32_t few_lds_bytes(uint32_t d) {
     return (stages > meet ? stages : meet) + 16u;   // and two words for the block
 }
 
-template <int D, bool CAP, bool WIDE>
+template <int D, bool CAP, bool WIDE, bool SINKS>
 __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedItem& it, uint32_t lane) {
     constexpr uint32_t ROW = D * 2u, P = D / 8u, KT = kFewStep * ROW, STAGE = 2u * KT, RPI = 1024u / ROW;   // pieces of a row; rows of a request
     constexpr int REQ = (int)(KT / 1024u), KS = D / 32, DT = D / 16, PARTS = WIDE ? 2 : 1;
@@ -723,14 +731,14 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
     const uint32_t G = a.group, e0 = it.tile * kFewCols, left_cols = it.s.rows * G - e0, columns = left_cols < kFewCols ? left_cols : kFewCols;   // of this tile
     auto limit_of = [&](uint32_t place) { return paged_limit(it.s, place); };
     auto low_of = [&](uint32_t limit) { return a.window && limit > a.window ? limit - a.window : 0u; };
-    const PagedRange range = paged_range<kFewRound>(a, it, e0, e0 + columns - 1u);
+    const PagedRange range = paged_range<kFewRound, SINKS>(a, it, e0, e0 + columns - 1u);
     const uint32_t kv_end = range.kv_end, n_active = range.n_active, lim_lo = __builtin_amdgcn_readfirstlane(limit_of(e0 / G));
     const uint32_t low_hi = __builtin_amdgcn_readfirstlane(low_of(kv_end));
     if (it.split >= n_active) return;
     const uint32_t round0 = it.split * range.per;
     uint32_t rounds = range.steps < round0 + range.per ? range.steps - round0 : range.per;   // of this item
     // (of the sinks' last round a wave whose positions lie behind them sees nothing, and leaves it out)
-    const uint32_t near_wave = a.sinks > wave * kFewStep ? (a.sinks - wave * kFewStep + kFewRound - 1u) / kFewRound : 0u;
+    const uint32_t sinks = paged_sinks<SINKS>(a), near_wave = sinks > wave * kFewStep ? (sinks - wave * kFewStep + kFewRound - 1u) / kFewRound : 0u;
     const bool leaves = near_wave < range.near && near_wave >= round0 && near_wave - round0 < rounds;
     rounds -= leaves ? 1u : 0u;
     auto at_round = [&](uint32_t j) {
@@ -842,11 +850,11 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[i] * turn2)), cap2);
         }
-        if (kv0 + kFewStep > lim_lo || kv0 < low_hi) {
+        if (kv0 + kFewStep > lim_lo || (kv0 < low_hi && kv0 + kFewStep > sinks)) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const uint32_t kv = kv0 + (uint32_t)(i / 4) * 16u + 4u * g + (uint32_t)(i % 4);
-                if (kv >= q_limit || (kv < q_low && kv >= a.sinks)) x[i] = -INFINITY;
+                if (kv >= q_limit || (kv < q_low && kv >= sinks)) x[i] = -INFINITY;
             }
         }
         float mx = x[0];
@@ -988,24 +996,24 @@ __device__ __forceinline__ void paged_few(const SdpaPagedArgs& a, const PagedIte
     }
     __syncthreads();
     for (uint32_t again = word[1], c = 0; again; again >>= 1, ++c)
-        if ((again & 1u) && c % 4u == wave) paged_row<D>(a, it.seq, it.s, (e0 + c) / G, it.kvh * G + (e0 + c) % G, lane);
+        if ((again & 1u) && c % 4u == wave) paged_row<D, SINKS>(a, it.seq, it.s, (e0 + c) / G, it.kvh * G + (e0 + c) % G, lane);
 }
 
 // Chunks and single tokens together: each sequence by its kind, in one launch, so that what is bound by the matrix units runs beside what is bound by the
 // bytes.
-template <int D, bool CAP, uint32_t SPLIT>
+template <int D, bool CAP, uint32_t SPLIT, bool SINKS>
 __global__ __launch_bounds__(256, 2) void sdpa_paged_kernel(const SdpaPagedArgs a) {
     const uint32_t lane = threadIdx.x & 63u;
-    const PagedItem it = paged_item<false, kTileCols / SPLIT>(a, blockIdx.x, lane);
+    const PagedItem it = paged_item<false, kTileCols / SPLIT, SINKS>(a, blockIdx.x, lane);
     if (!it.any) return;
-    if (it.s.rows * a.group <= kFewMost) paged_few<D, CAP, true>(a, it, lane);
-    else paged_tile<D, CAP, SPLIT>(a, it, lane);
+    if (it.s.rows * a.group <= kFewMost) paged_few<D, CAP, true, SINKS>(a, it, lane);
+    else paged_tile<D, CAP, SPLIT, SINKS>(a, it, lane);
 }
-template <int D, bool CAP, bool WIDE>
+template <int D, bool CAP, bool WIDE, bool SINKS>
 __global__ __launch_bounds__(256, 2) void sdpa_paged_few_kernel(const SdpaPagedArgs a) {
     const uint32_t lane = threadIdx.x & 63u;
-    const PagedItem it = paged_item<true, kFewCols>(a, blockIdx.x, lane);
-    if (it.any) paged_few<D, CAP, WIDE>(a, it, lane);
+    const PagedItem it = paged_item<true, kFewCols, SINKS>(a, blockIdx.x, lane);
+    if (it.any) paged_few<D, CAP, WIDE, SINKS>(a, it, lane);
 }
 
 namespace {
@@ -1094,16 +1102,25 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     a.counters = static_cast<uint32_t*>(workspace);
     a.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kPagedCounterBytes);
     a.slots = p.slots; a.target = p.target; a.min_steps = p.min_steps;
-    const void* tile[2][2][2] = {
-        {{reinterpret_cast<const void*>(&sdpa_paged_kernel<64, false, 1>), reinterpret_cast<const void*>(&sdpa_paged_kernel<64, false, 2>)},
-         {reinterpret_cast<const void*>(&sdpa_paged_kernel<64, true, 1>), reinterpret_cast<const void*>(&sdpa_paged_kernel<64, true, 2>)}},
-        {{reinterpret_cast<const void*>(&sdpa_paged_kernel<128, false, 1>), reinterpret_cast<const void*>(&sdpa_paged_kernel<128, false, 2>)},
-         {reinterpret_cast<const void*>(&sdpa_paged_kernel<128, true, 1>), reinterpret_cast<const void*>(&sdpa_paged_kernel<128, true, 2>)}}};
-    const void* few[2][2][2] = {
-        {{reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, false, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, false, true>)},
-         {reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, true, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, true, true>)}},
-        {{reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, true>)},
-         {reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, true>)}}};
+    // [sinks][D == 128][softcap][split or wide]
+    const void* tile[2][2][2][2] = {
+        {{{reinterpret_cast<const void*>(&sdpa_paged_kernel<64, false, 1, false>), reinterpret_cast<const void*>(&sdpa_paged_kernel<64, false, 2, false>)},
+          {reinterpret_cast<const void*>(&sdpa_paged_kernel<64, true, 1, false>), reinterpret_cast<const void*>(&sdpa_paged_kernel<64, true, 2, false>)}},
+         {{reinterpret_cast<const void*>(&sdpa_paged_kernel<128, false, 1, false>), reinterpret_cast<const void*>(&sdpa_paged_kernel<128, false, 2, false>)},
+          {reinterpret_cast<const void*>(&sdpa_paged_kernel<128, true, 1, false>), reinterpret_cast<const void*>(&sdpa_paged_kernel<128, true, 2, false>)}}},
+        {{{reinterpret_cast<const void*>(&sdpa_paged_kernel<64, false, 1, true>), reinterpret_cast<const void*>(&sdpa_paged_kernel<64, false, 2, true>)},
+          {reinterpret_cast<const void*>(&sdpa_paged_kernel<64, true, 1, true>), reinterpret_cast<const void*>(&sdpa_paged_kernel<64, true, 2, true>)}},
+         {{reinterpret_cast<const void*>(&sdpa_paged_kernel<128, false, 1, true>), reinterpret_cast<const void*>(&sdpa_paged_kernel<128, false, 2, true>)},
+          {reinterpret_cast<const void*>(&sdpa_paged_kernel<128, true, 1, true>), reinterpret_cast<const void*>(&sdpa_paged_kernel<128, true, 2, true>)}}}};
+    const void* few[2][2][2][2] = {
+        {{{reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, false, false, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, false, true, false>)},
+          {reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, true, false, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, true, true, false>)}},
+         {{reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, false, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, true, false>)},
+          {reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, false, false>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, true, false>)}}},
+        {{{reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, false, false, true>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, false, true, true>)},
+          {reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, true, false, true>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<64, true, true, true>)}},
+         {{reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, false, true>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, false, true, true>)},
+          {reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, false, true>), reinterpret_cast<const void*>(&sdpa_paged_few_kernel<128, true, true, true>)}}}};
     // Positions that a tile can see, in steps.  Chunks of up to 8 steps are not cut: the merge costs what it saves (a prompt of 512 rows, 32 / 8 heads x
     // 128: 18 us whole, 24 in halves).
     const uint32_t step = p.few ? kFewRound : kTileStep, span = (p.few ? kFewCols : kTileCols) / a.group + 2u;
@@ -1129,7 +1146,7 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
         a.target = kFewTarget;
         a.min_steps = kFewLeast;
     }
-    l->func = p.few ? few[D == 128][softcap > 0.f][batch->max_rows * (n_heads / n_kv) > 8u] : tile[D == 128][softcap > 0.f][split];
+    l->func = p.few ? few[a.sinks > 0][D == 128][softcap > 0.f][batch->max_rows * (n_heads / n_kv) > 8u] : tile[a.sinks > 0][D == 128][softcap > 0.f][split];
     // (no more blocks than there can be items: one that finds none costs what it takes to look)
     a.blocks = (uint32_t)(cut && !a.compact ? std::min<uint64_t>(p.slots, p.tiles * splits) : split ? halves : p.tiles + (cut || a.only_few ? a.target : 0u));
     l->grid = dim3(a.blocks, 1, 1);
@@ -1140,7 +1157,8 @@ fk_status plan_sdpa_paged(const uint16_t* q, uint32_t q_stride, uint16_t* out, u
     l->set_args(a);
     if (!p.few && cut) {
         Launch m;
-        m.func = D == 64 ? reinterpret_cast<const void*>(&sdpa_paged_merge_kernel<64>) : reinterpret_cast<const void*>(&sdpa_paged_merge_kernel<128>);
+        if (a.sinks) m.func = D == 64 ? reinterpret_cast<const void*>(&sdpa_paged_merge_kernel<64, true>) : reinterpret_cast<const void*>(&sdpa_paged_merge_kernel<128, true>);
+        else m.func = D == 64 ? reinterpret_cast<const void*>(&sdpa_paged_merge_kernel<64, false>) : reinterpret_cast<const void*>(&sdpa_paged_merge_kernel<128, false>);
         m.grid = dim3((uint32_t)p.tiles * (kTileCols / kMergeCols), 1, 1);
         m.block = dim3(256, 1, 1);
         m.set_args(a);
