@@ -7,6 +7,9 @@
   generate --model DIR --ids 1,2,3 --beams N [--eos T]
                                          beam search over a paged cache (dense decoders): the N likeliest continuations
                                          and the sums of their log probabilities
+  generate --model DIR --ids 1,2,3 --temperature T [--top-k K] [--top-p P] [--min-p M] [--seed S] [--eos T]
+                                         tokens drawn at random (dense decoders, over a paged cache); the same seed draws the
+                                         same tokens
   export-random --out DIR [--bits 4] [--layers 2] [--moe] ...
                                          write a small random-init model in the mlx-lm file layout (--moe: a
                                          mixture-of-experts model in the deepseek_v2 layout; generate / patch
@@ -36,7 +39,12 @@ def main() -> int:
     g.add_argument("--capacity", type=int, default=1024)
     g.add_argument("--artifact", default=None, help="directory written by `patch`")
     g.add_argument("--beams", type=int, default=0, help="beam search with this many beams (1 to 64)")
-    g.add_argument("--eos", type=int, default=None, help="with --beams: the token that ends a continuation")
+    g.add_argument("--eos", type=int, default=None, help="with --beams or --temperature: the token that ends a continuation")
+    g.add_argument("--temperature", type=float, default=None, help="draw tokens from the softmax of logits / TEMPERATURE (0: the likeliest)")
+    g.add_argument("--top-k", type=int, default=None, help="with --temperature: of the K likeliest tokens")
+    g.add_argument("--top-p", type=float, default=None, help="with --temperature: of the likeliest tokens that have this probability together, in (0, 1]")
+    g.add_argument("--min-p", type=float, default=None, help="with --temperature: of the tokens that are this likely against the likeliest, in [0, 1]")
+    g.add_argument("--seed", type=int, default=None, help="with --temperature: of the random numbers (0)")
     pa = sub.add_parser("patch")
     pa.add_argument("--model", required=True)
     pa.add_argument("--out", default=None)
@@ -63,8 +71,27 @@ def main() -> int:
     if args.cmd == "generate":
         if not 0 <= args.beams <= 64:
             ap.error("--beams: 1 to 64")
-        if args.eos is not None and not args.beams:
-            ap.error("--eos ends the continuations of a beam search: it goes with --beams")
+        if args.temperature is None:
+            for name in ("top_k", "top_p", "min_p", "seed"):
+                if getattr(args, name) is not None:
+                    ap.error(f"--{name.replace('_', '-')} is of a draw: it goes with --temperature")
+            if args.eos is not None and not args.beams:
+                ap.error("--eos ends the continuations of a beam search or of drawn tokens: it goes with --beams or --temperature")
+        else:
+            if args.beams or args.artifact:
+                ap.error("--temperature draws tokens: it goes without --beams and runs from the checkpoint, not from an artifact")
+            if not 0.0 <= args.temperature < float("inf"):
+                ap.error("--temperature: finite, not negative")
+            if args.top_k is not None and not 0 <= args.top_k < 1 << 32:
+                ap.error("--top-k: a count of tokens (0: all)")
+            if args.top_p is not None and not 0.0 < args.top_p <= 1.0:
+                ap.error("--top-p: above 0, 1 at most")
+            if args.min_p is not None and not 0.0 <= args.min_p <= 1.0:
+                ap.error("--min-p: 0 to 1")
+            if args.seed is not None and not 0 <= args.seed < 1 << 64:
+                ap.error("--seed: 0 up to 2^64 - 1")
+            if args.max_tokens < 1:
+                ap.error("--max-tokens: one at least")
     from . import native as fk
     if args.cmd == "info":
         t = fk.target_describe()
@@ -97,6 +124,8 @@ def main() -> int:
         from .moe_decoder import MoeRuntime
         if args.cmd == "generate" and args.beams:
             ap.error("--beams: beam search runs dense decoders")
+        if args.cmd == "generate" and args.temperature is not None:
+            ap.error("--temperature: tokens are drawn of dense decoders")
         cfg, w = load_moe_checkpoint(args.model, capacity=args.capacity)
         if args.cmd == "patch":
             rt = MoeRuntime(cfg, w)
@@ -134,6 +163,14 @@ def main() -> int:
         dec = PagedDecoder(cfg, w, pages, rows, max_rows=max(64, min(512, len(prompt))), max_seqs=args.beams)
         found = dec.beam_search(prompt, args.beams, args.max_tokens, args.eos)
         print(json.dumps({"beams": [{"tokens": t, "log_probability": round(p, 5)} for t, p in found]}))
+        return 0
+    if args.temperature is not None:
+        from .paged import PagedDecoder
+        rows = 16
+        dec = PagedDecoder(cfg, w, -(-(len(prompt) + args.max_tokens) // rows), rows, max_rows=max(64, min(512, len(prompt))), max_seqs=1)
+        toks = dec.sample([prompt], args.max_tokens, args.temperature, args.top_k or 0, 1.0 if args.top_p is None else args.top_p, args.min_p or 0.0,
+                          args.seed or 0, args.eos)[0]
+        print(json.dumps({"tokens": toks}))
         return 0
     if args.artifact:
         from .artifact import ArtifactRuntime

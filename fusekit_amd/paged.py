@@ -2,8 +2,8 @@
 
 PageAllocator keeps, on the host, which sequence has which pages: reference counts, a copy of the tail page where a shared one is about to be
 written, compaction.  It moves no memory: what has to be copied it returns as pairs for fk_pages_copy.  PagedDecoder holds the pools of a
-model's layers and runs batches over them; the kernels are rope_paged_store, sdpa_paged, beam_select, beam_reorder and those that
-prompt passes use.
+model's layers and runs batches over them; the kernels are rope_paged_store, sdpa_paged (sdpa_paged_sinks), beam_select, beam_reorder, paged_extend,
+sample and those that prompt passes use.
 """
 from __future__ import annotations
 
@@ -115,6 +115,20 @@ class PageAllocator:
         self.users[page] = 1
         return page
 
+    def adopt(self, seqs: Sequence[PagedSequence], lengths: Sequence[int], tables: np.ndarray, n_free: int) -> None:
+        """What launches of paged_extend did to `seqs` since their lengths, pages and the stack of free pages were handed to the device: the lengths they
+        have now, their rows of the tables and the free pages that are left.  Nothing else has happened to the pool meanwhile."""
+        taken = [[int(p) for p in row[len(s.pages):-(-int(length) // self.page_rows)]] for s, length, row in zip(seqs, lengths, tables)]
+        for seq in seqs:
+            self._mine(seq)
+        if sorted(p for pages in taken for p in pages) != sorted(self._free[n_free:]) or any(n < s.length for s, n in zip(seqs, lengths)):
+            raise RuntimeError("the device's pages are not the host's")
+        for seq, length, pages in zip(seqs, lengths, taken):
+            seq.pages.extend(pages)
+            seq.length = int(length)
+            self.users[pages] = 1
+        del self._free[n_free:]
+
     def truncate(self, seq: PagedSequence, length: int) -> None:
         """Drops the positions from `length` on."""
         self._mine(seq)
@@ -161,8 +175,9 @@ class PagedDecoder:
 
     def __init__(self, cfg: DecoderConfig, weights: DecoderWeights, n_pages: int, page_rows: int = 64, max_rows: int = 512, max_seqs: int = 64,
                  rope_dims: Optional[int] = None, interleaved: bool = False, rope: Optional[dict] = None, window: int = 0, softcap: float = 0.0,
-                 stream=None):
-        """rope: scaling and its numbers as native.rope_frequencies takes them; window, softcap: of every layer."""
+                 stream=None, sinks: int = 0):
+        """rope: scaling and its numbers as native.rope_frequencies takes them; window, softcap: of every layer; sinks: first positions that stay visible
+        besides the window."""
         if cfg.kv_bits:
             raise ValueError("pages hold a bf16 cache")
         if cfg.head_dim not in (64, 128) or cfg.n_kv < 1 or cfg.n_heads % cfg.n_kv:
@@ -175,9 +190,11 @@ class PagedDecoder:
             raise ValueError("rope_dims: a multiple of 16 up to head_dim, or 0")
         if not 0 <= window < 1 << 31 or not 0.0 <= softcap <= 1024.0:
             raise ValueError("window and softcap are not negative, softcap up to 1024 (0: none)")
+        if not 0 <= sinks < 1 << 31:
+            raise ValueError("sinks are not negative")
         self.cfg, self.w, self.stream = cfg, weights, stream
         self.pages = PageAllocator(n_pages, page_rows)
-        self.max_rows, self.max_seqs, self.window, self.softcap = max_rows, max_seqs, window, softcap
+        self.max_rows, self.max_seqs, self.window, self.sinks, self.softcap = max_rows, max_seqs, window, sinks, softcap
         self.interleaved, self.rope_dims = interleaved, cfg.head_dim if rope_dims is None else rope_dims
         c, R, S = cfg, max_rows, max_seqs
         self.page_bytes = c.n_kv * page_rows * c.head_dim * 2
@@ -209,7 +226,7 @@ class PagedDecoder:
     def forward(self, batch: Sequence[Tuple[PagedSequence, Sequence[int]]]) -> DeviceBuffer:
         """Each sequence takes its new tokens (one at least); returns the logits [len(batch), vocab], overwritten by the next call.  A call that raises
         leaves the sequences as they were.  Does not wait for the device: what a launch finds wrong in a batch is in `fault`, for native.paged_check
-        (beam_search and generate look at every step)."""
+        (beam_search and generate look at every step, sample at every round of steps)."""
         c = self.cfg
         seqs, tokens = [s for s, _ in batch], [list(t) for _, t in batch]
         n, rows = len(seqs), [len(t) for t in tokens]
@@ -230,7 +247,7 @@ class PagedDecoder:
 
     def _launch(self, seqs: List[PagedSequence], rows: List[int], flat: List[int]) -> DeviceBuffer:
         """The launches of forward(), for sequences that have room for their rows."""
-        c, w, st = self.cfg, self.w, self.stream
+        c, st = self.cfg, self.stream
         n, R = len(seqs), len(flat)
         starts = np.concatenate([[0], np.cumsum(rows)])
         stride = max(len(s.pages) for s in seqs)
@@ -240,7 +257,18 @@ class PagedDecoder:
         self.batch_words.upload(words)
         at = [self.batch_words.ptr + 4 * i for i in (0, n + 1, 2 * n + 1, 2 * n + 1 + R)]
         b = native.PagedBatch(at[0], at[1], at[3], stride, n, R, max(rows), max(s.length for s in seqs), self.fault)
-        native.embed_lookup_rows(w.mats["embed_tokens"], at[2], R, c.embed_scale, self.x, st)
+        self._layers(b, at[2])
+        last = self.x
+        if R > n:                                              # the last row of each sequence
+            last = self.last
+            for i in range(n):
+                native.copy(self.last.ptr + i * c.hidden * 2, self.x.ptr + (int(starts[i + 1]) - 1) * c.hidden * 2, c.hidden * 2, st)
+        return self._head(last, n)
+
+    def _layers(self, b: native.PagedBatch, tokens) -> None:
+        """A batch of rows from their tokens, on the device, to what the last layer leaves in self.x."""
+        c, w, st, R = self.cfg, self.w, self.stream, b.rows
+        native.embed_lookup_rows(w.mats["embed_tokens"], tokens, R, c.embed_scale, self.x, st)
         scale = float(c.head_dim) ** -0.5
         for l in range(c.n_layers):
             p = f"layers.{l}."
@@ -251,18 +279,21 @@ class PagedDecoder:
             norms = [vec("self_attn.q_norm"), vec("self_attn.k_norm")] if c.qk_norm else [None, None]
             native.rope_paged_store(self.q, c.n_q, self.k, c.n_kvd, self.v, c.n_kvd, self.q, c.n_q, c.n_heads, *norms, c.eps, self.rope_dims,
                                     self.interleaved, self.freq, b, self.layers[l], st)
-            native.sdpa_paged(self.q, c.n_q, self.att, c.n_q, c.n_heads, scale, self.softcap, self.window, b, self.layers[l], self.sdpa_ws,
-                              self.sdpa_ws.nbytes, st)
+            if self.sinks:
+                native.sdpa_paged_sinks(self.q, c.n_q, self.att, c.n_q, c.n_heads, scale, self.softcap, self.window, self.sinks, b, self.layers[l],
+                                        self.sdpa_ws, self.sdpa_ws.nbytes, st)
+            else:
+                native.sdpa_paged(self.q, c.n_q, self.att, c.n_q, c.n_heads, scale, self.softcap, self.window, b, self.layers[l], self.sdpa_ws,
+                                  self.sdpa_ws.nbytes, st)
             native.qgemm(m("self_attn.o_proj"), self.att, R, None, self.x, self.x2, self.ws, st)
             native.rmsnorm_rows(self.x2, vec("post_attention_layernorm"), c.eps, R, c.hidden, self.xn, st)
             native.qgemm_swiglu(m("mlp.gate_proj"), m("mlp.up_proj"), self.xn, R, c.swiglu_variant, self.mid, self.ws, st)
             native.qgemm(m("mlp.down_proj"), self.mid, R, None, self.x2, self.x, self.ws, st)
-        last = self.x
-        if R > n:                                              # the last row of each sequence
-            last = self.last
-            for i in range(n):
-                native.copy(self.last.ptr + i * c.hidden * 2, self.x.ptr + (int(starts[i + 1]) - 1) * c.hidden * 2, c.hidden * 2, st)
-        native.rmsnorm_rows(last, w.vecs["final_norm"], c.eps, n, c.hidden, self.xn, st)
+
+    def _head(self, last, n: int) -> DeviceBuffer:
+        """The logits of n rows of what the last layer left."""
+        c, st = self.cfg, self.stream
+        native.rmsnorm_rows(last, self.w.vecs["final_norm"], c.eps, n, c.hidden, self.xn, st)
         native.qgemm(self.head, self.xn, n, None, None, self.logits, self.ws, st)
         return self.logits
 
@@ -383,3 +414,104 @@ class PagedDecoder:
         finally:
             for s in seqs:
                 self.pages.release(s)
+
+    def sample(self, prompts: Sequence[Sequence[int]], max_tokens: int, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0,
+               eos: Optional[int] = None) -> List[List[int]]:
+        """Continuations of several prompts, decoded together, each token drawn as fk_sample draws it.  The settings are one value for all or one a
+        prompt; prompt i draws with random numbers of its own, from (seed, i).  A continuation ends behind `eos` or with max_tokens.
+
+        The steps run on the device, which makes the batches (paged_extend), takes free pages and hands a step's tokens to the next: without `eos` the
+        host does not wait between them.  With `eos` it looks after every 16 steps which have ended; those go no further then,
+        and what they drew behind `eos` is dropped.  A call that raises leaves pages and sequences as they were."""
+        c, pages = self.cfg, self.pages
+        prompts = [list(p) for p in prompts]
+        n = len(prompts)
+        if not 0 < n <= self.max_seqs or max_tokens < 1 or not all(prompts):
+            raise ValueError("one prompt at least, max_seqs at most, none empty, and a token at least")
+        if n > self.max_rows and max_tokens > 1:
+            raise ValueError("a step takes a row for every prompt: max_rows at most")
+        if not 0 <= seed < 1 << 64:
+            raise ValueError("a seed is a number of 64 bits, not negative")
+        settings = []
+        for name, value, word, sound in (("temperature", temperature, np.float32, lambda v: (v >= 0) & (v < np.inf)),
+                                         ("top_k", top_k, np.uint32, lambda v: (v >= 0) & (v < 1 << 32) & (v == np.floor(v))),
+                                         ("top_p", top_p, np.float32, lambda v: (v > 0) & (v <= 1)), ("min_p", min_p, np.float32, lambda v: (v >= 0) & (v <= 1))):
+            v = np.asarray(value, np.float64)
+            if v.shape not in ((), (n,)) or not sound(v).all():
+                raise ValueError(f"{name}: one for all or one a prompt; a temperature is finite and not negative, top_k a count (0: all), top_p in (0, 1], min_p in [0, 1]")
+            settings.append(np.broadcast_to(v, (n,)).astype(word))
+        held = lambda length: -(-length // pages.page_rows)
+        need = sum(held(len(p) + max_tokens - 1) for p in prompts)
+        if need > pages.free_pages:
+            raise OutOfPages(f"{need} pages wanted, {pages.free_pages} free")
+        draws = np.stack([np.random.Generator(np.random.PCG64([seed, i])).random(max_tokens, np.float32) for i in range(n)], 1)
+        ws = native.zeros(max(native.sample_workspace_bytes(r, c.vocab) for r in range(1, n + 1)))
+        seqs = [pages.new() for _ in prompts]
+        try:
+            start = _Steps(self, ws, settings, draws[:1], [0] * n)
+            for i, (s, p) in enumerate(zip(seqs, prompts)):
+                start.draw(self.prefill(s, p), 0, i, 1)
+            out = [[int(t)] for t in start.finish()[0]]
+            while True:
+                live = [i for i in range(n) if out[i][-1] != eos and len(out[i]) < max_tokens]
+                if not live:
+                    return out
+                done = len(out[live[0]])                       # (all that live have as many)
+                count = min(max_tokens - done, max_tokens if eos is None else self.LOOK)
+                steps = _Steps(self, ws, [v[live] for v in settings], draws[done:done + count, live], [out[i][-1] for i in live], [seqs[i] for i in live])
+                for j in range(count):
+                    steps.run(j)
+                for row in steps.finish():
+                    for i, t in zip(live, row):
+                        if out[i][-1] != eos:
+                            out[i].append(int(t))
+        finally:
+            for s in seqs:
+                pages.release(s)
+
+    LOOK = 16   # steps of sample() between two looks for `eos`
+
+
+class _Steps:
+    """Steps of PagedDecoder.sample for a number of sequences, one row each: what they read and write lies on the device, in one piece."""
+
+    def __init__(self, dec: PagedDecoder, ws: DeviceBuffer, settings, draws: np.ndarray, tokens: Sequence[int], seqs: Sequence[PagedSequence] = ()):
+        """settings: temperature, top_k, top_p and min_p of each sequence; draws: random numbers [steps, sequences]; tokens: what the first step reads."""
+        pages = dec.pages
+        self.dec, self.ws, self.seqs, self.shape = dec, ws, list(seqs), draws.shape
+        self.longest = max([s.length for s in seqs], default=0)
+        self.stride = -(-(self.longest + len(draws)) // pages.page_rows)
+        parts = [*settings, draws, tokens, np.zeros(draws.shape, np.uint32),                       # (the tokens drawn lie behind those read first)
+                 [s.length for s in seqs], pages.table(seqs, self.stride), pages._free + [0] * (pages.n_pages - len(pages._free)), [len(pages._free)],
+                 [0], np.zeros(len(seqs) + 1, np.uint32), np.zeros(len(seqs), np.uint32), np.zeros((len(seqs), self.stride), np.uint32)]
+        words = [(a if isinstance(a, np.ndarray) and a.dtype == np.float32 else np.asarray(a, np.uint32)).ravel().view(np.uint32) for a in parts]
+        self.mem = DeviceBuffer.from_numpy(np.concatenate(words))
+        self.at = np.concatenate([[0], np.cumsum([4 * len(w) for w in words])]).tolist()
+        place = [self.mem.ptr + a for a in self.at]
+        self.settings, self.draws, self.tokens = place[:4], place[4], place[5]
+        if seqs:
+            lengths, tables, free, n_free, counter, *self.batch = place[7:15]
+            self.requests = native.PagedRequests(None, None, len(seqs), lengths, lengths, tables, self.stride, free, n_free, n_free, counter)
+
+    def draw(self, logits, step: int, row: int, rows: int) -> None:
+        """Tokens of the sequences row .. row + rows - 1 from their logits."""
+        c, n, st = self.dec.cfg, self.shape[1], self.dec.stream
+        native.sample(logits, c.vocab, rows, c.vocab, *(p + 4 * row for p in self.settings), self.draws + 4 * (n * step + row),
+                      self.tokens + 4 * (n * (step + 1) + row), None, self.ws, self.ws.nbytes, st)
+
+    def run(self, step: int) -> None:
+        dec, n = self.dec, self.shape[1]
+        b = native.PagedBatch(*self.batch, self.stride, n, n, 1, self.longest + step + 1, dec.fault)
+        native.paged_extend(self.requests, b, dec.pages.n_pages, dec.pages.page_rows, None, dec.stream)
+        dec._layers(b, self.tokens + 4 * n * step)
+        self.draw(dec._head(dec.x, n), step, 0, n)
+
+    def finish(self) -> np.ndarray:
+        """Waits for the steps, hands what they took to the host's pages and returns the tokens drawn, [steps, sequences]."""
+        dec, at = self.dec, self.at
+        native.paged_check(dec.fault, dec.stream)
+        words = self.mem.to_numpy(np.uint32)
+        part = lambda i: words[at[i] // 4:at[i + 1] // 4]
+        if self.seqs:
+            dec.pages.adopt(self.seqs, part(7), part(8).reshape(-1, self.stride), int(part(10)[0]))
+        return part(6).reshape(self.shape)
