@@ -145,10 +145,16 @@ __device__ __forceinline__ void sample_load(const uint16_t* x, uint32_t at, uint
 }
 
 // One launch, a block for each piece of a row.  The piece's logits are counted in LDS; the blocks of a row add what they counted into its shared bins, and the
-// last of them, or the only one, forms the weights of the bins that are not empty, the sums of the chunks, and from these the token's logit and its
-// place among those that are equal to it; a last look at the row finds it.  A row that holds other logits (beyond 512, below 2^-32) is counted anew by that
-// block in windows of as many ranks as there are bins, from the largest logit on.  (Logits of -512 and below that weigh nothing, as masks of the
-// type's lowest value do, are no such others.)
+// last of them, or the only one, forms what each thread's run of bins holds and weighs, the sums up to each run, and from these, in up to three walks of one
+// wave, the token's logit and its place among those that are equal to it; a last look at the groups of the row that hold one as large finds it.  A row that
+// holds other logits (beyond 512, below 2^-32) is counted anew by that block in windows of as many ranks as there are bins, from the largest logit on.  (Logits
+// of -512 and below that weigh nothing, as masks of the type's lowest value do, are no such others.)
+// Many rows are bound by the counting and the bytes: an LDS atomic of a wave takes some 13 cycles where its lanes' bins are spread as logits spread them, 13 us
+// for a row of 152 000 tokens on a CU, whose share of the memory takes 15 for its bytes; 2000 rows 173 us (607 MB, 3.5 TB/s), 22 us a row on its CU.  Between
+// 257 and 512 rows some CUs have two rows and others one: 389 rows 42 us (118 MB, 2.8 TB/s).  A
+// single row is bound by steps that wait for each other: of 15 us for 151851 tokens the launch and the first bytes 3, the count 2.7, the pieces' meeting 2.5,
+// the largest logit 0.6, the weights 2.5, three walks 3.2, the token 1.4.  Sums of fixed-point weights (5.3 for the weights' 2.5), sums by
+// reductions over chunks of bins (5.3) and bins that are not empty dealt to lanes (5.4) were slower.
 template <uint32_t THREADS, uint32_t AHEAD>   // requests of 16 bytes that a lane has in flight
 __global__ __launch_bounds__(THREADS, 4) void sample_kernel(const SampleArgs a) {
     constexpr uint32_t WAVES = THREADS / 64, UNIT = 512 * AHEAD;   // tokens that a wave takes at a time
@@ -162,7 +168,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(const SampleArgs a) 
     __shared__ double wave_m[WAVES], wave_plain[WAVES], log_plain, reach;   // reach: how far below the largest min_p's border is
     __shared__ double ratio[2][kSampleSizes];       // of two weights, at T and at 1, whose logits of a size are next to each other
     __shared__ uint16_t list[kSampleGroups];
-    __shared__ uint32_t words[WAVES], odd, lower, flag, next, best_word, found_rank, found_bin, found_place, over;
+    __shared__ uint32_t words[WAVES], odd, lower, flag, next, best_word, found_rank, found_bin, found_place, found_held, of_wave[2][WAVES], over;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = blockIdx.y;
     const uint16_t* const x = a.logits + (size_t)row * a.row_stride;
     const uint32_t from = blockIdx.x * a.piece, left = a.vocab - from, to = from + (left < a.piece ? left : a.piece);
@@ -472,6 +478,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(const SampleArgs a) 
                     found_rank = rank;
                     found_bin = bin;
                     found_place = take;
+                    found_held = held;
                 }
                 wave_lds_order();
                 return true;
@@ -559,7 +566,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(const SampleArgs a) 
     if (tid == 0 && a.logprobs) a.logprobs[row] = (float)((best == 0 ? 0.0 : sample_value(found_rank) - r.top) - log_plain);
 
     // ---- the token: of those that hold the logit, in their order, the one at found_place; looked for in the groups that hold one as large ----
-    const uint32_t bin = found_bin, zero = found_rank == 0x7f80u, want = zero ? 0u : sample_bits(found_rank), mask = zero ? 0x7fffu : 0xffffu;
+    const uint32_t bin = found_bin, zero = found_rank == 0x7f80u, want = zero ? 0u : sample_bits(found_rank) * 0x10001u, mask = zero ? 0x7fff7fffu : ~0u;   // (both halves of a word)
     const int least_most = bin < ZERO ? (int)(kSampleSpan - 1u - bin) : bin < NEGATIVE ? 0 : ~(int)(bin - NEGATIVE);
     const bool may = tid < groups && (windows || most_of[tid] >= least_most);
     const unsigned long long may_all = __builtin_amdgcn_ballot_w64(may);
@@ -573,48 +580,63 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(const SampleArgs a) 
     }
     if (may) list[listed_before + (uint32_t)__builtin_popcountll(may_all & ((1ull << lane) - 1ull))] = (uint16_t)tid;
     __syncthreads();
-    uint32_t place = found_place;
-    const uint32_t units = (listed << a.group_shift) * AHEAD;   // of 512 tokens
-    constexpr uint32_t UNITS = 8;                               // of a wave at a time
-    for (uint32_t unit0 = 0; unit0 < units; unit0 += WAVES * UNITS) {
-        uint32_t w[UNITS][4], at[UNITS];
+    // (from the end that is nearer, if those that hold it lie as they fall: a logit that a whole row of 151851 holds took 17 us of the 55 of 389 rows from the
+    // first one on; a round's requests ahead of the one that is counted do not fit the registers)
+    const bool back = found_place > (found_held - 1u) / 2u;
+    uint32_t place = back ? found_held - 1u - found_place : found_place;
+    const uint32_t units = (listed << a.group_shift) * AHEAD, in = AHEAD << a.group_shift;   // of 512 tokens
+    constexpr uint32_t UNITS = 8;                                                            // of a wave at a time
+    auto at_unit = [&](uint32_t u) {   // this lane's first token of the u-th one
+        const uint32_t unit = back ? units - 1u - u : u;
+        return (uint32_t)list[unit / AHEAD >> a.group_shift] * (512u * in) + (unit & (in - 1u)) * 512u + lane * 8u;
+    };
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    auto differ = [&](const uint32_t (&w)[4]) __attribute__((always_inline)) {   // of this lane's eight, in two halves
+        u16x2 n = {0, 0};
 #pragma unroll
-        for (uint32_t i = 0; i < UNITS; ++i) {
-            const uint32_t unit = unit0 + wave * UNITS + i, in = AHEAD << a.group_shift;
-            at[i] = a.vocab;
-            if (unit < units) {
-                at[i] = (uint32_t)list[unit / AHEAD >> a.group_shift] * (512u * in) + (unit & (in - 1u)) * 512u + lane * 8u;
-                sample_load(x, at[i], a.vocab, w[i]);
+        for (int e = 0; e < 4; ++e) n += __builtin_elementwise_min(__builtin_bit_cast(u16x2, (w[e] & mask) ^ want), u16x2{1, 1});
+        return n;
+    };
+#pragma unroll 1
+    for (uint32_t unit0 = 0, turn = 0; unit0 < units; unit0 += WAVES * UNITS, turn ^= 1u) {
+        const uint32_t mine0 = unit0 + wave * UNITS, mine = mine0 < units ? min(units - mine0, UNITS) : 0u;   // units of this wave
+        uint32_t w[UNITS][4], all = 0;
+        if (mine) {
+#pragma unroll
+            for (uint32_t i = 0; i < UNITS; ++i) {
+                if (i < mine) sample_load(x, at_unit(mine0 + i), a.vocab, w[i]);
+                else w[i][0] = w[i][1] = w[i][2] = w[i][3] = 0xff80ff80u;
             }
-        }
-        uint32_t here[UNITS], mine = 0;
+            u16x2 other = {0, 0};
 #pragma unroll
-        for (uint32_t i = 0; i < UNITS; ++i) {
-            here[i] = 0;
-            if (at[i] >= a.vocab) continue;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) here[i] |= ((w[i][e] & mask) == want ? 1u : 0u) << (2 * e) | ((w[i][e] >> 16 & mask) == want ? 2u : 0u) << (2 * e);
-            mine += (uint32_t)__builtin_popcount(here[i]);
+            for (uint32_t i = 0; i < UNITS; ++i) other += differ(w[i]);
+            all = last_lane(wave_upto(8u * UNITS - other[0] - other[1]));
         }
-        const uint32_t all = last_lane(wave_upto(mine));
-        if (lane == 0) words[wave] = all;
+        if (lane == 0) of_wave[turn][wave] = all;
         __syncthreads();
         uint32_t before = 0, every = 0;
 #pragma unroll
         for (uint32_t i = 0; i < WAVES; ++i) {
-            before += i < wave ? words[i] : 0u;
-            every += words[i];
+            before += i < wave ? of_wave[turn][i] : 0u;
+            every += of_wave[turn][i];
         }
         if (place >= before && place < before + all) {
             uint32_t skip = place - before;
 #pragma unroll
             for (uint32_t i = 0; i < UNITS; ++i) {
-                const uint32_t n = (uint32_t)__builtin_popcount(here[i]), upto = wave_upto(n), unit_all = last_lane(upto);
+                const u16x2 o = differ(w[i]);
+                const uint32_t n = 8u - o[0] - o[1], upto = wave_upto(n), unit_all = last_lane(upto);
                 if (skip < unit_all) {
-                    if (skip >= upto - n && skip < upto) {
-                        uint32_t bits = here[i];
-                        for (uint32_t o = skip - (upto - n); o; --o) bits &= bits - 1u;
-                        a.tokens[row] = at[i] + (uint32_t)__builtin_ctz(bits);
+                    const uint32_t first = back ? unit_all - 1u - skip : skip;
+                    if (first >= upto - n && first < upto) {
+                        uint32_t bits = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t d = (w[i][e] & mask) ^ want;
+                            bits |= (d & 0xffffu ? 0u : 1u) << (2 * e) | (d >> 16 ? 0u : 2u) << (2 * e);
+                        }
+                        for (uint32_t o1 = first - (upto - n); o1; --o1) bits &= bits - 1u;
+                        a.tokens[row] = at_unit(mine0 + i) + (uint32_t)__builtin_ctz(bits);
                     }
                     break;
                 }
@@ -623,7 +645,6 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(const SampleArgs a) 
         }
         if (place < every) break;
         place -= every;
-        __syncthreads();
     }
 }
 
@@ -635,7 +656,7 @@ constexpr uint32_t kSampleMostVocab = 1u << 24;
 // every CU one block, 16 at most, of 8192 tokens at least.  us of 1, 16, 64 and 96 rows of some 151900 whole, in 2, 4, 8 and 16 pieces: 23.3, 20.2, 17.7, 16.5,
 // 15.6; 24.6, 21.4, 18.7, 17.9, 18.2; 28.1, 25.8, 24.4, 40.1, 64.5; 28.3, 26.4, 37.5, 52.9, 87.6; of 1 and 128 rows of 32000 whole and in 4 15.2, 15.3; 19.3, 33.9.
 // More rows: blocks of 512 threads, two on a CU, one of which counts while the other is at its last steps: 389 rows of 151851 55 us (1024 threads: 66), 512 of
-// 32000 23 (35).
+// 32000 23 (35).  Those whole: their bins meet in memory, 389 rows in 1 to 4 pieces 49, 63, 57 and 86 us.  (All before the token was looked for from the nearer end.)
 constexpr uint32_t kSampleWide = 256, kSampleWhole = 32768, kSampleMostPieces = 16, kSampleLeastPiece = 8192;
 struct SamplePlan {
     uint32_t pieces, piece, group_shift;

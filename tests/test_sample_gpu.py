@@ -272,3 +272,15 @@ def test_few_tokens_that_min_p_cuts(fk):
     for rows in (300, 20):
         Draw(fk, bits[:rows], min_p=r.uniform(0, 1, rows), temperature=10.0 ** r.uniform(-3, 2, rows), top_k=r.integers(0, 6, rows)).run().check()
         Draw(fk, bits[:rows], top_p=r.uniform(0, 1, rows), temperature=10.0 ** r.uniform(-3, 2, rows)).run().check()
+
+
+@pytest.mark.parametrize("rows,vocab,share", [(13, 40000, 0.3), (300, 9001, 0.5), (16, 70001, 0.001), (6, 262145, 0.6), (40, 1000, 1.0), (270, 70001, 0.4)])
+def test_places_among_equal_logits(fk, rows, vocab, share):
+    """From the first of those that hold a logit to the last: they are counted from the nearer end."""
+    bits = np.where(rng(71).random((rows, vocab)) < share, 0x4040, 0x4000).astype(np.uint16)      # 3 and 2
+    bits[:, ::97] = 0xFF80
+    u = np.linspace(0, 1, rows, endpoint=False, dtype=np.float32)
+    u[-1] = 1 - 2.0 ** -24
+    d = Draw(fk, bits, pad=1, seed=72, u=u, logprobs=False)
+    d.run().check()
+    Draw(fk, bits, seed=72, u=u[::-1].copy(), temperature=3.0, top_p=0.9).run().check()
