@@ -446,9 +446,10 @@ class PagedDecoder:
             raise OutOfPages(f"{need} pages wanted, {pages.free_pages} free")
         draws = np.stack([np.random.Generator(np.random.PCG64([seed, i])).random(max_tokens, np.float32) for i in range(n)], 1)
         ws = native.zeros(max(native.sample_workspace_bytes(r, c.vocab) for r in range(1, n + 1)))
+        free = DeviceBuffer(4 * pages.n_pages)
         seqs = [pages.new() for _ in prompts]
         try:
-            start = _Steps(self, ws, settings, draws[:1], [0] * n)
+            start = _Steps(self, ws, free, settings, draws[:1], [0] * n)
             for i, (s, p) in enumerate(zip(seqs, prompts)):
                 start.draw(self.prefill(s, p), 0, i, 1)
             out = [[int(t)] for t in start.finish()[0]]
@@ -458,7 +459,7 @@ class PagedDecoder:
                     return out
                 done = len(out[live[0]])                       # (all that live have as many)
                 count = min(max_tokens - done, max_tokens if eos is None else self.LOOK)
-                steps = _Steps(self, ws, [v[live] for v in settings], draws[done:done + count, live], [out[i][-1] for i in live], [seqs[i] for i in live])
+                steps = _Steps(self, ws, free, [v[live] for v in settings], draws[done:done + count, live], [out[i][-1] for i in live], [seqs[i] for i in live])
                 for j in range(count):
                     steps.run(j)
                 for row in steps.finish():
@@ -475,22 +476,27 @@ class PagedDecoder:
 class _Steps:
     """Steps of PagedDecoder.sample for a number of sequences, one row each: what they read and write lies on the device, in one piece."""
 
-    def __init__(self, dec: PagedDecoder, ws: DeviceBuffer, settings, draws: np.ndarray, tokens: Sequence[int], seqs: Sequence[PagedSequence] = ()):
-        """settings: temperature, top_k, top_p and min_p of each sequence; draws: random numbers [steps, sequences]; tokens: what the first step reads."""
+    def __init__(self, dec: PagedDecoder, ws: DeviceBuffer, free: DeviceBuffer, settings, draws: np.ndarray, tokens: Sequence[int],
+                 seqs: Sequence[PagedSequence] = ()):
+        """free: room for the stack of free pages; settings: temperature, top_k, top_p and min_p of each sequence; draws: random numbers
+        [steps, sequences]; tokens: what the first step reads."""
         pages = dec.pages
         self.dec, self.ws, self.seqs, self.shape = dec, ws, list(seqs), draws.shape
         self.longest = max([s.length for s in seqs], default=0)
         self.stride = -(-(self.longest + len(draws)) // pages.page_rows)
         parts = [*settings, draws, tokens, np.zeros(draws.shape, np.uint32),                       # (the tokens drawn lie behind those read first)
-                 [s.length for s in seqs], pages.table(seqs, self.stride), pages._free + [0] * (pages.n_pages - len(pages._free)), [len(pages._free)],
-                 [0], np.zeros(len(seqs) + 1, np.uint32), np.zeros(len(seqs), np.uint32), np.zeros((len(seqs), self.stride), np.uint32)]
+                 [s.length for s in seqs], pages.table(seqs, self.stride), [pages.free_pages], [0],
+                 np.zeros(len(seqs) + 1, np.uint32), np.zeros(len(seqs), np.uint32), np.zeros((len(seqs), self.stride), np.uint32)]
         words = [(a if isinstance(a, np.ndarray) and a.dtype == np.float32 else np.asarray(a, np.uint32)).ravel().view(np.uint32) for a in parts]
         self.mem = DeviceBuffer.from_numpy(np.concatenate(words))
         self.at = np.concatenate([[0], np.cumsum([4 * len(w) for w in words])]).tolist()
         place = [self.mem.ptr + a for a in self.at]
         self.settings, self.draws, self.tokens = place[:4], place[4], place[5]
         if seqs:
-            lengths, tables, free, n_free, counter, *self.batch = place[7:15]
+            lengths, tables, n_free, counter, *self.batch = place[7:14]
+            need = sum(-(-(s.length + len(draws)) // pages.page_rows) - len(s.pages) for s in seqs)
+            if need:                                           # (of the stack the steps read no more)
+                free.upload(np.asarray(pages._free[-need:], np.uint32), 4 * (pages.free_pages - need))
             self.requests = native.PagedRequests(None, None, len(seqs), lengths, lengths, tables, self.stride, free, n_free, n_free, counter)
 
     def draw(self, logits, step: int, row: int, rows: int) -> None:
@@ -513,5 +519,5 @@ class _Steps:
         words = self.mem.to_numpy(np.uint32)
         part = lambda i: words[at[i] // 4:at[i + 1] // 4]
         if self.seqs:
-            dec.pages.adopt(self.seqs, part(7), part(8).reshape(-1, self.stride), int(part(10)[0]))
+            dec.pages.adopt(self.seqs, part(7), part(8).reshape(-1, self.stride), int(part(9)[0]))
         return part(6).reshape(self.shape)

@@ -152,9 +152,9 @@ def test_a_captured_round(fk, models, stream):  # noqa: F811
     seqs = [d.pages.new() for _ in prompts]
     for s, p in zip(seqs, prompts):
         d.prefill(s, p)
-    ws = fk.zeros(fk.sample_workspace_bytes(4, cfg.vocab))
+    ws, free = fk.zeros(fk.sample_workspace_bytes(4, cfg.vocab)), fk.DeviceBuffer(4 * d.pages.n_pages)
     draws = [rng(i).random((count, 4), np.float32) for i in range(3)]
-    make = lambda u: _Steps(d, ws, settings, u, [5, 6, 7, 8], seqs)
+    make = lambda u: _Steps(d, ws, free, settings, u, [5, 6, 7, 8], seqs)
 
     def run(steps):
         for j in range(count):
