@@ -179,14 +179,27 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(const SampleArgs a) 
 
     // ---- the piece's logits, counted ----
     auto count_all = [&](uint32_t begin, uint32_t end, auto&& ready, auto&& each) __attribute__((always_inline)) {   // ready(): behind the first requests
-        for (uint32_t at0 = begin; at0 < end; at0 += WAVES * UNIT) {
-            const uint32_t unit = at0 + wave * UNIT;
-            uint32_t w[AHEAD][4];
-            if (unit < end)   // (all of a wave's lanes; -inf behind the row)
+        auto request = [&](uint32_t unit, uint32_t (&w)[AHEAD][4]) __attribute__((always_inline)) {   // (-inf behind the row)
 #pragma unroll
-                for (uint32_t i = 0; i < AHEAD; ++i) sample_load(x, unit + i * 512u + lane * 8u, a.vocab, w[i]);
-            if (at0 == begin) ready();
-            if (unit < end) each(unit, w);
+            for (uint32_t i = 0; i < AHEAD; ++i) sample_load(x, unit + i * 512u + lane * 8u, a.vocab, w[i]);
+        };
+        // (a request of 16 bytes a lane is followed by the next before it is counted: 200 rows from memory 37 us without, 33 with; of four there are enough)
+        constexpr bool TWO = AHEAD == 1;
+        uint32_t w[AHEAD][4], behind[AHEAD][4];
+        uint32_t unit = begin + wave * UNIT;   // (all of a wave's lanes)
+        if (unit < end) request(unit, w);
+        ready();
+        while (unit < end) {
+            const uint32_t next = unit + WAVES * UNIT;
+            if (TWO && next < end) request(next, behind);
+            each(unit, w);
+            if (TWO)
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[i][e] = behind[i][e];
+            else if (next < end) request(next, w);
+            unit = next;
         }
     };
     double by = 0.0;
