@@ -149,9 +149,9 @@ __device__ __forceinline__ void sample_load(const uint16_t* x, uint32_t at, uint
 // wave, the token's logit and its place among those that are equal to it; a last look at the groups of the row that hold one as large finds it.  A row that
 // holds other logits (beyond 512, below 2^-32) is counted anew by that block in windows of as many ranks as there are bins, from the largest logit on.  (Logits
 // of -512 and below that weigh nothing, as masks of the type's lowest value do, are no such others.)
-// Many rows are bound by the counting and the bytes: an LDS atomic of a wave takes some 13 cycles where its lanes' bins are spread as logits spread them, 13 us
-// for a row of 152 000 tokens on a CU, whose share of the memory takes 15 for its bytes; 2000 rows 173 us (607 MB, 3.5 TB/s), 22 us a row on its CU.  Between
-// 257 and 512 rows some CUs have two rows and others one: 389 rows 42 us (118 MB, 2.8 TB/s).  A
+// Many rows are bound by a CU's units, none of which works all the time: for a row of 152 000 tokens that spread as logits do its LDS takes 8 us (8 cycles a
+// wave's atomic, two thirds of them bank conflicts), its vector instructions 10 and its share of the memory 15; 2000 rows 175 us (607 MB, 3.5 TB/s), 22 us a row
+// on its CU.  Between 257 and 512 rows some CUs have two rows and others one: 389 rows 43 us from the last-level cache, 50 from memory (118 MB, 2.4 TB/s).  A
 // single row is bound by steps that wait for each other: of 15 us for 151851 tokens the launch and the first bytes 3, the count 2.7, the pieces' meeting 2.5,
 // the largest logit 0.6, the weights 2.5, three walks 3.2, the token 1.4.  Sums of fixed-point weights (5.3 for the weights' 2.5), sums by
 // reductions over chunks of bins (5.3) and bins that are not empty dealt to lanes (5.4) were slower.

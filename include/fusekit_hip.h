@@ -655,9 +655,9 @@ fk_status fk_sdpa_paged_sinks(const uint16_t *q, uint32_t q_stride, uint16_t *ou
  * the lengths that the requests have, so that a decode loop, or a captured graph of one step, goes on without the host.  Requests keep their length and
  * their pages in slots (a row of `tables` each); the batch names the slots that run and how many new rows each has.  Sequence i gets the pages that
  * its new rows need, from the top of the stack free_pages[0 .. *n_free - 1] on in the sequences' order, at the end of its row of `tables`, and a copy of that
- * row in batch->page_table (as many entries as it has pages; what is behind stays as it is).  row_slots (may be NULL): new row r lies in row row_slots[r] of the pool, its page
- * times page_rows + its row there (rows behind the last stay as they are).  lengths_out and n_free_out are what is then held and free; they may be lengths
- * and n_free.  A slot's last page, where it is partly filled, must be its own (fork: fk_pages_copy).
+ * row in batch->page_table (as many entries as it has pages; what is behind stays as it is).  row_slots (may be NULL): new row r lies in row row_slots[r] of
+ * the pool, its page times page_rows + its row there (rows behind the last stay as they are).  lengths_out and n_free_out are what is then held and free;
+ * they may be lengths and n_free.  A slot's last page, where it is partly filled, must be its own (fork: fk_pages_copy).
  * All or nothing: where a slot, a count of rows, a length or the free pages do not fit, no sequence has a new row, kv_len is 0, tables, lengths and free
  * pages stay as they were, and bits of *batch->fault say why.  What is written overlaps nothing else. */
 typedef struct fk_paged_requests {
