@@ -264,6 +264,8 @@ constexpr int kPastCaches = 16;   // (sc1: what another block wrote, or is to re
 
 // What a tile's columns e_tile .. e_last see, in steps of STEP positions, and how its items share them: item i takes `per` of the `steps` from i * per on.
 // The steps are counted without those that lie between the sinks and the window: step number n is n, from `near` on n + gap.
+// (Sinks cost their own steps: 64 tokens of up to 20000 positions, 32 / 8 heads x 128, with a window of 4096 and 100 of them 118 us, 115 without; two chunks of
+// 2048 rows with as wide a window and 128 of them 302, 289 without.)
 struct PagedRange {
     uint32_t kv_end, steps, per, n_active;   // n_active: items that have steps, one at least
     uint32_t near, gap;

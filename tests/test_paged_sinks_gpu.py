@@ -160,3 +160,9 @@ def test_replays_while_lengths_grow(fk, stream):  # noqa: F811
         off = np.abs(wide(out.to_numpy(np.uint16, q.shape)) - ref) - (2.0 ** -8 * np.abs(ref) + (2.0 ** -8 + 2.0 ** -11) * size)
         assert off.max() <= 0, lens
     g.free()
+
+
+@pytest.mark.parametrize("window,sinks", [(2 ** 32 - 1, 2 ** 32 - 1), (2 ** 32 - 1, 7), (1, 2 ** 32 - 1), (1, 2 ** 31), (599, 1), (600, 1), (2 ** 31, 2 ** 31 + 1)])
+def test_windows_and_sinks_of_any_size(fk, window, sinks):
+    check(fk, Paged([1, 1, 0], [600, 1, 5], 2, 64, 16, seed=8), 8, window, sinks)
+    check(fk, Paged([90, 1], [600, 30], 2, 128, 32, seed=9), 8, window, sinks)
