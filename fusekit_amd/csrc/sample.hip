@@ -409,19 +409,21 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(const SampleArgs a) 
             const double w0 = ratio[0][size0], w1 = ratio[0][size1], one0 = ratio[1][size0], one1 = ratio[1][size1];
             const double first = above ? r.top : sample_value(rank_of(bin0, base));
             const int at = (int)SampleBins<THREADS>::place(bin0), step = positive ? -1 : 1;
-            // (from the last one on: each sum times the ratio, and the next count)
-            all = hist[at + step * (int)(RUN - 1u)];
-            m = p = (double)all;
+            uint32_t n[RUN];
 #pragma unroll
-            for (int i = (int)RUN - 2; i >= 0; --i) {
-                const uint32_t n = hist[at + step * i];
-                const bool near = (uint32_t)i < border, over = (uint32_t)i < above;
-                all += n;
-                m = fma(m, over ? 1.0 : near ? w0 : w1, (double)n);
-                p = fma(p, over ? 1.0 : near ? one0 : one1, (double)n);
+            for (uint32_t i = 0; i < RUN; ++i) all += n[i] = hist[at + step * (int)i];
+            if (__builtin_amdgcn_ballot_w64(all != 0)) {   // (of 82 sizes of both signs a row fills some 25)
+                // (from the last one on: each sum times the ratio, and the next count)
+                m = p = (double)n[RUN - 1u];
+#pragma unroll
+                for (int i = (int)RUN - 2; i >= 0; --i) {
+                    const bool near = (uint32_t)i < border, over = (uint32_t)i < above;
+                    m = fma(m, over ? 1.0 : near ? w0 : w1, (double)n[i]);
+                    p = fma(p, over ? 1.0 : near ? one0 : one1, (double)n[i]);
+                }
+                m *= sample_exp2(fmax((first - r.top) * r.by, -2000.0));
+                p *= sample_exp2(fmax((first - r.top) * kSampleLog2E, -2000.0));
             }
-            m *= sample_exp2(fmax((first - r.top) * r.by, -2000.0));
-            p *= sample_exp2(fmax((first - r.top) * kSampleLog2E, -2000.0));
         } else {
 #pragma unroll 1
             for (uint32_t i = 0; i < RUN; ++i) {
@@ -433,8 +435,13 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(const SampleArgs a) 
                 p = fma((double)n, r.plain(v), p);
             }
         }
-        const uint32_t n_upto = wave_upto(all);
-        const double m_upto = wave_upto(m), p_upto = wave_upto(p);
+        uint32_t n_upto = 0;
+        double m_upto = 0.0, p_upto = 0.0;
+        if (__builtin_amdgcn_ballot_w64(all != 0)) {
+            n_upto = wave_upto(all);
+            m_upto = wave_upto(m);
+            p_upto = wave_upto(p);
+        }
         count_upto[tid] = n_upto;
         mass_upto[tid] = m_upto;
         if (lane == 63u) {
